@@ -278,6 +278,159 @@ RMOE_API rmoe_status rmoe_gguf_meta_uint(const rmoe_gguf* g, const char* key, ui
  * points into the mapping: pass it to rmoe_layer_create before rmoe_gguf_close. */
 RMOE_API rmoe_status rmoe_gguf_moe_layer_desc(rmoe_gguf* g, uint32_t block, rmoe_layer_desc* out);
 
+/* ---- serving the block around the layer: an 8-bit paged KV cache and its attention ---------
+ *
+ * Element types of q / k / v / out are ggml codes: RMOE_GGML_F32, _F16 or _BF16.  All tensors
+ * below are device memory of the handle's device; every call is stream-ordered and waits for
+ * nothing.  rusty-engine's PagedKvCache (src/infer.rs:328) holds f32 rows and is not read by its
+ * forward; its attention (src/forward.rs:218-283) and RoPE (src/infer.rs:90-145) are the formulas
+ * these calls compute, over a cache held in 8 bits. */
+
+/* Rotary positions.  Pair i < rot_dim / 2 of a head is (x[i], x[i + rot_dim / 2]) in the half
+ * layout, (x[2i], x[2i + 1]) in the interleaved one; it is turned by the angle pos * f_i and
+ * scaled by m:  y0 = x0 c - x1 s, y1 = x1 c + x0 s  with c, s = m cos, m sin.  Elements from
+ * rot_dim on are copied.  f_i = base^(-2i / rot_dim), then
+ *   RMOE_ROPE_LINEAR: f_i / factor;
+ *   RMOE_ROPE_YARN:   f_i (1 - g_i) / factor + f_i g_i with g_i falling from 1 to 0 between the
+ *                     pairs that make beta_fast and beta_slow turns in orig_ctx positions
+ *                     (arXiv 2309.00071, section 3), and m = 0.1 ln(factor) + 1;
+ * and divided by freq_factors[i] where given (a model file's rope_freqs tensor). */
+enum { RMOE_ROPE_INTERLEAVED = 0, RMOE_ROPE_HALF = 1 };
+enum { RMOE_ROPE_PLAIN = 0, RMOE_ROPE_LINEAR = 1, RMOE_ROPE_YARN = 2 };
+
+typedef struct {
+    uint32_t rot_dim;          /* even, >= 2 */
+    uint32_t layout;           /* RMOE_ROPE_INTERLEAVED / _HALF */
+    uint32_t scaling;          /* RMOE_ROPE_PLAIN / _LINEAR / _YARN */
+    uint32_t max_pos;          /* positions 0 .. max_pos - 1 */
+    double base;               /* > 0 */
+    double factor;             /* >= 1 with LINEAR / YARN */
+    double beta_fast, beta_slow; /* YARN; 0 = 32 and 1 */
+    double mscale;             /* factor of cos and sin; 0 = the scaling's own */
+    const float* freq_factors; /* host, rot_dim / 2 values, or null */
+    uint32_t orig_ctx;         /* YARN: positions the model was trained on */
+    int32_t device;
+} rmoe_rope_desc;
+
+typedef struct rmoe_rope rmoe_rope;
+
+/* Makes the table of (cos, sin) f32 pairs for every position and pair, computed on the device in
+ * 64 bits and rounded once (8 * max_pos * rot_dim / 2 bytes, owned by the handle). */
+RMOE_API rmoe_status rmoe_rope_create(const rmoe_rope_desc* desc, rmoe_rope** out);
+RMOE_API void rmoe_rope_destroy(rmoe_rope* rope);
+
+/* Heads of T tokens: element (t, h, i) at data[t * stride_t + h * stride_h + i], strides in
+ * elements (16-byte aligned data and strides take the vector path; any others work). */
+typedef struct {
+    void* data;
+    int64_t stride_t, stride_h;
+    uint32_t heads;
+    uint32_t pad;
+} rmoe_rows;
+
+/* Turns q (and k where k.heads > 0) of T tokens by positions[t] (inverse != 0: back, by the
+ * negated angles: the transpose, which is also the gradient where m = 1).  In place where
+ * q_out.data == q.data with the same strides.  A position outside the table sets the handle's
+ * status word and leaves its token unturned. */
+typedef struct {
+    rmoe_rows q, q_out, k, k_out;
+    const int32_t* positions;
+    uint32_t T, head_dim, type, inverse;
+} rmoe_rope_args;
+RMOE_API rmoe_status rmoe_rope_apply(rmoe_rope* rope, const rmoe_rope_args* args, void* stream);
+/* Device errors of the calls so far; synchronises with the device and clears the word. */
+RMOE_API rmoe_status rmoe_rope_status(rmoe_rope* rope);
+
+/* Block tables and slot maps from request lengths, on the GPU: request r holds lens[r] tokens in
+ * blocks table[r][0 .. ceil(lens[r] / block_size)) and adds new_lens[r] (negative counts as 0).
+ *   cu[R + 1]: exclusive prefix sums of the new lengths (the batch's token layout);
+ *   new blocks are popped off the stack free_list[0 .. *n_free) in request order and written to
+ *   the table; a request whose blocks do not all fit in what is left, whose table row would
+ *   overflow, or whose tokens would lie past T, gets none and keeps its length (so do later ones
+ *   that need a block once the stack ran out);
+ *   lens_out, n_free_out: the lengths and the stack height afterwards;
+ *   positions[t] = lens[r] + i and slots[t] = block * block_size + position % block_size of
+ *   token t = cu[r] + i; slots of refused requests and past cu[R] are -1, positions past it 0.
+ * lens_out / n_free_out may not alias lens / n_free.  block_size: 16, 32, 64 or 128; R at most
+ * 16384. */
+typedef struct {
+    int32_t* table;
+    const int32_t *lens, *new_lens, *free_list, *n_free;
+    int32_t *cu, *positions, *slots, *lens_out, *n_free_out;
+    uint32_t R, max_blocks, T, block_size, free_cap, pad;
+} rmoe_kv_extend_args;
+RMOE_API rmoe_status rmoe_kv_extend(const rmoe_kv_extend_args* args, void* stream);
+
+/* Requests that ended: the blocks of every r with done[r] != 0 go back on the stack in request
+ * and block order, its table row becomes -1 and its length 0. */
+typedef struct {
+    int32_t *table, *lens, *free_list;
+    const int32_t *done, *n_free;
+    int32_t* n_free_out;
+    uint32_t R, max_blocks, block_size, free_cap;
+} rmoe_kv_release_args;
+RMOE_API rmoe_status rmoe_kv_release(const rmoe_kv_release_args* args, void* stream);
+
+/* The cache: codes [n_blocks][n_kv_heads][block_size][head_dim], 8 bits each, and one f32 scale
+ * per block and head ([n_blocks][n_kv_heads]) for K and for V; a cached value is code * scale. */
+enum { RMOE_KV_INT8 = 0, RMOE_KV_E4M3 = 1 };
+
+typedef struct {
+    uint32_t n_blocks, block_size, n_kv_heads, head_dim; /* head_dim 64, 128 or 256 */
+    uint32_t code;                                       /* RMOE_KV_INT8 / _E4M3 */
+    int32_t device;
+    void *k, *v;             /* the caller's memory (16-byte aligned), or all four null: the handle */
+    float *k_scale, *v_scale;/* allocates them, zeroed */
+} rmoe_kv_desc;
+
+typedef struct rmoe_kv rmoe_kv;
+RMOE_API rmoe_status rmoe_kv_create(const rmoe_kv_desc* desc, rmoe_kv** out);
+RMOE_API void rmoe_kv_destroy(rmoe_kv* kv);
+/* The memory in use (desc->k, v, k_scale, v_scale are filled). */
+RMOE_API rmoe_status rmoe_kv_buffers(const rmoe_kv* kv, rmoe_kv_desc* desc);
+/* Device errors of the calls so far (a slot, block or position out of range, a K / V value that is
+ * not finite, a timed-out wait); synchronises with the device and clears the word. */
+RMOE_API rmoe_status rmoe_kv_status(rmoe_kv* kv);
+
+/* Writes T tokens' keys and values at slots[t] (-1: skipped).  Tokens of one block are given as
+ * one run of consecutive slots; the slots before a run in its block hold the request's earlier
+ * tokens.  Per run and head: s = max(scale of the block if it holds earlier tokens, max|x| / 127
+ * (448 for e4m3)), codes round(x / s) to nearest even; where s grew, the earlier codes are
+ * rounded again to the new scale.  NaN is stored as 0 and infinities as the largest code, and
+ * both set the status word.  With rope, k is turned by positions[t] first (in f32), and where
+ * q.heads > 0 so is q into q_out. */
+typedef struct {
+    rmoe_rows k, v, q, q_out;
+    const int32_t *slots, *positions;
+    rmoe_rope* rope;
+    uint32_t T, type;
+} rmoe_kv_append_args;
+RMOE_API rmoe_status rmoe_kv_append(rmoe_kv* kv, const rmoe_kv_append_args* args, void* stream);
+
+/* Cached values code * scale of n slots, as [n][n_kv_heads][head_dim] of `type` (a slot of -1
+ * gives zeros): for code that wants plain keys and values, or to move a request elsewhere. */
+RMOE_API rmoe_status rmoe_kv_read(rmoe_kv* kv, const int32_t* slots, uint32_t n, uint32_t type, void* k_out,
+                                  void* v_out, void* stream);
+
+/* Attention of T query tokens over the cache (src/forward.rs:218-283, for R requests at once):
+ * request r has lens[r] cached tokens, the queries of tokens cu[r] .. cu[r + 1) being those of its
+ * last positions; query at position p sees keys max(0, p - window + 1) .. p (window 0: from 0),
+ * query head h reads kv head h / (q heads / kv heads).
+ *   out[t][h] = sum_j softmax_j(scale q.k_j) v_j ;  lse[t][h] = ln sum_j exp(scale q.k_j)
+ * (lse, natural logarithm, optional: [T][q heads] f32).  A row that sees no key gives 0 and
+ * -infinity, as do tokens past cu[R].  max_new: an upper bound of the new tokens of any request
+ * where the caller knows one (0: unknown); it only chooses kernels.  f32 calls carry q and the
+ * probabilities as pairs of fp16; codes are exact in fp16. */
+typedef struct {
+    rmoe_rows q, out;
+    const int32_t *table, *lens, *cu;
+    float* lse;
+    uint32_t R, max_blocks, T, type;
+    float scale;
+    uint32_t window, max_new, pad;
+} rmoe_kv_attend_args;
+RMOE_API rmoe_status rmoe_kv_attend(rmoe_kv* kv, const rmoe_kv_attend_args* args, void* stream);
+
 /* Self-test of the tensor-core kernels' bounded waits (no counterpart in the reference): one
  * CTA on `device` allocates tensor memory, waits on an mbarrier that nothing arrives at with a
  * limit of limit_us (1 .. 1000000) instead of the kernels' 1 s, then records DERR_TIMEOUT,

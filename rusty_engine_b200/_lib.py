@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -48,6 +49,32 @@ class LayerDesc(C.Structure):
     ]
 
 
+class RopeDesc(C.Structure):
+    _fields_ = [
+        ("rot_dim", C.c_uint32), ("layout", C.c_uint32), ("scaling", C.c_uint32), ("max_pos", C.c_uint32),
+        ("base", C.c_double), ("factor", C.c_double), ("beta_fast", C.c_double), ("beta_slow", C.c_double),
+        ("mscale", C.c_double), ("freq_factors", C.c_void_p), ("orig_ctx", C.c_uint32), ("device", C.c_int32),
+    ]
+
+
+class KvDesc(C.Structure):
+    _fields_ = [
+        ("n_blocks", C.c_uint32), ("block_size", C.c_uint32), ("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+        ("code", C.c_uint32), ("device", C.c_int32),
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+    ]
+
+
+# The argument blocks of the per-token calls, packed in one step (a ctypes Structure would be
+# filled field by field on every call).  P: pointer, q: int64 stride, I: uint32, f: float; an
+# rmoe_rows is "PqqII" (data, token stride, head stride, heads, padding).
+_ROWS = "PqqII"
+ROPE_ARGS = struct.Struct("@" + 4 * _ROWS + "PIIII")              # rmoe_rope_args
+KV_EXTEND_ARGS = struct.Struct("@PPPPPPPPPPIIIIII")               # rmoe_kv_extend_args
+KV_RELEASE_ARGS = struct.Struct("@PPPPPPIIII")                    # rmoe_kv_release_args
+KV_APPEND_ARGS = struct.Struct("@" + 4 * _ROWS + "PPPII")         # rmoe_kv_append_args
+KV_ATTEND_ARGS = struct.Struct("@" + 2 * _ROWS + "PPPPIIIIfIII")  # rmoe_kv_attend_args
+
 # Every symbol include/rmoe.h declares (the tests check the library exports all of them).
 EXPORTS = [
     "rmoe_layer_create", "rmoe_layer_forward", "rmoe_layer_routing", "rmoe_layer_logits", "rmoe_layer_destroy",
@@ -56,6 +83,9 @@ EXPORTS = [
     "rmoe_route_grouped", "rmoe_qmat_create", "rmoe_qmat_forward", "rmoe_qmat_status", "rmoe_qmat_destroy",
     "rmoe_gguf_open", "rmoe_gguf_close", "rmoe_gguf_tensor", "rmoe_gguf_meta_uint", "rmoe_gguf_moe_layer_desc",
     "rmoe_layer_router_refined", "rmoe_noalloc_status", "rmoe_selftest_bounded_wait",
+    "rmoe_rope_create", "rmoe_rope_destroy", "rmoe_rope_apply", "rmoe_rope_status",
+    "rmoe_kv_create", "rmoe_kv_destroy", "rmoe_kv_buffers", "rmoe_kv_status", "rmoe_kv_extend", "rmoe_kv_release",
+    "rmoe_kv_append", "rmoe_kv_read", "rmoe_kv_attend",
 ]
 
 NOALLOC_SCRATCH_BYTES = 8 << 20  # RMOE_NOALLOC_SCRATCH_BYTES
@@ -105,6 +135,21 @@ def load():
         L.rmoe_gguf_tensor.argtypes = [vp, C.c_char_p, C.POINTER(Tensor)]
         L.rmoe_gguf_meta_uint.argtypes = [vp, C.c_char_p, C.POINTER(u64)]
         L.rmoe_gguf_moe_layer_desc.argtypes = [vp, u32, C.POINTER(LayerDesc)]
+        L.rmoe_rope_create.argtypes = [C.POINTER(RopeDesc), C.POINTER(vp)]
+        L.rmoe_rope_destroy.argtypes = [vp]
+        L.rmoe_rope_destroy.restype = None
+        L.rmoe_rope_apply.argtypes = [vp, vp, vp]
+        L.rmoe_rope_status.argtypes = [vp]
+        L.rmoe_kv_create.argtypes = [C.POINTER(KvDesc), C.POINTER(vp)]
+        L.rmoe_kv_destroy.argtypes = [vp]
+        L.rmoe_kv_destroy.restype = None
+        L.rmoe_kv_buffers.argtypes = [vp, C.POINTER(KvDesc)]
+        L.rmoe_kv_status.argtypes = [vp]
+        L.rmoe_kv_extend.argtypes = [vp, vp]
+        L.rmoe_kv_release.argtypes = [vp, vp]
+        L.rmoe_kv_append.argtypes = [vp, vp, vp]
+        L.rmoe_kv_read.argtypes = [vp, vp, u32, u32, vp, vp, vp]
+        L.rmoe_kv_attend.argtypes = [vp, vp, vp]
         for name in EXPORTS:
             fn = getattr(L, name)
             if fn.restype is C.c_int or name in ("rmoe_layer_create",):

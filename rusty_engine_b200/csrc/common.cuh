@@ -36,7 +36,9 @@ __host__ __device__ __forceinline__ int kperm_pos(int i) { return (i & ~3) | ((i
 
 // Status word bits written by kernels when a device-side check fails (never trap).
 enum DevErr : uint32_t { DERR_NONE = 0, DERR_BAD_EXPERT = 1, DERR_ROWS_OVERFLOW = 2, DERR_TILES_OVERFLOW = 4,
-                         DERR_TIMEOUT = 8, DERR_FP16_RANGE = 16 };
+                         DERR_TIMEOUT = 8, DERR_FP16_RANGE = 16,
+                         DERR_INDEX = 32,       // a slot, block or position out of range
+                         DERR_NONFINITE = 64 }; // a cached value that is not finite
 
 // Rows of SwiGLU activations are stored as fp16 * 2^e per 64-feature block (tensor-core and
 // small-batch kernels) or per 16-feature block (the decode GEMV kernels).

@@ -1,0 +1,246 @@
+// rope.cu -- rotary positions: the table of cosines and sines, and turning q and k by it.
+//
+// Pair i of a head is turned by pos * f_i.  At position 1e5 an f32 product carries an error of
+// several milliradians, so the angles are formed in 64 bits, once, when the handle is made, and
+// cos and sin are rounded to f32 there; a call reads 4 * rot_dim bytes of table per token against
+// (q heads + k heads) * head_dim elements of data (3% more traffic at 36 heads of 128 in bf16).
+#include <math.h>
+
+#include <vector>
+
+#include "rope.cuh"
+
+namespace rmoe {
+
+__global__ void __launch_bounds__(256) rope_table_kernel(float2* table, const double* freq, int pairs, uint64_t n,
+                                                         double m) {
+    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += gridDim.x * 256ull) {
+        double s, c;
+        sincos((double)(i / pairs) * freq[i % pairs], &s, &c);
+        table[i] = make_float2((float)(c * m), (float)(s * m));
+    }
+}
+
+// One thread per unit of 16 elements (rope.cuh); a token's units are neighbours, q heads first.
+template <typename T>
+__global__ void __launch_bounds__(256) rope_units_kernel(Rows q, Rows qo, Rows k, Rows ko, RopeArg ra, int T_, int dim,
+                                                         unsigned* status) {
+    const int per_head = dim / 16, per_tok = (q.heads + k.heads) * per_head;
+    const uint64_t n = (uint64_t)T_ * per_tok;
+    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += gridDim.x * 256ull) {
+        const int t = (int)(i / per_tok), r = (int)(i - (uint64_t)t * per_tok), h = r / per_head, u = r - h * per_head;
+        const bool isq = h < q.heads;
+        const Rows& in = isq ? q : k;
+        const Rows& out = isq ? qo : ko;
+        const int hh = isq ? h : h - q.heads;
+        const T* x = reinterpret_cast<const T*>(in.p) + t * in.st + hh * in.sh;
+        T* y = reinterpret_cast<T*>(out.p) + t * out.st + hh * out.sh;
+        int a, b;
+        unit_chunks(u, ra.rot, ra.half, a, b);
+        float v[16];
+        load8(x + a, in.vec, v);
+        load8(x + b, in.vec, v + 8);
+        const int p = __ldg(ra.pos + t);
+        if ((unsigned)p < (unsigned)ra.max_pos)
+            turn_unit(v, u, ra.table + (size_t)p * (ra.rot / 2), ra.rot, ra.half, ra.sign);
+        else if (u == 0 && h == 0)
+            atomicOr(status, (unsigned)DERR_INDEX);
+        store8(y + a, out.vec, v);
+        store8(y + b, out.vec, v + 8);
+    }
+}
+
+// Head and rotary sizes that are not multiples of 16: one thread per pair, then per copied element.
+template <typename T>
+__global__ void __launch_bounds__(256) rope_pairs_kernel(Rows q, Rows qo, Rows k, Rows ko, RopeArg ra, int T_, int dim,
+                                                         unsigned* status) {
+    const int per_head = ra.rot / 2 + (dim - ra.rot), per_tok = (q.heads + k.heads) * per_head;
+    const uint64_t n = (uint64_t)T_ * per_tok;
+    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += gridDim.x * 256ull) {
+        const int t = (int)(i / per_tok), r = (int)(i - (uint64_t)t * per_tok), h = r / per_head, u = r - h * per_head;
+        const bool isq = h < q.heads;
+        const Rows& in = isq ? q : k;
+        const Rows& out = isq ? qo : ko;
+        const int hh = isq ? h : h - q.heads;
+        const T* x = reinterpret_cast<const T*>(in.p) + t * in.st + hh * in.sh;
+        T* y = reinterpret_cast<T*>(out.p) + t * out.st + hh * out.sh;
+        if (u >= ra.rot / 2) {
+            const int e = u + ra.rot / 2;
+            y[e] = x[e];
+            continue;
+        }
+        const int a = ra.half ? u : 2 * u, b = ra.half ? u + ra.rot / 2 : 2 * u + 1;
+        float x0 = Elt<T>::get(x[a]), x1 = Elt<T>::get(x[b]);
+        const int p = __ldg(ra.pos + t);
+        if ((unsigned)p < (unsigned)ra.max_pos) {
+            const float2 cs = __ldg(ra.table + (size_t)p * (ra.rot / 2) + u);
+            turn(x0, x1, cs.x, ra.sign * cs.y);
+        } else if (u == 0 && h == 0) {
+            atomicOr(status, (unsigned)DERR_INDEX);
+        }
+        y[a] = Elt<T>::put(x0);
+        y[b] = Elt<T>::put(x1);
+    }
+}
+
+template <typename T>
+static cudaError_t rope_launch(const Rows& q, const Rows& qo, const Rows& k, const Rows& ko, const RopeArg& ra, int T_,
+                               int dim, unsigned* status, cudaStream_t s) {
+    const bool units = dim % 16 == 0 && ra.rot % 16 == 0;
+    const uint64_t n = (uint64_t)T_ * (q.heads + k.heads) * (units ? dim / 16 : dim - ra.rot / 2);
+    const unsigned grid = (unsigned)((n + 255) / 256 < 148 * 64 ? (n + 255) / 256 : 148 * 64);
+    if (units)
+        rope_units_kernel<T><<<grid, 256, 0, s>>>(q, qo, k, ko, ra, T_, dim, status);
+    else
+        rope_pairs_kernel<T><<<grid, 256, 0, s>>>(q, qo, k, ko, ra, T_, dim, status);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_rope_apply(const Rows& q, const Rows& qo, const Rows& k, const Rows& ko, const RopeArg& ra, int T,
+                              int dim, uint32_t type, unsigned* status, cudaStream_t s) {
+    if (type == T_F32) return rope_launch<float>(q, qo, k, ko, ra, T, dim, status, s);
+    if (type == T_F16) return rope_launch<__half>(q, qo, k, ko, ra, T, dim, status, s);
+    return rope_launch<__nv_bfloat16>(q, qo, k, ko, ra, T, dim, status, s);
+}
+
+rmoe_status check_rows(const rmoe_rows& a, uint32_t T, uint32_t type, const char* what, Rows& r) {
+    const uint32_t es = elt_size(type);
+    if (a.heads > 65535) return fail(RMOE_ERR_UNSUPPORTED, "%s: %u heads", what, a.heads);
+    if (a.heads && T && !a.data) return fail(RMOE_ERR_INVALID, "%s: null data", what);
+    if (reinterpret_cast<uintptr_t>(a.data) % es) return fail(RMOE_ERR_INVALID, "%s: misaligned data", what);
+    r.p = static_cast<char*>(a.data);
+    r.st = a.stride_t;
+    r.sh = a.stride_h;
+    r.heads = (int)a.heads;
+    r.vec = reinterpret_cast<uintptr_t>(a.data) % 16 == 0 && (a.stride_t * es) % 16 == 0 && (a.stride_h * es) % 16 == 0;
+    return RMOE_OK;
+}
+
+}  // namespace rmoe
+
+using namespace rmoe;
+
+extern "C" {
+
+rmoe_status rmoe_rope_create(const rmoe_rope_desc* d, rmoe_rope** out) {
+    if (!out) return fail(RMOE_ERR_INVALID, "null output handle");
+    *out = nullptr;
+    if (!d) return fail(RMOE_ERR_INVALID, "null rope description");
+    if (d->rot_dim < 2 || d->rot_dim % 2 || d->rot_dim > 4096)
+        return fail(RMOE_ERR_INVALID, "rot_dim %u must be even, 2 .. 4096", d->rot_dim);
+    if (d->layout > RMOE_ROPE_HALF) return fail(RMOE_ERR_INVALID, "rope layout %u", d->layout);
+    if (d->scaling > RMOE_ROPE_YARN) return fail(RMOE_ERR_INVALID, "rope scaling %u", d->scaling);
+    if (d->max_pos == 0 || d->max_pos > 0x7fffffffu) return fail(RMOE_ERR_INVALID, "max_pos %u", d->max_pos);
+    if (!(d->base > 0.0) || !isfinite(d->base)) return fail(RMOE_ERR_INVALID, "rope base %g", d->base);
+    const bool scaled = d->scaling != RMOE_ROPE_PLAIN;
+    if (scaled && (!(d->factor >= 1.0) || !isfinite(d->factor)))
+        return fail(RMOE_ERR_INVALID, "rope scaling factor %g must be at least 1", d->factor);
+    if (d->scaling == RMOE_ROPE_YARN && (d->orig_ctx == 0 || d->base == 1.0))
+        return fail(RMOE_ERR_INVALID, "YaRN needs orig_ctx > 0 and a base other than 1");
+    const double fast = d->beta_fast == 0.0 ? 32.0 : d->beta_fast, slow = d->beta_slow == 0.0 ? 1.0 : d->beta_slow;
+    if (d->scaling == RMOE_ROPE_YARN && (!(fast > 0.0) || !(slow > 0.0) || !(fast >= slow)))
+        return fail(RMOE_ERR_INVALID, "YaRN beta_fast %g, beta_slow %g", fast, slow);
+    if (!isfinite(d->mscale)) return fail(RMOE_ERR_INVALID, "rope mscale %g", d->mscale);
+    const uint32_t pairs = d->rot_dim / 2;
+    for (uint32_t i = 0; d->freq_factors && i < pairs; i++)
+        if (!(fabsf(d->freq_factors[i]) > 0.0f) || !isfinite(d->freq_factors[i]))
+            return fail(RMOE_ERR_INVALID, "freq_factors[%u] = %g", i, d->freq_factors[i]);
+    double low = 0, high = 0, m = 1.0;
+    if (d->scaling == RMOE_ROPE_YARN) {
+        // the pair that makes n turns in orig_ctx positions: base^(-2i/rot) = 2 pi n / orig_ctx
+        const double two_pi = 6.283185307179586476925286766559;
+        auto at = [&](double n) { return d->rot_dim * log(d->orig_ctx / (n * two_pi)) / (2.0 * log(d->base)); };
+        low = fmax(floor(at(fast)), 0.0);
+        high = fmin(ceil(at(slow)), (double)d->rot_dim - 1.0);
+        m = 0.1 * log(d->factor) + 1.0;
+    }
+    if (d->mscale != 0.0) m = d->mscale;
+    if (rmoe_status s = check_device(d->device)) return s;
+    std::vector<double> f;
+    rmoe_rope* r = nullptr;
+    try {
+        f.resize(pairs);
+        r = new rmoe_rope();
+    } catch (...) {
+        return fail(RMOE_ERR_OOM, "rope handle");
+    }
+    for (uint32_t i = 0; i < pairs; i++) {
+        double v = pow(d->base, -2.0 * i / d->rot_dim);
+        if (d->scaling == RMOE_ROPE_LINEAR) v /= d->factor;
+        if (d->scaling == RMOE_ROPE_YARN) {
+            const double g = 1.0 - fmin(fmax((i - low) / fmax(high - low, 0.001), 0.0), 1.0);
+            v = v * g + v / d->factor * (1.0 - g);
+        }
+        f[i] = d->freq_factors ? v / d->freq_factors[i] : v;
+    }
+    DeviceGuard g(d->device);
+    r->device = d->device;
+    r->rot = d->rot_dim;
+    r->layout = d->layout;
+    r->max_pos = d->max_pos;
+    const uint64_t n = (uint64_t)d->max_pos * pairs;
+    r->table = (float2*)r->own.alloc(n * sizeof(float2));
+    double* fd = (double*)r->own.alloc(pairs * sizeof(double));
+    r->status = (unsigned*)r->own.alloc(16);
+    if (!r->table || !fd || !r->status) {
+        delete r;
+        cudaGetLastError();
+        return fail(RMOE_ERR_OOM, "rope table: cudaMalloc(%llu) failed", (unsigned long long)(n * sizeof(float2)));
+    }
+    cudaError_t e = cudaMemcpy(fd, f.data(), pairs * sizeof(double), cudaMemcpyHostToDevice);
+    if (e == cudaSuccess) e = cudaMemset(r->status, 0, 16);
+    if (e == cudaSuccess) {
+        rope_table_kernel<<<(unsigned)((n + 255) / 256 < 148 * 16 ? (n + 255) / 256 : 148 * 16), 256>>>(r->table, fd,
+                                                                                                   (int)pairs, n, m);
+        e = cudaGetLastError();
+    }
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    if (e != cudaSuccess) {
+        delete r;
+        return cuda_fail(e, "rope table");
+    }
+    *out = r;
+    return RMOE_OK;
+}
+
+void rmoe_rope_destroy(rmoe_rope* r) {
+    if (!r) return;
+    DeviceGuard g(r->device);
+    cudaDeviceSynchronize();
+    delete r;
+}
+
+rmoe_status rmoe_rope_apply(rmoe_rope* r, const rmoe_rope_args* a, void* stream) {
+    if (!r || !a) return fail(RMOE_ERR_INVALID, "null rope / arguments");
+    if (!elt_ok(a->type)) return fail(RMOE_ERR_UNSUPPORTED, "rope: ggml type %u (F32, F16 or BF16)", a->type);
+    if (a->head_dim < r->rot) return fail(RMOE_ERR_INVALID, "head_dim %u is below rot_dim %u", a->head_dim, r->rot);
+    if (a->T > 0x7fffffffu || a->head_dim > 65536) return fail(RMOE_ERR_UNSUPPORTED, "rope: T %u x %u", a->T, a->head_dim);
+    Rows q, qo, k, ko;
+    rmoe_status s;
+    if ((s = check_rows(a->q, a->T, a->type, "q", q)) || (s = check_rows(a->q_out, a->T, a->type, "q_out", qo)) ||
+        (s = check_rows(a->k, a->T, a->type, "k", k)) || (s = check_rows(a->k_out, a->T, a->type, "k_out", ko)))
+        return s;
+    if (q.heads != qo.heads || k.heads != ko.heads) return fail(RMOE_ERR_INVALID, "rope: heads of the outputs differ");
+    if (a->T == 0 || q.heads + k.heads == 0) return RMOE_OK;
+    if (!a->positions) return fail(RMOE_ERR_INVALID, "null positions");
+    DeviceGuard g(r->device);
+    RopeArg ra{r->table, a->positions, (int)r->rot, r->layout == RMOE_ROPE_HALF, (int)r->max_pos,
+               a->inverse ? -1.0f : 1.0f};
+    cudaError_t e = launch_rope_apply(q, qo, k, ko, ra, (int)a->T, (int)a->head_dim, a->type, r->status,
+                                      static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? RMOE_OK : cuda_fail(e, "rope launch");
+}
+
+rmoe_status rmoe_rope_status(rmoe_rope* r) {
+    if (!r) return fail(RMOE_ERR_INVALID, "null rope");
+    DeviceGuard g(r->device);
+    unsigned hs = 0;
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = cudaMemcpy(&hs, r->status, 4, cudaMemcpyDeviceToHost);
+    if (e == cudaSuccess && hs) e = cudaMemset(r->status, 0, 4);
+    if (e != cudaSuccess) return cuda_fail(e, "rope status");
+    if (hs) return fail(RMOE_ERR_DEVICE, "rope: device status 0x%x (a position outside the table)", hs);
+    return RMOE_OK;
+}
+
+}  // extern "C"

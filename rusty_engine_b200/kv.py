@@ -1,0 +1,390 @@
+"""The paged 8-bit KV cache next to the MoE layer, and the operators that serve a block with it.
+
+* ``extend_tables`` / ``KVBatch``  -- block tables and slot maps, built on the GPU from lengths
+* ``Rope``                         -- rotary positions (src/infer.rs:90-145), both layouts, part of
+  the head, scaled for long contexts
+* ``KVCache.append`` / ``read``    -- keys and values into 8-bit codes with a scale per block of
+  tokens and head (rope of q and k with it), and back
+* ``KVCache.attend``               -- attention over the cache (src/forward.rs:218-283) for prompts,
+  prompt chunks and single tokens, any mix of them in one call
+
+One step of a server:  ``step = batch.extend(new_lens, total)``, then per block of the model
+``q = cache.append(k, v, step.slots, rope=rope, positions=step.positions, q=q)`` and
+``ctx = cache.attend(q, batch.table, batch.lens, step.cu)``; ``batch.release(done)`` when requests
+end.  Calls are stream-ordered on the current stream (or ``stream=``) and wait for nothing, so a
+step can be captured in a CUDA graph; lengths live on the GPU only.  Shape and type errors raise
+``EngineError``; what only the device can see (a slot out of range, a key that is not finite) is
+kept in the handle's status word, which ``check()`` reads and raises.  Tensors are float32,
+float16 or bfloat16 CUDA tensors [tokens, heads, head_dim] whose last dimension is contiguous.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import enum
+import math
+from dataclasses import dataclass
+from typing import Optional, Sequence
+
+import numpy as np
+
+from . import _lib
+from .moe import EngineError, _call, _require_cuda, torch
+
+if torch is not None:
+    _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}  # ggml codes
+    _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+
+
+class RopeLayout(enum.IntEnum):
+    Interleaved = 0  # pairs (x[2i], x[2i + 1])
+    Half = 1         # pairs (x[i], x[i + rot_dim / 2]), rusty-engine's NeoX rotate-half
+
+
+class RopeScaling(enum.IntEnum):
+    NoScaling = 0
+    Linear = 1
+    Yarn = 2
+
+
+class CacheCode(enum.IntEnum):
+    Int8 = 0
+    E4M3 = 1
+
+
+@dataclass(frozen=True)
+class RopeConfig:
+    """rmoe_rope_desc: angle of pair i at position p is p * base^(-2i / rot_dim), scaled."""
+
+    rot_dim: int
+    base: float = 1e6
+    layout: RopeLayout = RopeLayout.Half
+    scaling: RopeScaling = RopeScaling.NoScaling
+    factor: float = 1.0
+    orig_ctx: int = 0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    mscale: float = 0.0  # factor of cos and sin; 0: the scaling's own
+    freq_factors: Optional[Sequence[float]] = None
+
+
+def _stream_of(x, stream, *others):
+    """The raw stream a call runs on.  With an explicit stream, the tensors' memory is also kept
+    from being reused before that stream is done with it."""
+    if stream is None:
+        return _raw_stream(x.device.index) if _raw_stream else torch.cuda.current_stream(x.device).cuda_stream
+    for t in (x, *others):
+        if t is not None:
+            t.record_stream(stream)
+    return stream.cuda_stream
+
+
+def _rows(x, what):
+    """(data, token stride, head stride, heads, 0) of an rmoe_rows."""
+    if x.dim() != 3 or x.stride(2) != 1 and x.shape[2] != 1:
+        raise EngineError(f"{what}: a [tokens, heads, head_dim] tensor with contiguous heads, got {tuple(x.shape)} "
+                          f"strides {tuple(x.stride())}")
+    st = x.stride()
+    return x.data_ptr(), st[0], st[1], x.shape[1], 0
+
+
+_NO_ROWS = (0, 0, 0, 0, 0)
+
+
+def _type_of(x, what):
+    t = _TYPES.get(x.dtype)
+    if t is None or not x.is_cuda:
+        raise EngineError(f"{what}: a float32, float16 or bfloat16 CUDA tensor, got {x.dtype} on {x.device}")
+    return t
+
+
+def _int32(x, what, like, n=None):
+    if x.dtype != torch.int32 or not x.is_contiguous() or x.device != like.device:
+        raise EngineError(f"{what}: a contiguous int32 tensor on {like.device}, got {x.dtype} on {x.device}")
+    if n is not None and x.numel() != n:
+        raise EngineError(f"{what}: {x.numel()} entries, expected {n}")
+    return x.data_ptr()
+
+
+def _same(x, like, what):
+    if x.dtype != like.dtype or x.device != like.device:
+        raise EngineError(f"{what}: {x.dtype} on {x.device}, expected {like.dtype} on {like.device}")
+
+
+class Rope:
+    """Rotary positions 0 .. max_pos - 1 (rmoe_rope_create): the table of cosines and sines."""
+
+    def __init__(self, cfg: RopeConfig, max_pos: int, device: Optional[int] = None):
+        _require_cuda()
+        self.cfg, self.max_pos = cfg, max_pos
+        self.device = torch.cuda.current_device() if device is None else device
+        d = _lib.RopeDesc()
+        d.rot_dim, d.layout, d.scaling, d.max_pos = cfg.rot_dim, int(cfg.layout), int(cfg.scaling), max_pos
+        d.base, d.factor, d.beta_fast, d.beta_slow, d.mscale = cfg.base, cfg.factor, cfg.beta_fast, cfg.beta_slow, cfg.mscale
+        d.orig_ctx, d.device = cfg.orig_ctx, self.device
+        if cfg.freq_factors is not None:
+            ff = np.ascontiguousarray(cfg.freq_factors, dtype=np.float32)
+            if ff.shape != (cfg.rot_dim // 2,):
+                raise EngineError(f"freq_factors: {ff.shape}, expected ({cfg.rot_dim // 2},)")
+            d.freq_factors = ff.ctypes.data
+        h = C.c_void_p()
+        L = _lib.load()
+        _call(L.rmoe_rope_create(C.byref(d), C.byref(h)))
+        self._h, self._apply = h, L.rmoe_rope_apply
+
+    def apply(self, q, positions, k=None, *, out=None, k_out=None, inverse: bool = False, stream=None):
+        """q (and k) [tokens, heads, head_dim] turned by positions [tokens] (int32); returns the
+        turned q, or (q, k) when k is given.  `out=q` turns in place.  inverse: turns back."""
+        ty = _type_of(q, "q")
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        qr, orow = _rows(q, "q"), _rows(out, "out")
+        _same(out, q, "out")
+        T, _, dim = q.shape
+        if out.shape != q.shape:
+            raise EngineError(f"out: {tuple(out.shape)}, expected {tuple(q.shape)}")
+        if k is not None:
+            _same(k, q, "k")
+            if k_out is None:
+                k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+            _same(k_out, q, "k_out")
+            kr, kor = _rows(k, "k"), _rows(k_out, "k_out")
+            if k.shape[0] != T or k.shape[2] != dim or k_out.shape != k.shape:
+                raise EngineError(f"k: {tuple(k.shape)} / {tuple(k_out.shape)} beside q {tuple(q.shape)}")
+        else:
+            kr = kor = _NO_ROWS
+        if q.device.index != self.device:
+            raise EngineError(f"q is on {q.device}, the rope on device {self.device}")
+        args = _lib.ROPE_ARGS.pack(*qr, *orow, *kr, *kor, _int32(positions, "positions", q, T), T, dim, ty,
+                                   1 if inverse else 0)
+        st = self._apply(self._h, args, _stream_of(q, stream, out, k, k_out, positions))
+        if st:
+            _call(st)
+        return out if k is None else (out, k_out)
+
+    def check(self):
+        """Raises if a call so far met a position outside the table (synchronises)."""
+        _call(_lib.load().rmoe_rope_status(self._h))
+
+    def close(self):
+        if getattr(self, "_h", None) is not None and self._h.value:
+            _lib.load().rmoe_rope_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+@dataclass
+class KVStep:
+    """What extend made for one step: cu [R + 1], positions and slots [tokens], and the lengths
+    [R] and free-stack height [1] afterwards (all int32)."""
+
+    cu: "torch.Tensor"
+    positions: "torch.Tensor"
+    slots: "torch.Tensor"
+    lens: "torch.Tensor"
+    n_free: "torch.Tensor"
+
+
+def extend_tables(table, lens, new_lens, free, n_free, total: int, block_size: int, *, stream=None) -> KVStep:
+    """rmoe_kv_extend: request r, holding lens[r] tokens, adds new_lens[r]; `total` is the batch's
+    token count (slots past the requests' tokens are -1).  New blocks come off the stack
+    free[:n_free] in request order and are written into `table` [R, max_blocks]; a request that
+    cannot have all its blocks gets none: its slots are -1 and its length stays."""
+    if table.dim() != 2:
+        raise EngineError(f"table: [requests, blocks], got {tuple(table.shape)}")
+    if not table.is_cuda:
+        raise EngineError(f"table: a CUDA tensor, got {table.device}")
+    if total < 0:
+        raise EngineError(f"total {total}")
+    R, mb = table.shape
+    # one allocation: cu, then the [R] and [total] outputs
+    buf = torch.empty(2 * R + 2 + 2 * total, dtype=torch.int32, device=table.device)
+    cu, out_lens, out_free, positions, slots = buf.split((R + 1, R, 1, total, total))
+    base = buf.data_ptr()
+    args = _lib.KV_EXTEND_ARGS.pack(
+        _int32(table, "table", table), _int32(lens, "lens", table, R), _int32(new_lens, "new_lens", table, R),
+        _int32(free, "free", table), _int32(n_free, "n_free", table, 1), base, base + 4 * (2 * R + 2),
+        base + 4 * (2 * R + 2 + total), base + 4 * (R + 1), base + 4 * (2 * R + 1), R, mb, total, block_size, free.numel(), 0)
+    with torch.cuda.device(table.device):
+        st = _lib.load().rmoe_kv_extend(args, _stream_of(table, stream, lens, new_lens, free, n_free, buf))
+    if st:
+        _call(st)
+    return KVStep(cu, positions, slots, out_lens, out_free)
+
+
+class KVBatch:
+    """The requests in flight: table [R, max_blocks], lens [R] and the free-block stack, on the GPU."""
+
+    def __init__(self, max_requests: int, max_blocks: int, n_blocks: int, block_size: int, device=None):
+        _require_cuda()
+        dev = torch.device("cuda", torch.cuda.current_device() if device is None else device)
+        self.block_size = block_size
+        self.table = torch.full((max_requests, max_blocks), -1, dtype=torch.int32, device=dev)
+        self.lens = torch.zeros(max_requests, dtype=torch.int32, device=dev)
+        self.free = torch.arange(n_blocks - 1, -1, -1, dtype=torch.int32, device=dev)
+        self.n_free = torch.full((1,), n_blocks, dtype=torch.int32, device=dev)
+
+    def extend(self, new_lens, total: int, *, stream=None) -> KVStep:
+        """extend_tables on this batch; lens and the stack move on."""
+        step = extend_tables(self.table, self.lens, new_lens, self.free, self.n_free, total, self.block_size, stream=stream)
+        self.lens, self.n_free = step.lens, step.n_free
+        return step
+
+    def release(self, done, *, stream=None):
+        """rmoe_kv_release: requests with done[r] != 0 (int32 [R]) give their blocks back."""
+        R, mb = self.table.shape
+        out = torch.empty_like(self.n_free)
+        args = _lib.KV_RELEASE_ARGS.pack(self.table.data_ptr(), self.lens.data_ptr(), self.free.data_ptr(),
+                                         _int32(done, "done", self.table, R), self.n_free.data_ptr(), out.data_ptr(), R, mb,
+                                         self.block_size, self.free.numel())
+        with torch.cuda.device(self.table.device):
+            _call(_lib.load().rmoe_kv_release(args, _stream_of(self.table, stream, self.lens, self.free, done, self.n_free,
+                                                               out)))
+        self.n_free = out
+
+
+class KVCache:
+    """One layer's keys and values: codes [n_blocks, n_kv_heads, block_size, head_dim] in 8 bits and
+    one f32 scale per block and head (rmoe_kv_create)."""
+
+    def __init__(self, n_blocks: int, block_size: int, n_kv_heads: int, head_dim: int,
+                 code: CacheCode = CacheCode.Int8, device: Optional[int] = None):
+        _require_cuda()
+        dev = torch.device("cuda", torch.cuda.current_device() if device is None else device)
+        dt = torch.int8 if code == CacheCode.Int8 else torch.float8_e4m3fn
+        if min(n_blocks, block_size, n_kv_heads, head_dim) < 1:
+            raise EngineError(f"cache of {n_blocks} blocks x {n_kv_heads} heads x {block_size} x {head_dim}")
+        z = lambda: torch.zeros((n_blocks, n_kv_heads, block_size, head_dim), dtype=torch.uint8, device=dev).view(dt)  # noqa: E731
+        s = lambda: torch.zeros((n_blocks, n_kv_heads), dtype=torch.float32, device=dev)  # noqa: E731
+        self._bind(z(), z(), s(), s())
+
+    @classmethod
+    def from_buffers(cls, k, v, k_scale, v_scale) -> "KVCache":
+        """A cache over the caller's tensors: int8 or float8_e4m3fn codes and f32 scales."""
+        self = cls.__new__(cls)
+        self._bind(k, v, k_scale, v_scale)
+        return self
+
+    def _bind(self, k, v, ks, vs):
+        codes = {torch.int8: CacheCode.Int8, torch.float8_e4m3fn: CacheCode.E4M3}
+        if k.dtype not in codes or k.dim() != 4 or not k.is_cuda:
+            raise EngineError(f"cache codes: int8 or float8_e4m3fn [blocks, heads, block, dim] on CUDA, got {k.dtype} "
+                              f"{tuple(k.shape)} on {k.device}")
+        for name, t, shape, dt in (("v", v, k.shape, k.dtype), ("k_scale", ks, k.shape[:2], torch.float32),
+                                   ("v_scale", vs, k.shape[:2], torch.float32)):
+            if t.shape != shape or t.dtype != dt or t.device != k.device:
+                raise EngineError(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device} beside k {k.dtype} {tuple(k.shape)}")
+        for name, t in (("k", k), ("v", v), ("k_scale", ks), ("v_scale", vs)):
+            if not t.is_contiguous():
+                raise EngineError(f"{name}: cache memory must be contiguous")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, ks, vs
+        self.code, self.device = codes[k.dtype], k.device.index
+        self.n_blocks, self.n_kv_heads, self.block_size, self.head_dim = k.shape
+        d = _lib.KvDesc()
+        d.n_blocks, d.block_size, d.n_kv_heads, d.head_dim = self.n_blocks, self.block_size, self.n_kv_heads, self.head_dim
+        d.code, d.device = int(self.code), self.device
+        d.k, d.v, d.k_scale, d.v_scale = k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()
+        h = C.c_void_p()
+        L = _lib.load()
+        _call(L.rmoe_kv_create(C.byref(d), C.byref(h)))
+        self._h, self._append, self._read, self._attend = h, L.rmoe_kv_append, L.rmoe_kv_read, L.rmoe_kv_attend
+
+    def append(self, k, v, slots, *, rope: Optional[Rope] = None, positions=None, q=None, q_out=None, stream=None):
+        """Writes k and v [tokens, n_kv_heads, head_dim] at `slots` (int32, -1 skips).  With a
+        rope, k is turned by `positions` first, and so is q where given; returns the turned q."""
+        ty = _type_of(k, "k")
+        T = k.shape[0]
+        _same(v, k, "v")
+        kr, vr = _rows(k, "k"), _rows(v, "v")
+        want = (T, self.n_kv_heads, self.head_dim)
+        if k.shape != want or v.shape != want:
+            raise EngineError(f"k {tuple(k.shape)} / v {tuple(v.shape)}, expected {want}")
+        if k.device.index != self.device:
+            raise EngineError(f"k is on {k.device}, the cache on device {self.device}")
+        qr = qor = _NO_ROWS
+        pp = rh = 0
+        if rope is not None:
+            if positions is None:
+                raise EngineError("rope needs positions")
+            pp, rh = _int32(positions, "positions", k, T), rope._h.value
+            if q is not None:
+                _same(q, k, "q")
+                if q_out is None:
+                    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                _same(q_out, q, "q_out")
+                qr, qor = _rows(q, "q"), _rows(q_out, "q_out")
+                if q.shape[0] != T or q.shape[2] != self.head_dim or q_out.shape != q.shape:
+                    raise EngineError(f"q {tuple(q.shape)} / {tuple(q_out.shape)} beside k {tuple(k.shape)}")
+        elif q is not None:
+            raise EngineError("q is only taken with a rope")
+        args = _lib.KV_APPEND_ARGS.pack(*kr, *vr, *qr, *qor, _int32(slots, "slots", k, T), pp, rh, T, ty)
+        st = self._append(self._h, args, _stream_of(k, stream, v, slots, positions, q, q_out))
+        if st:
+            _call(st)
+        return q_out
+
+    def read(self, slots, dtype=None, *, stream=None):
+        """(k, v) of cached tokens [slots, n_kv_heads, head_dim], code * scale, as `dtype` (float32)."""
+        dtype = torch.float32 if dtype is None else dtype
+        if dtype not in _TYPES:
+            raise EngineError(f"read as {dtype}")
+        n = slots.numel()
+        p = _int32(slots, "slots", self.k)
+        both = torch.empty((2, n, self.n_kv_heads, self.head_dim), dtype=dtype, device=self.k.device)
+        k, v = both.unbind(0)
+        st = self._read(self._h, p, n, _TYPES[dtype], k.data_ptr(), v.data_ptr(), _stream_of(both, stream, slots))
+        if st:
+            _call(st)
+        return k, v
+
+    def attend(self, q, table, lens, cu, *, scale: Optional[float] = None, window: int = 0, max_new: Optional[int] = None,
+               out=None, return_lse: bool = False, stream=None):
+        """Attention of q [tokens, q heads, head_dim]: request r, with lens[r] cached tokens in
+        blocks table[r], has the queries cu[r] .. cu[r + 1) at its last positions.  Causal; with a
+        window, each query sees that many keys at most.  scale: 1 / sqrt(head_dim) by default.
+        max_new: an upper bound of any request's new tokens, where known (chooses kernels only).
+        Returns out (as q), or (out, lse [tokens, q heads] f32)."""
+        ty = _type_of(q, "q")
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        else:
+            _same(out, q, "out")
+        qr, orow = _rows(q, "q"), _rows(out, "out")
+        T, nq, dim = q.shape
+        if dim != self.head_dim or out.shape != q.shape:
+            raise EngineError(f"q {tuple(q.shape)} / out {tuple(out.shape)} with head_dim {self.head_dim}")
+        if q.device.index != self.device:
+            raise EngineError(f"q is on {q.device}, the cache on device {self.device}")
+        if table.dim() != 2:
+            raise EngineError(f"table: [requests, blocks], got {tuple(table.shape)}")
+        R, mb = table.shape
+        if window < 0 or (max_new is not None and max_new < 0):
+            raise EngineError(f"window {window}, max_new {max_new}")
+        lse = torch.empty((T, nq), dtype=torch.float32, device=q.device) if return_lse else None
+        args = _lib.KV_ATTEND_ARGS.pack(
+            *qr, *orow, _int32(table, "table", q), _int32(lens, "lens", q, R), _int32(cu, "cu", q, R + 1),
+            lse.data_ptr() if return_lse else 0, R, mb, T, ty, 1.0 / math.sqrt(dim) if scale is None else scale, window,
+            max_new or 0, 0)
+        st = self._attend(self._h, args, _stream_of(q, stream, out, table, lens, cu, lse))
+        if st:
+            _call(st)
+        return (out, lse) if return_lse else out
+
+    def check(self):
+        """Raises if a call so far met a device error (synchronises and clears it)."""
+        _call(_lib.load().rmoe_kv_status(self._h))
+
+    def close(self):
+        if getattr(self, "_h", None) is not None and self._h.value:
+            _lib.load().rmoe_kv_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass

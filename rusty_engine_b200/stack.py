@@ -12,8 +12,11 @@ the MoE layer, as moe_block_forward does for one token:
     y = x + o(ctx)                                                   (src/forward.rs:557-558)
     out = y + moe_layer_forward(rmsnorm(y, ffn_norm))                (src/moe.rs:462-468)
 
-Only the MoE layers are this library's hot path and only they are timed (CUDA events around
-each MoE forward).  The rest runs on the GPU as plumbing: the q/k/v/o projections on this
+``MoEStack.step`` serves the same blocks: many requests' prompts, chunks and single tokens over
+the paged 8-bit KV cache (kv.py), with rope, cache write and attention on this library's kernels.
+
+In ``MoEStack.forward`` only the MoE layers are this library's hot path and only they are timed
+(CUDA events around each MoE forward).  The rest runs on the GPU as plumbing: the q/k/v/o projections on this
 library's resident QMat products, norms, RoPE and the attention core as torch f32 operations.
 Weights are random (seeded); the expert stacks of the layers are generated quickly as
 variants of one base stack (the quant bytes xor-ed with a per-layer random mask, the block
@@ -225,7 +228,51 @@ class MoEStack:
             self.moe_ms = [a.elapsed_time(b) for a, b in events]
         return x
 
+    # ---- serving: prompts, chunks and single tokens of many requests over the paged 8-bit cache ----
+    def open_cache(self, max_requests: int, n_blocks: int, block_size: int = 64, max_pos: int = 4096, code=None,
+                   rope_cfg=None):
+        """A paged 8-bit KV cache of n_blocks blocks per layer for up to max_requests requests of up
+        to max_pos tokens, and the rotary plan (NeoX halves over the whole head by default)."""
+        from . import kv
+
+        g = self.g
+        cfg = rope_cfg or kv.RopeConfig(rot_dim=g.head_dim, base=g.rope_freq_base, layout=kv.RopeLayout.Half)
+        code = kv.CacheCode.Int8 if code is None else code
+        self.rope = kv.Rope(cfg, max_pos, self.device)
+        self.batch = kv.KVBatch(max_requests, -(-max_pos // block_size), n_blocks, block_size, self.device)
+        self.caches = [kv.KVCache(n_blocks, block_size, g.n_kv_heads, g.head_dim, code, self.device) for _ in self.layers]
+
+    def step(self, x, new_lens, max_new: Optional[int] = None, collect: bool = False):
+        """One serving step: x [T, d_model] holds the new tokens of every request in order
+        (request r adds new_lens[r] of them: a prompt, a chunk of one, a decoded token, or none).
+        Returns the hidden states [T, d_model]; the tokens' keys and values are in the caches
+        afterwards.  max_new: the largest new_lens, where known on the host.  collect: as forward."""
+        g, T = self.g, x.shape[0]
+        st = self.batch.extend(new_lens, T)
+        self.last_step = st
+        self.block_inputs, self.block_mids = [], []
+        for L, cache in zip(self.layers, self.caches):
+            if collect:
+                self.block_inputs.append(x.clone())
+            xn = self._rmsnorm(x, L["attn_norm"])
+            q = L["q"].matmul_device(xn).view(T, g.n_heads, g.head_dim)
+            k = L["k"].matmul_device(xn).view(T, g.n_kv_heads, g.head_dim)
+            v = L["v"].matmul_device(xn).view(T, g.n_kv_heads, g.head_dim)
+            q = cache.append(k, v, st.slots, rope=self.rope, positions=st.positions, q=q, q_out=q)
+            ctx = cache.attend(q, self.batch.table, self.batch.lens, st.cu, max_new=max_new)
+            y = x + L["o"].matmul_device(ctx.view(T, g.n_heads * g.head_dim))
+            if collect:
+                self.block_mids.append(y.clone())
+            x = y + L["moe"].forward(self._rmsnorm(y, L["ffn_norm"]).contiguous())
+        return x
+
+    def finish(self, done):
+        """Requests with done[r] != 0 (int32 [max_requests] on the GPU) leave the batch."""
+        self.batch.release(done)
+
     def close(self):
+        for c in getattr(self, "caches", []):
+            c.close()
         for L in self.layers:
             L["moe"].close()
-        self.layers = []
+        self.layers, self.caches = [], []

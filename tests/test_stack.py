@@ -60,3 +60,74 @@ def test_rope_tables_match_reference_formula():
             f = np.float32(1.0) / np.power(np.float32(g.rope_freq_base), np.float32(2 * i) / np.float32(d))
             ang = np.float32(pos) * np.float32(f)
             assert c[pos - 3, i] == np.float32(np.cos(ang)) and s[pos - 3, i] == np.float32(np.sin(ang))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", ["Int8", "E4M3"])
+def test_stack_serving_steps(gpu, code):
+    """MoEStack.step over prompts, chunks and single tokens of three requests: every block's
+    attention residual against a float64 restatement over the keys and values that the cache holds
+    (relative L2 <= 5e-3, the bar of the prefill test: the QMat products' fp16 operands), and those
+    values against the exact rotated keys and values, off by at most a rounding step of the cache
+    (half a step, and half again for each time a block's scale grew)."""
+    import torch
+
+    from oracle import stack_ref
+    from rusty_engine_b200 import kv
+    from rusty_engine_b200.stack import MoEStack, make_block, rope_tables
+
+    g = small_geometry()
+    blocks = [make_block(g, seed=30 + i, dlo=0.001, dhi=0.004, attn_dlo=0.002, attn_dhi=0.01) for i in range(2)]
+    stack = MoEStack(g, blocks, device=0)
+    stack.open_cache(max_requests=3, n_blocks=40, block_size=16, max_pos=512, code=kv.CacheCode[code])
+    steps = [[33, 0, 150], [1, 20, 1], [17, 1, 0], [1, 1, 1]]
+    xs, ins, mids, outs = [], [[] for _ in blocks], [[] for _ in blocks], []
+    req, pos, lens = [], [], [0, 0, 0]
+    for i, new in enumerate(steps):
+        x = synth.activations(sum(new), g.d_model, seed=50 + i)
+        xs.append(x)
+        outs.append(stack.step(torch.from_numpy(x).cuda(), torch.tensor(new, dtype=torch.int32, device="cuda"),
+                               max_new=max(new), collect=True).cpu().numpy())
+        for b in range(len(blocks)):
+            ins[b].append(stack.block_inputs[b].cpu().numpy())
+            mids[b].append(stack.block_mids[b].cpu().numpy())
+        for r, n in enumerate(new):
+            req += [r] * n
+            pos += range(lens[r], lens[r] + n)
+            lens[r] += n
+    req, pos = np.array(req), np.array(pos)
+    assert stack.batch.lens.tolist() == lens
+    table = stack.batch.table.cpu().numpy()
+    cos, sin = rope_tables(g, 512)
+    hd, qd, kvd = g.head_dim, g.n_heads * g.head_dim, g.n_kv_heads * g.head_dim
+    rel = lambda a, b: float(np.linalg.norm(a.astype(np.float64) - b) / np.linalg.norm(b))
+    for b, w in enumerate(blocks):
+        x = np.concatenate(ins[b])
+        xn = stack_ref.rmsnorm(x, w.attn_norm, g.rms_eps)
+        q = stack_ref.rope(stack_ref.proj(w.q, qd, g.d_model, xn), g.n_heads, hd, cos[pos], sin[pos])
+        k = stack_ref.rope(stack_ref.proj(w.k, kvd, g.d_model, xn), g.n_kv_heads, hd, cos[pos], sin[pos])
+        v = stack_ref.proj(w.v, kvd, g.d_model, xn)
+        slots = torch.tensor(table[req, pos // 16] * 16 + pos % 16, dtype=torch.int32, device="cuda")
+        ck, cv = (t.cpu().numpy().reshape(-1, kvd) for t in stack.caches[b].read(slots))
+        stack.caches[b].check()
+        # a step is max|x| / 127 of the block and head (1 / 16 of the value itself for e4m3, whose
+        # last bit is a half of an eighth); the products' own error is 5e-3 of the row's size
+        for got, want in ((ck, k), (cv, v)):
+            unit = 3 / 127 if code == "Int8" else 3 / 16
+            assert np.abs(got - want).max() <= unit * np.abs(want).max()
+        ctx = np.zeros((len(req), qd))
+        for t in range(len(req)):
+            seen = (req == req[t]) & (pos <= pos[t])
+            for h in range(g.n_heads):
+                c = slice(h // (g.n_heads // g.n_kv_heads) * hd, (h // (g.n_heads // g.n_kv_heads) + 1) * hd)
+                z = ck[seen][:, c].astype(np.float64) @ q[t, h * hd:(h + 1) * hd] / np.sqrt(hd)
+                p = np.exp(z - z.max())
+                ctx[t, h * hd:(h + 1) * hd] = p @ cv[seen][:, c].astype(np.float64) / p.sum()
+        want = x + stack_ref.proj(w.o, g.d_model, qd, ctx)
+        # attention before a block's scale grew saw codes of the smaller step: the cache's rounding
+        e = rel(np.concatenate(mids[b]), want)
+        print(f"stack step {code} block {b}: attention residual rel-L2 {e:.2e}")
+        assert e <= (5e-3 if code == "Int8" else 2e-2)
+    stack.finish(torch.tensor([1, 0, 1], dtype=torch.int32, device="cuda"))
+    assert stack.batch.lens.tolist() == [0, lens[1], 0]
+    stack.close()
