@@ -107,6 +107,12 @@ bool make_weight_maps(const DevMat& M, WMaps& out, uint32_t rows) {
     }
 }
 
+bool make_code_map(const void* base, uint64_t rows, uint32_t dim, uint32_t box_rows, CUtensorMap& out) {
+    const uint32_t w = dim < 128 ? dim : 128;
+    return encode2d(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, dim, rows, dim, w, box_rows,
+                    w == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
 bool make_rows_map(const __half* base, uint64_t rows, uint32_t width, CUtensorMap& out) {
     return encode2d(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, base, width, rows, (uint64_t)width * 2, TC_KS, TC_BN,
                     CU_TENSOR_MAP_SWIZZLE_128B);

@@ -168,6 +168,9 @@ cudaError_t launch_gvt_down(const GroupedParams& p, const TcMaps& maps, int max_
 
 // Build the maps of one stack (after upload_mat) / of the h workspace; false on a driver error.
 bool make_weight_maps(const DevMat& M, WMaps& out, uint32_t rows = 128);  // rows: box height
+// TMA map of `rows` rows of `dim` cached bytes (kv_impl.h), in boxes of box_rows rows of at most
+// 128 bytes, swizzled over their width (128 or 64 bytes).
+bool make_code_map(const void* base, uint64_t rows, uint32_t dim, uint32_t box_rows, CUtensorMap& out);
 bool make_rows_map(const __half* base, uint64_t rows, uint32_t width, CUtensorMap& out);
 // fp32 [rows, width] row-major, 128-B-swizzled boxes of box_w (32) x box_rows
 bool make_f32_rows_map(const float* base, uint64_t rows, uint32_t width, uint32_t box_w, uint32_t box_rows,

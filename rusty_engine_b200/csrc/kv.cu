@@ -1,5 +1,7 @@
 // kv.cu -- the paged 8-bit KV cache handle: memory, checks, status.
-#include "kv_impl.h"
+#include <algorithm>
+
+#include "kv_attend.h"
 
 using namespace rmoe;
 
@@ -40,9 +42,13 @@ rmoe_status rmoe_kv_create(const rmoe_kv_desc* d, rmoe_kv** out) {
     kv->dim = d->head_dim;
     kv->code = d->code;
     const uint64_t bytes = rows * d->head_dim, sb = (uint64_t)d->n_blocks * d->n_kv_heads * 4;
+    cudaDeviceGetAttribute(&kv->sms, cudaDevAttrMultiProcessorCount, d->device);
     kv->status = (unsigned*)kv->own.alloc(16);
-    bool ok = kv->status != nullptr;
+    kv->split_part = (float*)kv->own.alloc(kv->sms * split_part_bytes((int)kv->dim));
+    kv->split_ticket = (unsigned*)kv->own.alloc(kv->sms * 4);
+    bool ok = kv->status && kv->split_part && kv->split_ticket;
     cudaError_t e = ok ? cudaMemset(kv->status, 0, 16) : cudaSuccess;
+    if (ok && e == cudaSuccess) e = cudaMemset(kv->split_ticket, 0, kv->sms * 4);
     if (given) {
         kv->k = (uint8_t*)d->k;
         kv->v = (uint8_t*)d->v;
@@ -65,6 +71,11 @@ rmoe_status rmoe_kv_create(const rmoe_kv_desc* d, rmoe_kv** out) {
         cudaGetLastError();
         return ok ? cuda_fail(e, "cache memory")
                   : fail(RMOE_ERR_OOM, "cache memory: cudaMalloc of 2 x %llu bytes failed", (unsigned long long)bytes);
+    }
+    const uint32_t box = std::min<uint32_t>(kv->bs, split_tile_tokens((int)kv->dim));
+    if (!make_code_map(kv->k, rows, kv->dim, box, kv->split_maps.k) || !make_code_map(kv->v, rows, kv->dim, box, kv->split_maps.v)) {
+        delete kv;
+        return fail(RMOE_ERR_CUDA, "cuTensorMapEncodeTiled failed for the cache");
     }
     *out = kv;
     return RMOE_OK;

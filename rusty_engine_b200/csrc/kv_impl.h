@@ -13,12 +13,22 @@ struct rmoe_rope {
     rmoe::Owned own;
 };
 
+namespace rmoe {
+struct KvMaps {
+    CUtensorMap k, v;  // the codes as rows of head_dim bytes (make_code_map)
+};
+}  // namespace rmoe
+
 struct rmoe_kv {
     int device = 0;
     uint32_t n_blocks = 0, bs = 0, heads = 0, dim = 0, code = 0;
     uint8_t *k = nullptr, *v = nullptr;
     float *ks = nullptr, *vs = nullptr;
     unsigned* status = nullptr;
+    rmoe::KvMaps split_maps{};     // boxes of a split-kernel tile
+    int sms = 0;
+    float* split_part = nullptr;   // split kernel: pieces of items that span CTAs
+    unsigned* split_ticket = nullptr;
     rmoe::Owned own;
 };
 

@@ -1,0 +1,705 @@
+// kv_split.cu -- attention over the 8-bit paged cache for few query rows per request: decoded
+// tokens, short speculative chunks.  The work is reading the cache once; it is bound by HBM.
+//
+// Mathematics.  With x_j = scale log2(e) ks_j q.kc_j + log2(vs_j) over the keys j that a row sees,
+//   out = sum_j 2^(x_j - M) vc_j / sum_j 2^(x_j - M) / vs_j ,   lse = (M + log2 of that sum) ln 2
+// for any M; M is the running maximum of x_j.  Folding the V scale into the exponent keeps the
+// weights of P V in (0, 1] whatever the scales are, so fp16 holds them; a scale below 2^-100 counts
+// as 2^-100.  Codes are exact in fp16; q is carried as fp16 times a power of two per row, f32
+// calls carry q and the weights as fp16 pairs (hi + lo), and all sums are f32.
+//
+// Shape.  A unit of work is a tile of TW tokens of one item (request, kv head, tile of NR rows);
+// rows are a request's new tokens x the query heads that share the kv head.  All units of the call
+// are numbered, every warp of the grid takes an equal share of consecutive ones, so any mix of
+// lengths balances to one tile; no warp waits for another until its share is done.  A warp streams
+// its tiles by TMA into its own ring (its own mbarriers, no CTA-wide step) and works with
+// mma.sync on the transposed products S^T = K q^T and O^T = V^T P^T: tokens and head elements are
+// the M = 16 side, rows the N = 8 side, so eight rows fill the instruction.  The codes widen to
+// fp16 in the operand registers; the order of d inside a contraction and of tokens inside a tile
+// are free, and are chosen so that each lane's operand is the 16 bytes that it reads.
+//
+// Joining.  A share's incomplete first and last items leave (M, l, O) pieces; the CTA joins its
+// warps' pieces, and items that span CTAs go through a workspace slot per CTA, where the last
+// arriving CTA (an atomic count, nobody waits) joins them in CTA order: the result does not depend
+// on timing.
+#include "kv_code.cuh"
+#include "rope.cuh"
+#include "kv_attend.h"
+#include "tc_ptx.cuh"
+
+namespace rmoe {
+
+static constexpr int SPLIT_NW = 8;      // warps per CTA
+static constexpr int SPLIT_DEPTH = 2;   // tiles in a warp's ring
+
+template <int D>
+struct SplitShape {
+    static constexpr int TW = D == 256 ? 16 : 32;     // tokens per tile
+    static constexpr int STAGE = 2 * TW * D;          // K, then V
+    static constexpr int MT = TW / 16, KS = D / 16, HF = D / 64;
+};
+
+template <int D, int NR>
+struct SplitSmem {
+    static constexpr int PIECE = NR * (D + 2);        // floats: M[NR], l[NR], O[NR][D]
+    static constexpr int RING = SPLIT_NW * SPLIT_DEPTH * SplitShape<D>::STAGE;
+    static constexpr int FIRST = SPLIT_NW * PIECE * 4;
+    static constexpr int TOTAL = RING + FIRST + 1024;  // + alignment of the ring
+};
+
+// What the warps need of a request.
+struct SplitReq {
+    int q0, n;       // its first token and its token count
+    int pos0;        // position of its first token
+    int hi;          // keys 0 .. hi - 1 exist
+    int t0, tiles;   // tiles of an item
+    int items;       // row tiles x kv heads
+};
+
+__device__ __forceinline__ SplitReq split_req(const AttendArg& a, int r, int heads, int group, int bs, int nr, int tw) {
+    SplitReq q;
+    const int c0 = __ldg(a.cu + r), c1 = __ldg(a.cu + r + 1), len = __ldg(a.lens + r);
+    q.q0 = min(max(c0, 0), a.T);
+    q.n = max(0, min(c1, a.T) - q.q0);
+    q.pos0 = len - (c1 - c0);
+    const int64_t rows = (int64_t)q.n * group;
+    q.hi = (int)min((int64_t)max(len, 0), (int64_t)a.max_blocks * bs);
+    const int lo = a.window ? max(0, q.pos0 - a.window + 1) : 0;
+    q.t0 = min(lo, q.hi) / tw;
+    q.tiles = max(1, (q.hi + tw - 1) / tw - q.t0);
+    q.items = rows > a.split_rows ? 0 : (int)((rows + nr - 1) / nr) * heads;
+    return q;
+}
+
+// 4 codes -> two registers of two fp16 each (elements 0, 1 and 2, 3 of the word), exactly.
+template <int CODE>
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& a, uint32_t& b) {
+    if (CODE == RMOE_KV_INT8) {
+        // 0x6400 | u is 1024 + u for a byte u; u = code + 128
+        const uint32_t u = w ^ 0x80808080u;
+        const uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
+        const __half2 c = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
+        const __half2 p = __hsub2(*reinterpret_cast<const __half2*>(&x), c), q = __hsub2(*reinterpret_cast<const __half2*>(&y), c);
+        a = *reinterpret_cast<const uint32_t*>(&p);
+        b = *reinterpret_cast<const uint32_t*>(&q);
+    } else {
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}\n"
+            : "=r"(a), "=r"(b) : "r"(w));
+    }
+}
+
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(a));
+    return v;
+}
+
+struct SplitPiece {   // where a piece belongs
+    int64_t a;        // the item's first unit
+    int tiles;
+    int q0, n, row0, head;
+    int flags;        // 1: valid, 2: holds the item's first tile, 4: holds its last
+};
+
+template <typename T, int CODE, int D, int NR>
+__global__ void __launch_bounds__(SPLIT_NW * 32, 1)
+kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, KvArg kv, AttendArg a,
+                SplitWs ws) {
+    using S = SplitShape<D>;
+    using M = SplitSmem<D, NR>;
+    constexpr int NW = SPLIT_NW, NT = NW * 32, DEPTH = SPLIT_DEPTH, TW = S::TW, MT = S::MT, KS = S::KS, HF = S::HF;
+    constexpr int QT = NR / 8;                 // n-tiles of 8 rows
+    constexpr bool PAIR = sizeof(T) == 4;      // f32: hi + lo
+    constexpr int VB = D == 64 ? 8 : 16;       // V bytes per lane, token and 128-byte box
+    constexpr int BX = D == 256 ? 2 : 1;       // 128-byte boxes per row
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t s_full[NW][DEPTH];
+    __shared__ float s_scale[NW][DEPTH][2][2];  // per box of the tile: K scale (-1: no such block), V scale
+    __shared__ int64_t s_pre[NT];
+    __shared__ int64_t s_tot[NW];
+    __shared__ SplitPiece s_piece[2 * NW];
+    __shared__ int s_last;
+
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, c = lane & 3;
+    const uint32_t ring0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* ring_ptr = smem_raw + (ring0 - smem_u32(smem_raw));
+    const int heads = kv.heads, bs = kv.bs, group = a.q.heads / heads;
+
+    // ---- tokens of no request ----
+    {
+        const int first = min(max(__ldg(a.cu), 0), a.T), end = min(max(__ldg(a.cu + a.R), first), a.T);
+        const int64_t rest = (int64_t)(a.T - (end - first)) * a.q.heads;
+        for (int64_t i = (int64_t)blockIdx.x * NW + w; i < rest; i += (int64_t)gridDim.x * NW) {
+            const int k = (int)(i / a.q.heads), h = (int)(i % a.q.heads), t = k < first ? k : end + (k - first);
+            T* o = reinterpret_cast<T*>(a.out.p) + t * a.out.st + h * a.out.sh;
+            for (int d = lane; d < D; d += 32) o[d] = Elt<T>::put(0.0f);
+            if (lane == 0 && a.lse) a.lse[(int64_t)t * a.q.heads + h] = -INFINITY;
+        }
+    }
+
+    // ---- this CTA's share of the units ----
+    const int per = (a.R + NT - 1) / NT;
+    int64_t mine = 0;
+    for (int r = tid * per; r < min(a.R, (tid + 1) * per); r++) {
+        const SplitReq q = split_req(a, r, heads, group, bs, NR, TW);
+        mine += (int64_t)q.items * q.tiles;
+    }
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+    }
+    if (lane == 31) s_tot[w] = incl;
+    if (tid < 2 * NW) s_piece[tid].flags = 0;
+    if (lane == 0) {
+        for (int i = 0; i < DEPTH; i++) tc::mbar_init(smem_u32(&s_full[w][i]), 1 + (bs < TW ? TW / bs : 1));
+        tc::fence_mbar_init();
+    }
+    __syncthreads();
+    int64_t before = 0, W = 0;
+#pragma unroll
+    for (int i = 0; i < NW; i++) {
+        if (i < w) before += s_tot[i];
+        W += s_tot[i];
+    }
+    s_pre[tid] = before + incl - mine;
+    __syncthreads();
+    // a share of less than a tile per warp would only add joining
+    const int64_t active = min((int64_t)gridDim.x, (W + NW - 1) / NW);
+    if (blockIdx.x >= active) return;
+    auto share = [&](int64_t cta) { return W * cta / active; };
+    const int64_t u0 = share(blockIdx.x), u1 = share(blockIdx.x + 1);
+    const int64_t wu0 = u0 + (u1 - u0) * w / NW, wu1 = u0 + (u1 - u0) * (w + 1) / NW;
+
+    if (wu0 < wu1) {
+        // ---- the request, item and tile of the warp's first unit ----
+        int lo = 0, hi = NT - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (s_pre[mid] <= wu0) lo = mid; else hi = mid - 1;
+        }
+        int r = lo * per;
+        int64_t rem = wu0 - s_pre[lo];
+        SplitReq rq = split_req(a, r, heads, group, bs, NR, TW);
+        while (rem >= (int64_t)rq.items * rq.tiles) {
+            rem -= (int64_t)rq.items * rq.tiles;
+            rq = split_req(a, ++r, heads, group, bs, NR, TW);
+        }
+        int item = (int)(rem / rq.tiles), tile = (int)(rem % rq.tiles);
+
+        // ---- the issuing side: runs DEPTH tiles ahead ----
+        const int br = min(bs, TW), nb = TW / br;  // rows and number of a tile's boxes
+        SplitReq pq = rq;
+        int pr = r, pitem = item, ptile = tile;
+        int64_t pleft = wu1 - wu0;
+        int pblk = -1;
+        auto lookup = [&]() {  // lane b < nb: the block of box b of the tile to issue next
+            const int j = (pq.t0 + ptile) * TW + lane * br;
+            pblk = -1;
+            if (lane < nb && pleft > 0 && j < pq.hi) pblk = __ldg(a.table + (int64_t)pr * a.max_blocks + j / bs);
+        };
+        lookup();
+        auto issue = [&](int stage) {
+            const uint32_t bar = smem_u32(&s_full[w][stage]);
+            const int j = (pq.t0 + ptile) * TW + lane * br;
+            const bool want = lane < nb && j < pq.hi, ok = want && (unsigned)pblk < (unsigned)kv.n_blocks;
+            if (want && !ok) atomicOr(kv.status, (unsigned)DERR_INDEX);
+            const unsigned mask = __ballot_sync(0xffffffffu, ok);
+            if (lane == 0) tc::mbar_arrive_expect_tx(bar, __popc(mask) * br * D * 2);
+            __syncwarp();
+            if (ok) {
+                const int kh = pitem % heads;
+                const int64_t bh = (int64_t)pblk * heads + kh;
+                const int row = (int)(bh * bs + (j & (bs - 1)));
+                const uint32_t dst = ring0 + (w * DEPTH + stage) * S::STAGE + lane * br * (D < 128 ? D : 128);
+#pragma unroll
+                for (int x = 0; x < BX; x++) {
+                    tc::tma_2d(dst + x * TW * 128, &kmap, x * 128, row, bar);
+                    tc::tma_2d(dst + TW * D + x * TW * 128, &vmap, x * 128, row, bar);
+                }
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(smem_u32(&s_scale[w][stage][lane][0])), "l"(kv.ks + bh) : "memory");
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(smem_u32(&s_scale[w][stage][lane][1])), "l"(kv.vs + bh) : "memory");
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(bar) : "memory");
+            } else if (lane < nb) {
+                s_scale[w][stage][lane][0] = -1.0f;
+                s_scale[w][stage][lane][1] = 1.0f;
+                tc::mbar_arrive(bar);
+            }
+            if (--pleft > 0 && ++ptile == pq.tiles) {
+                ptile = 0;
+                if (++pitem == pq.items) {
+                    pitem = 0;
+                    do pq = split_req(a, ++pr, heads, group, bs, NR, TW);
+                    while (pq.items == 0);
+                }
+            }
+            lookup();
+        };
+        for (int i = 0; i < DEPTH; i++)
+            if (pleft > 0) issue(i);
+
+        // ---- the computing side ----
+        // position in a token group of 8 of the S^T row n, and of d chunks over the rows of O^T:
+        // the two rows of a quarter-warp's 16-byte reads then fall into different halves of the banks
+        const int tg = D == 64 ? g : (g >> 1) + 4 * (g & 1);
+        const int t2c = D == 64 ? 2 * c : c, t2c1 = D == 64 ? 2 * c + 1 : c + 4;  // rows 2c and 2c + 1
+        const int vg = (g >> 1) + 4 * (g & 1);
+        int64_t left = wu1 - wu0;
+        uint32_t cnt = 0;
+        bool dead = false, firstseg = true;
+        while (left > 0 && !dead) {
+            const int seg = (int)min(left, (int64_t)(rq.tiles - tile));
+            const int kh = item % heads, row0 = item / heads * NR;
+            // q rows as B operands, scaled to the fp16 range row by row
+            uint32_t qh[QT][KS][2], ql[PAIR ? QT : 1][PAIR ? KS : 1][2];
+            float qs[QT][2];
+            int vhi[QT][2], vlo[QT][2];
+#pragma unroll
+            for (int nt = 0; nt < QT; nt++) {
+                const int row = row0 + nt * 8 + g, tok = row / group;
+                const bool live = tok < rq.n;
+                const T* qp = reinterpret_cast<const T*>(a.q.p) + (int64_t)(rq.q0 + (live ? tok : 0)) * a.q.st +
+                              (int64_t)(kh * group + row % group) * a.q.sh;
+                float v[HF][16], mx = 0.0f;
+#pragma unroll
+                for (int hf = 0; hf < HF; hf++) {
+                    load8(qp + (hf * 4 + c) * 16, a.q.vec, v[hf]);
+                    load8(qp + (hf * 4 + c) * 16 + 8, a.q.vec, v[hf] + 8);
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        if (!live) v[hf][e] = 0.0f;
+                        mx = fmaxf(mx, fabsf(v[hf][e]));
+                    }
+                }
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                // 2^e with mx 2^-e in [2^13, 2^14); nothing to scale at 0 and at infinities
+                const int ex = (int)((__float_as_uint(mx) >> 23) & 0xffu) - 127 - 13;
+                const int e = mx > 0.0f && mx <= 3.4e38f ? max(-126, min(113, ex)) : 0;
+                const float dn = exp2i(-e);
+#pragma unroll
+                for (int hf = 0; hf < HF; hf++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int p = 0; p < 2; p++) {
+                            const float x = v[hf][4 * i + 2 * p] * dn, y = v[hf][4 * i + 2 * p + 1] * dn;
+                            const uint32_t hh = pack_f16x2(x, y);
+                            qh[nt][hf * 4 + i][p] = hh;
+                            if (PAIR) {
+                                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hh));
+                                ql[nt][hf * 4 + i][p] = pack_f16x2(x - f.x, y - f.y);
+                            }
+                        }
+                const float up = exp2i(e) * a.scale * 1.4426950408889634f;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {  // of the rows 2c, 2c + 1 whose sums this lane holds
+                    qs[nt][i] = __shfl_sync(0xffffffffu, up, (2 * c + i) * 4);
+                    const int t2 = (row0 + nt * 8 + 2 * c + i) / group, p = rq.pos0 + t2;
+                    vhi[nt][i] = t2 < rq.n ? min(p + 1, rq.hi) : 0;
+                    vlo[nt][i] = a.window ? max(0, p - a.window + 1) : 0;
+                }
+            }
+            // keys that every row of the tile sees: no masks there
+            const int last = min(rq.n - 1, (row0 + NR - 1) / group), firstt = row0 / group;
+            const int all_hi = min(rq.pos0 + firstt + 1, rq.hi);
+            const int all_lo = a.window ? max(0, rq.pos0 + last - a.window + 1) : 0;
+            const int any_lo = a.window ? max(0, rq.pos0 + firstt - a.window + 1) : 0;
+
+            float o[QT][KS][4], m[QT][2], l[QT][2];
+#pragma unroll
+            for (int nt = 0; nt < QT; nt++) {
+                m[nt][0] = m[nt][1] = -INFINITY;
+                l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < KS; i++) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f;
+            }
+            for (int s = 0; s < seg; s++, cnt++) {
+                const int stage = cnt % DEPTH;
+                if (!tc::mbar_wait(smem_u32(&s_full[w][stage]), (cnt / DEPTH) & 1)) {
+                    dead = true;
+                    break;
+                }
+                const uint32_t kb = ring0 + (w * DEPTH + stage) * S::STAGE, vb = kb + TW * D;
+                const int j0 = (rq.t0 + tile + s) * TW;
+                float kscale[MT], lv[MT], iv[MT];
+                bool gone = false;
+#pragma unroll
+                for (int i = 0; i < MT; i++) {
+                    const int b = MT == 2 && br == 16 ? i : 0;
+                    kscale[i] = s_scale[w][stage][b][0];
+                    const float vs = fmaxf(s_scale[w][stage][b][1], 7.8886090522101181e-31f);  // 2^-100
+                    lv[i] = log2f(vs);
+                    iv[i] = 1.0f / vs;
+                    gone |= kscale[i] < 0.0f;
+                }
+                const bool masked = gone || j0 < all_lo || j0 + TW > all_hi;
+                if (CODE == RMOE_KV_E4M3 && masked) {
+                    // places that no row sees may hold the format's NaN, and 0 * NaN is NaN
+                    for (int i = lane; i < TW * (D / 16); i += 32) {
+                        const int t = i / (D / 16), ch = i % (D / 16), j = j0 + t;
+                        const bool no = j >= rq.hi || j < any_lo || (MT == 2 && t >= 16 ? kscale[MT - 1] : kscale[0]) < 0.0f;
+                        // whole rows are cleared, so the swizzle inside a row does not matter
+                        if (no)
+                            *reinterpret_cast<uint4*>(ring_ptr + (vb - ring0) + (D == 256 ? (ch / 8) * TW * 128 + t * 128 + (ch % 8) * 16 : t * D + ch * 16)) =
+                                make_uint4(0, 0, 0, 0);
+                    }
+                    tc::fence_proxy_async_smem();  // before the next copy into this stage
+                    __syncwarp();
+                }
+                // S^T = K q^T: rows tokens, columns query rows.  The tensor cores cut the sums of a
+                // chain of products short at each step, so a chain is 64 elements long and the
+                // chains are added by the f32 unit (256 elements in one chain cost 1e-5 of the
+                // score); the low halves have their own chain.
+                float st[QT][MT][4], su[PAIR ? QT : 1][PAIR ? MT : 1][4];
+#pragma unroll
+                for (int nt = 0; nt < QT; nt++)
+#pragma unroll
+                    for (int i = 0; i < MT; i++) {
+                        st[nt][i][0] = st[nt][i][1] = st[nt][i][2] = st[nt][i][3] = 0.0f;
+                        if (PAIR) su[nt][i][0] = su[nt][i][1] = su[nt][i][2] = su[nt][i][3] = 0.0f;
+                    }
+#pragma unroll
+                for (int hf = 0; hf < HF; hf++)
+#pragma unroll
+                    for (int i = 0; i < MT; i++) {
+                        uint4 x[2];
+#pragma unroll
+                        for (int z = 0; z < 2; z++) {
+                            const int row = 16 * i + 8 * z + tg;
+                            x[z] = D == 64 ? lds128(kb + row * 64 + ((c ^ ((row >> 1) & 3)) << 4))
+                                           : lds128(kb + (hf / 2) * TW * 128 + row * 128 + ((((hf & 1) * 4 + c) ^ (row & 7)) << 4));
+                        }
+                        float ch[QT][4];
+#pragma unroll
+                        for (int nt = 0; nt < QT; nt++) ch[nt][0] = ch[nt][1] = ch[nt][2] = ch[nt][3] = 0.0f;
+                        const uint32_t x0[4] = {x[0].x, x[0].y, x[0].z, x[0].w}, x1[4] = {x[1].x, x[1].y, x[1].z, x[1].w};
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            uint32_t f[4];
+                            widen4<CODE>(x0[k], f[0], f[2]);
+                            widen4<CODE>(x1[k], f[1], f[3]);
+#pragma unroll
+                            for (int nt = 0; nt < QT; nt++) {
+                                mma_f16_16816(ch[nt], f, qh[nt][hf * 4 + k][0], qh[nt][hf * 4 + k][1]);
+                                if (PAIR) mma_f16_16816(su[nt][i], f, ql[nt][hf * 4 + k][0], ql[nt][hf * 4 + k][1]);
+                            }
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < QT; nt++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) st[nt][i][e] += ch[nt][e];
+                    }
+                // weights
+                uint32_t ph[QT][MT][2], pl[PAIR ? QT : 1][MT][2];
+#pragma unroll
+                for (int nt = 0; nt < QT; nt++) {
+                    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < MT; i++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int q = e & 1, j = j0 + 16 * i + 8 * (e >> 1) + tg;
+                            float x = fmaf(PAIR ? st[nt][i][e] + su[nt][i][e] : st[nt][i][e], qs[nt][q] * kscale[i], lv[i]);
+                            if (masked && (j >= vhi[nt][q] || j < vlo[nt][q] || kscale[i] < 0.0f)) x = -INFINITY;
+                            st[nt][i][e] = x;
+                            mx[q] = fmaxf(mx[q], x);
+                        }
+                    float al[2], mu[2];
+#pragma unroll
+                    for (int q = 0; q < 2; q++) {
+                        mx[q] = fmaxf(mx[q], __shfl_xor_sync(0xffffffffu, mx[q], 4));
+                        mx[q] = fmaxf(mx[q], __shfl_xor_sync(0xffffffffu, mx[q], 8));
+                        mx[q] = fmaxf(mx[q], __shfl_xor_sync(0xffffffffu, mx[q], 16));
+                        const float mn = fmaxf(m[nt][q], mx[q]);
+                        mu[q] = mn == -INFINITY ? 0.0f : mn;
+                        al[q] = ex2(m[nt][q] - mu[q]);
+                        m[nt][q] = mn;
+                    }
+                    if (__any_sync(0xffffffffu, al[0] != 1.0f || al[1] != 1.0f)) {
+                        l[nt][0] *= al[0];
+                        l[nt][1] *= al[1];
+#pragma unroll
+                        for (int i = 0; i < KS; i++) {
+                            o[nt][i][0] *= al[0];
+                            o[nt][i][1] *= al[1];
+                            o[nt][i][2] *= al[0];
+                            o[nt][i][3] *= al[1];
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < MT; i++) {
+                        float p[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            p[e] = ex2(st[nt][i][e] - mu[e & 1]);
+                            l[nt][e & 1] = fmaf(p[e], iv[i], l[nt][e & 1]);
+                        }
+#pragma unroll
+                        for (int z = 0; z < 2; z++) {
+                            const uint32_t hh = pack_f16x2(p[2 * z], p[2 * z + 1]);
+                            ph[nt][i][z] = movmatrix(hh);
+                            if (PAIR) {
+                                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hh));
+                                pl[nt][i][z] = movmatrix(pack_f16x2(p[2 * z] - f.x, p[2 * z + 1] - f.y));
+                            }
+                        }
+                    }
+                }
+                // O^T += V^T P^T: rows head elements, columns query rows
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+#pragma unroll
+                    for (int x = 0; x < BX; x++) {
+                        uint32_t v[4][VB / 4];
+#pragma unroll
+                        for (int z = 0; z < 4; z++) {
+                            const int row = 16 * i + 8 * (z >> 1) + ((z & 1) ? t2c1 : t2c);
+                            if (D == 64) {
+                                const uint2 y = lds64(vb + row * 64 + (((vg >> 1) ^ ((row >> 1) & 3)) << 4) + (vg & 1) * 8);
+                                v[z][0] = y.x;
+                                v[z][1] = y.y;
+                            } else {
+                                const uint4 y = lds128(vb + x * TW * 128 + row * 128 + ((vg ^ (row & 7)) << 4));
+                                v[z][0] = y.x;
+                                v[z][1] = y.y;
+                                v[z][VB / 4 - 2] = y.z;
+                                v[z][VB / 4 - 1] = y.w;
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < VB / 4; k++) {
+                            uint32_t f[2][4];  // of the two O^T tiles of this word
+                            widen4<CODE>(__byte_perm(v[0][k], v[1][k], 0x5140), f[0][0], f[0][1]);
+                            widen4<CODE>(__byte_perm(v[2][k], v[3][k], 0x5140), f[0][2], f[0][3]);
+                            widen4<CODE>(__byte_perm(v[0][k], v[1][k], 0x7362), f[1][0], f[1][1]);
+                            widen4<CODE>(__byte_perm(v[2][k], v[3][k], 0x7362), f[1][2], f[1][3]);
+#pragma unroll
+                            for (int nt = 0; nt < QT; nt++)
+#pragma unroll
+                                for (int y = 0; y < 2; y++) {
+                                    float* acc = o[nt][x * 8 + 2 * k + y];
+                                    mma_f16_16816(acc, f[y], ph[nt][i][0], ph[nt][i][1]);
+                                    if (PAIR) mma_f16_16816(acc, f[y], pl[nt][i][0], pl[nt][i][1]);
+                                }
+                        }
+                    }
+                __syncwarp();  // every lane has read the stage
+                if (pleft > 0) issue(stage);
+            }
+            if (dead) break;
+            // ---- the item's share is done ----
+#pragma unroll
+            for (int nt = 0; nt < QT; nt++)
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    l[nt][q] += __shfl_xor_sync(0xffffffffu, l[nt][q], 4);
+                    l[nt][q] += __shfl_xor_sync(0xffffffffu, l[nt][q], 8);
+                    l[nt][q] += __shfl_xor_sync(0xffffffffu, l[nt][q], 16);
+                }
+            const bool starts = tile == 0, ends = tile + seg == rq.tiles;
+            if (starts && ends) {
+#pragma unroll
+                for (int nt = 0; nt < QT; nt++)
+#pragma unroll
+                    for (int q = 0; q < 2; q++) {
+                        const int row = row0 + nt * 8 + 2 * c + q, tok = row / group;
+                        if (tok >= rq.n) continue;
+                        const int h = kh * group + row % group;
+                        const float inv = l[nt][q] > 0.0f ? 1.0f / l[nt][q] : (l[nt][q] == 0.0f ? 0.0f : l[nt][q]);
+                        T* op = reinterpret_cast<T*>(a.out.p) + (int64_t)(rq.q0 + tok) * a.out.st + h * a.out.sh;
+#pragma unroll
+                        for (int x = 0; x < BX; x++)
+#pragma unroll
+                            for (int b = 0; b < VB / 8; b++) {
+                                float v[8];
+#pragma unroll
+                                for (int e = 0; e < 8; e++) v[e] = o[nt][x * 8 + b * 4 + e / 2][(e & 1) * 2 + q] * inv;
+                                store8(op + x * 128 + vg * VB + b * 8, a.out.vec, v);
+                            }
+                        if (g == 0 && a.lse)
+                            a.lse[(int64_t)(rq.q0 + tok) * a.q.heads + h] =
+                                l[nt][q] == 0.0f ? -INFINITY : (m[nt][q] + log2f(l[nt][q])) * 0.69314718055994531f;
+                    }
+            } else {
+                const bool into_first = firstseg && left > seg;  // the ring is still in use then
+                float* pc = into_first ? reinterpret_cast<float*>(ring_ptr + M::RING) + w * M::PIECE
+                                       : reinterpret_cast<float*>(ring_ptr + w * DEPTH * S::STAGE);
+#pragma unroll
+                for (int nt = 0; nt < QT; nt++)
+#pragma unroll
+                    for (int q = 0; q < 2; q++) {
+                        const int row = nt * 8 + 2 * c + q;
+                        if (g == 0) pc[row] = m[nt][q], pc[NR + row] = l[nt][q];
+                        float* po = pc + 2 * NR + row * D;
+#pragma unroll
+                        for (int x = 0; x < BX; x++)
+#pragma unroll
+                            for (int e = 0; e < VB; e++) po[x * 128 + vg * VB + e] = o[nt][x * 8 + e / 2][(e & 1) * 2 + q];
+                    }
+                if (lane == 0)
+                    s_piece[2 * w + (into_first ? 0 : 1)] =
+                        SplitPiece{wu1 - left - tile, rq.tiles, rq.q0, rq.n, row0, kh, 1 | (starts ? 2 : 0) | (ends ? 4 : 0)};
+            }
+            firstseg = false;
+            left -= seg;
+            tile += seg;
+            if (left > 0 && tile == rq.tiles) {
+                tile = 0;
+                if (++item == rq.items) {
+                    item = 0;
+                    do rq = split_req(a, ++r, heads, group, bs, NR, TW);
+                    while (rq.items == 0);
+                }
+            }
+        }
+        if (dead) {  // a copy did not arrive: say so, and let what is in flight land
+            if (lane == 0) atomicOr(kv.status, (unsigned)DERR_TIMEOUT);
+            for (int64_t k = (wu1 - wu0) - pleft; (int64_t)cnt < k; cnt++)
+                tc::mbar_wait(smem_u32(&s_full[w][cnt % DEPTH]), (cnt / DEPTH) & 1);
+        }
+    }
+
+    // ---- joining ----
+    __syncthreads();
+    auto piece_ptr = [&](int i) {
+        return (i & 1) ? reinterpret_cast<const float*>(ring_ptr + (i >> 1) * DEPTH * S::STAGE)
+                       : reinterpret_cast<const float*>(ring_ptr + M::RING) + (i >> 1) * M::PIECE;
+    };
+    // (M, l, o) of element (row, d) over n pieces at get(i)
+    auto join = [&](int n, auto get, int row, int d, float& mm, float& ll, float& oo) {
+        mm = -INFINITY;
+        for (int i = 0; i < n; i++) mm = fmaxf(mm, __ldcg(get(i) + row));
+        const float mu = mm == -INFINITY ? 0.0f : mm;
+        ll = oo = 0.0f;
+        for (int i = 0; i < n; i++) {
+            const float* p = get(i);
+            const float f = ex2(__ldcg(p + row) - mu);
+            ll = fmaf(__ldcg(p + NR + row), f, ll);
+            oo = fmaf(__ldcg(p + 2 * NR + row * D + d), f, oo);
+        }
+    };
+    auto emit = [&](const SplitPiece& pc, int row, int d, float mm, float ll, float oo) {
+        const int rr = pc.row0 + row, tok = rr / group;
+        if (tok >= pc.n) return;
+        const int h = pc.head * group + rr % group;
+        reinterpret_cast<T*>(a.out.p)[(int64_t)(pc.q0 + tok) * a.out.st + (int64_t)h * a.out.sh + d] =
+            Elt<T>::put(ll > 0.0f ? oo / ll : (ll == 0.0f ? 0.0f : ll));
+        if (d == 0 && a.lse)
+            a.lse[(int64_t)(pc.q0 + tok) * a.q.heads + h] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.69314718055994531f;
+    };
+    for (int i = 0; i < 2 * NW;) {
+        if (!(s_piece[i].flags & 1)) { i++; continue; }
+        const SplitPiece pc = s_piece[i];
+        int idx[2 * NW], n = 0, k = i;
+        int flags = 0;
+        for (; k < 2 * NW; k++) {
+            if (!(s_piece[k].flags & 1)) continue;
+            if (s_piece[k].a != pc.a) break;
+            idx[n++] = k;
+            flags |= s_piece[k].flags;
+        }
+        i = k;
+        const bool whole = (flags & 6) == 6;
+        float* slot = ws.part + (size_t)(2 * blockIdx.x + ((flags & 2) ? 1 : 0)) * M::PIECE;
+        for (int e = tid; e < NR * D; e += NT) {
+            const int row = e / D, d = e % D;
+            float mm = -INFINITY, ll = 0.0f, oo = 0.0f;
+            for (int x = 0; x < n; x++) mm = fmaxf(mm, piece_ptr(idx[x])[row]);
+            const float mu = mm == -INFINITY ? 0.0f : mm;
+            for (int x = 0; x < n; x++) {
+                const float* p = piece_ptr(idx[x]);
+                const float f = ex2(p[row] - mu);
+                ll = fmaf(p[NR + row], f, ll);
+                oo = fmaf(p[2 * NR + row * D + d], f, oo);
+            }
+            if (whole) {
+                emit(pc, row, d, mm, ll, oo);
+            } else {
+                if (d == 0) slot[row] = mm, slot[NR + row] = ll;
+                slot[2 * NR + row * D + d] = oo;
+            }
+        }
+        if (whole) continue;
+        // the CTAs that hold the item's first and last unit
+        auto cta_of = [&](int64_t u) {
+            int64_t x = u * active / W;
+            while (share(x + 1) <= u) x++;
+            while (share(x) > u) x--;
+            return (int)x;
+        };
+        const int c0 = cta_of(pc.a), c1 = cta_of(pc.a + pc.tiles - 1);
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) s_last = atomicAdd(ws.ticket + c0, 1u) == (unsigned)(c1 - c0);
+        __syncthreads();
+        if (s_last) {
+            __threadfence();
+            auto get = [&](int x) { return ws.part + (size_t)(2 * (c0 + x) + (x == 0 ? 1 : 0)) * M::PIECE; };
+            for (int e = tid; e < NR * D; e += NT) {
+                float mm, ll, oo;
+                join(c1 - c0 + 1, get, e / D, e % D, mm, ll, oo);
+                emit(pc, e / D, e % D, mm, ll, oo);
+            }
+            if (tid == 0) ws.ticket[c0] = 0;
+        }
+        __syncthreads();
+    }
+}
+
+template <typename T, int CODE, int D, int NR>
+static cudaError_t split_launch(const KvMaps& maps, const KvArg& kv, const AttendArg& a, const SplitWs& ws, int sms, cudaStream_t s) {
+    constexpr int smem = SplitSmem<D, NR>::TOTAL;
+    static_assert(SplitSmem<D, NR>::PIECE * 4 <= SPLIT_DEPTH * SplitShape<D>::STAGE, "a last piece takes the place of the ring");
+    auto k = kv_split_kernel<T, CODE, D, NR>;
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    k<<<sms, SPLIT_NW * 32, smem, s>>>(maps.k, maps.v, kv, a, ws);
+    return cudaGetLastError();
+}
+
+// nr: 8 or 16 rows per item (16 only up to head_dim 128: the accumulators of 256 would spill)
+template <typename T, int CODE>
+static cudaError_t split_dims(const KvMaps& maps, const KvArg& kv, const AttendArg& a, const SplitWs& ws, int sms, int nr,
+                              cudaStream_t s) {
+    if (kv.dim == 64)
+        return nr == 8 ? split_launch<T, CODE, 64, 8>(maps, kv, a, ws, sms, s) : split_launch<T, CODE, 64, 16>(maps, kv, a, ws, sms, s);
+    if (kv.dim == 128)
+        return nr == 8 ? split_launch<T, CODE, 128, 8>(maps, kv, a, ws, sms, s) : split_launch<T, CODE, 128, 16>(maps, kv, a, ws, sms, s);
+    return split_launch<T, CODE, 256, 8>(maps, kv, a, ws, sms, s);
+}
+
+int split_tile_tokens(int dim) { return dim == 256 ? SplitShape<256>::TW : SplitShape<128>::TW; }
+size_t split_part_bytes(int dim) { return (size_t)(dim == 256 ? 8 : 16) * (dim + 2) * 4 * 2; }
+
+cudaError_t launch_split(const KvMaps& maps, const KvArg& kv, const AttendArg& a, const SplitWs& ws, int sms, int nr,
+                         uint32_t type, int code, cudaStream_t s) {
+    const bool i8 = code == RMOE_KV_INT8;
+    if (type == T_F32)
+        return i8 ? split_dims<float, RMOE_KV_INT8>(maps, kv, a, ws, sms, nr, s) : split_dims<float, RMOE_KV_E4M3>(maps, kv, a, ws, sms, nr, s);
+    if (type == T_F16)
+        return i8 ? split_dims<__half, RMOE_KV_INT8>(maps, kv, a, ws, sms, nr, s)
+                  : split_dims<__half, RMOE_KV_E4M3>(maps, kv, a, ws, sms, nr, s);
+    return i8 ? split_dims<__nv_bfloat16, RMOE_KV_INT8>(maps, kv, a, ws, sms, nr, s)
+              : split_dims<__nv_bfloat16, RMOE_KV_E4M3>(maps, kv, a, ws, sms, nr, s);
+}
+
+}  // namespace rmoe
