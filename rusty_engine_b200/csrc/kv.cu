@@ -73,7 +73,8 @@ rmoe_status rmoe_kv_create(const rmoe_kv_desc* d, rmoe_kv** out) {
                   : fail(RMOE_ERR_OOM, "cache memory: cudaMalloc of 2 x %llu bytes failed", (unsigned long long)bytes);
     }
     const uint32_t box = std::min<uint32_t>(kv->bs, split_tile_tokens((int)kv->dim));
-    if (!make_code_map(kv->k, rows, kv->dim, box, kv->split_maps.k) || !make_code_map(kv->v, rows, kv->dim, box, kv->split_maps.v)) {
+    if (!make_code_map(kv->k, rows, kv->dim, box, kv->split_maps.k) || !make_code_map(kv->v, rows, kv->dim, box, kv->split_maps.v) ||
+        !make_code_map(kv->k, rows, kv->dim, kv->bs, kv->prompt_maps.k) || !make_code_map(kv->v, rows, kv->dim, kv->bs, kv->prompt_maps.v)) {
         delete kv;
         return fail(RMOE_ERR_CUDA, "cuTensorMapEncodeTiled failed for the cache");
     }

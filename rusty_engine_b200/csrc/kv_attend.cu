@@ -1,4 +1,6 @@
 // kv_attend.cu -- attention over the 8-bit paged cache: checks, and the choice of kernel.
+#include <algorithm>
+
 #include "kv_attend.h"
 
 using namespace rmoe;
@@ -23,11 +25,17 @@ extern "C" rmoe_status rmoe_kv_attend(rmoe_kv* kv, const rmoe_kv_attend_args* a,
     DeviceGuard g(kv->device);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const KvArg ka = kv_arg(kv);
-    p.split_rows = INT64_MAX;
+    const uint64_t group = a->q.heads / kv->heads;
+    // Without a bound on any request's new tokens: one each when there are as many tokens as
+    // requests.  A wrong guess costs time only, the split kernel takes whatever the other does not.
+    const uint64_t longest = std::min<uint64_t>(a->max_new ? a->max_new : a->T > a->R ? a->T : 1, a->T);
+    p.prompts = kv->dim <= 128 && longest * group >= PROMPT_MIN_ROWS &&
+                (a->T * group / PROMPT_PAIR_ROWS + std::min(a->R, a->T)) * kv->heads >= PROMPT_MIN_CTAS;
+    cudaError_t e = p.prompts ? launch_prompt(kv->prompt_maps, ka, p, a->type, (int)kv->code, s) : cudaSuccess;
     // 16 rows per item where a request has more than 8 on average: the cache is read once for them
-    const uint64_t group = a->q.heads / kv->heads, mean = group * ((a->T + a->R - 1) / a->R);
+    const uint64_t mean = group * (p.prompts ? 1 : (a->T + a->R - 1) / a->R);
     const int nr = mean > 8 && kv->dim <= 128 ? 16 : 8;
-    cudaError_t e = launch_split(kv->split_maps, ka, p, SplitWs{kv->split_part, kv->split_ticket}, kv->sms, nr, a->type,
-                                 (int)kv->code, s);
+    if (e == cudaSuccess)
+        e = launch_split(kv->split_maps, ka, p, SplitWs{kv->split_part, kv->split_ticket}, kv->sms, nr, a->type, (int)kv->code, s);
     return e == cudaSuccess ? RMOE_OK : cuda_fail(e, "kv attend launch");
 }

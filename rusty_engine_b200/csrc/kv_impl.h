@@ -26,6 +26,7 @@ struct rmoe_kv {
     float *ks = nullptr, *vs = nullptr;
     unsigned* status = nullptr;
     rmoe::KvMaps split_maps{};     // boxes of a split-kernel tile
+    rmoe::KvMaps prompt_maps{};    // boxes of a prompt-kernel tile: a block
     int sms = 0;
     float* split_part = nullptr;   // split kernel: pieces of items that span CTAs
     unsigned* split_ticket = nullptr;

@@ -1,0 +1,517 @@
+// kv_prompt.cu -- attention over the 8-bit paged cache for many query rows: prompts and chunks of
+// them, on the tensor cores (tcgen05).  head_dim 64 and 128.
+//
+// Mathematics: as in kv_split.cu,  out = sum_j 2^(x_j - M) vc_j / sum_j 2^(x_j - M) / vs_j  with
+// x_j = scale log2(e) ks_j q.kc_j + log2(vs_j).  A row may be any (token, query head) of the kv
+// head, so the rows of a CTA are 128-row tiles of consecutive (token, head of the group).
+//
+// Roles of the CTA's 16 warps: one brings raw 8-bit tiles of 128 keys by TMA, four widen them to
+// fp16 operand tiles (128-byte swizzle; K as the K-major and V as the MN-major operand, both in
+// the cache's own [key][element] order), one issues the products, and eight read S out of tensor
+// memory, one row per thread.
+//   16-bit calls: two row tiles share every K / V tile (the widening is paid once for 256 rows);
+//     while one tile's softmax runs, the other's products do.  P goes back to tensor memory as
+//     fp16 over its own S and is the A operand from there.  O stays in tensor memory; it is only
+//     rescaled when a row's maximum grew by more than 2^8 (P then stays below 2^8, exact in
+//     range), by the softmax threads.
+//   f32 calls: q and P are fp16 pairs (hi + lo, twice the products), one row tile, S in two
+//     buffers.  The tensor cores cut every partial sum short, about 2^-24 per step and all one
+//     way, which over a long row is more than f32 attention may lose; so each key tile has its own
+//     O in tensor memory, and the other four warps add the tiles up in registers.
+#include "kv_attend.h"
+#include "kv_widen.cuh"
+#include "rope.cuh"
+#include "tc_ptx.cuh"
+
+namespace rmoe {
+
+static constexpr int PT = 512;    // threads
+static constexpr int PKV = 128;   // keys per tile
+
+template <int D, bool PAIR>
+struct PromptShape {
+    static constexpr int NRT = PAIR ? 1 : 2;             // row tiles
+    static constexpr int QB = 128 * D * 2;               // fp16 bytes of a Q, K or V tile
+    static constexpr int RAW = PKV * D;
+    static constexpr int KN = 2, VN = PAIR ? 1 : 2;      // operand buffers
+    static constexpr int Q0 = 0, K0 = 2 * QB, V0 = K0 + KN * QB, R0 = V0 + VN * QB, END = R0 + 2 * RAW;
+    static constexpr int SMEM = END + 1024;              // + alignment
+};
+
+struct PromptBars {
+    uint64_t q_full, raw_full[2], raw_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2],
+        o_empty[2], meta_full[4], drain;
+};
+
+template <typename T, int CODE, int D>
+__global__ void __launch_bounds__(PT, 1)
+kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, KvArg kv, AttendArg a) {
+    constexpr bool PAIR = sizeof(T) == 4;
+    using S = PromptShape<D, PAIR>;
+    constexpr int NRT = S::NRT, KN = S::KN, VN = S::VN, CH = D / 32;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ PromptBars bars;
+    __shared__ uint32_t s_tmem;
+    __shared__ int64_t s_sum[PT / 32];
+    __shared__ int s_req[2];
+    __shared__ float4 s_meta[4][PKV / 16];                // per 16 keys: K scale, log2 V scale, 1 / V scale, 1: no such block
+    __shared__ float s_alpha[PAIR ? 4 : 1][PAIR ? 128 : 1];  // f32: what the earlier tiles' O is multiplied by
+    __shared__ float s_fin[2][PAIR ? 128 : 1];            // f32: M and l of the rows
+
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, wg = w >> 2;
+    const int heads = kv.heads, bs = kv.bs, group = a.q.heads / heads;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+
+    // ---- which request, head and rows ----
+    const int64_t max_rows = split_max_rows(a, heads, group, s_sum);
+    if (max_rows == INT64_MAX) return;
+    auto rows_of = [&](int r) -> int64_t {
+        const int q0 = min(max(__ldg(a.cu + r), 0), a.T);
+        return (int64_t)max(0, min(__ldg(a.cu + r + 1), a.T) - q0) * group;
+    };
+    auto items_of = [&](int r) -> int64_t {
+        const int64_t rows = rows_of(r);
+        return rows > max_rows ? (rows + NRT * 128 - 1) / (NRT * 128) * heads : 0;
+    };
+    {
+        const int per = (a.R + PT - 1) / PT, r0 = min(a.R, tid * per), r1 = min(a.R, r0 + per);
+        int64_t mine = 0;
+        for (int r = r0; r < r1; r++) mine += items_of(r);
+        int64_t incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        if (lane == 31) s_sum[w] = incl;
+        if (tid == 0) s_req[0] = -1;
+        __syncthreads();
+        int64_t before = 0;
+        for (int i = 0; i < w; i++) before += s_sum[i];
+        int64_t at = before + incl - mine, me = blockIdx.x;
+        if (me >= at && me < at + mine) {
+            int r = r0;
+            while (me >= at + items_of(r)) at += items_of(r++);
+            s_req[0] = r;
+            s_req[1] = (int)(items_of(r) - 1 - (me - at));  // the request's last rows, which see most, first
+        }
+        __syncthreads();
+    }
+    const int r = s_req[0];
+    if (r < 0) return;
+    const int kh = s_req[1] % heads, row0 = s_req[1] / heads * (NRT * 128);
+    const int q0 = min(max(__ldg(a.cu + r), 0), a.T), n = max(0, min(__ldg(a.cu + r + 1), a.T) - q0);
+    const int len = __ldg(a.lens + r), pos0 = len - (__ldg(a.cu + r + 1) - __ldg(a.cu + r));
+    const int hi = (int)min((int64_t)max(len, 0), (int64_t)a.max_blocks * bs);
+    const int tok_last = min(n - 1, (row0 + NRT * 128 - 1) / group);
+    const int kmax = min(pos0 + tok_last + 1, hi), kmin = a.window ? max(0, pos0 + row0 / group - a.window + 1) : 0;
+    const int jt0 = kmin / PKV, nt = kmax > kmin ? (kmax + PKV - 1) / PKV - jt0 : 0;  // key tiles
+
+    if (tid == 0) {
+        tc::mbar_init(smem_u32(&bars.q_full), 4 * NRT);
+        for (int i = 0; i < 2; i++) {
+            tc::mbar_init(smem_u32(&bars.raw_full[i]), 1);
+            tc::mbar_init(smem_u32(&bars.raw_empty[i]), 4);
+            tc::mbar_init(smem_u32(&bars.k_full[i]), 4);
+            tc::mbar_init(smem_u32(&bars.k_empty[i]), 1);
+            tc::mbar_init(smem_u32(&bars.v_full[i]), 4);
+            tc::mbar_init(smem_u32(&bars.v_empty[i]), 1);
+            tc::mbar_init(smem_u32(&bars.s_full[i]), 1);
+            tc::mbar_init(smem_u32(&bars.p_full[i]), 4);
+            tc::mbar_init(smem_u32(&bars.o_full[i]), 1);
+            tc::mbar_init(smem_u32(&bars.o_empty[i]), 4);
+        }
+        for (int i = 0; i < 4; i++) tc::mbar_init(smem_u32(&bars.meta_full[i]), 1);
+        tc::mbar_init(smem_u32(&bars.drain), 1);
+        tc::fence_mbar_init();
+    }
+    if (w == 13) tc::tmem_alloc(smem_u32(&s_tmem), 512);
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tm = s_tmem;
+    // tensor memory columns: S (and P) of tile / buffer i at 128 i, O at 256 + 128 i
+    bool dead = false;
+    auto wait = [&](uint64_t& b, uint32_t parity) {  // by whole warps: all lanes go on, or none
+        if (!dead) dead = !__all_sync(0xffffffffu, tc::mbar_wait(smem_u32(&b), parity & 1));
+        return !dead;
+    };
+    auto wait1 = [&](uint64_t& b, uint32_t parity) {  // by one thread
+        if (!dead) dead = !tc::mbar_wait(smem_u32(&b), parity & 1);
+        return !dead;
+    };
+
+    if (w == 12) {
+        // ---- producer: raw tiles and the scales of their blocks ----
+        const int br = min(bs, PKV), nb = PKV / br;
+        auto lookup = [&](int j) {
+            const int t = (jt0 + j) * PKV + 16 * lane;
+            return j < nt && lane < 8 && t < kmax ? __ldg(a.table + (int64_t)r * a.max_blocks + t / bs) : -1;
+        };
+        int blk = lookup(0), issued = 0;
+        for (int j = 0; j < nt; j++) {
+            const int t = (jt0 + j) * PKV + 16 * lane;
+            const bool want = lane < 8 && t < kmax, ok = want && (unsigned)blk < (unsigned)kv.n_blocks;
+            if (want && !ok) atomicOr(kv.status, (unsigned)DERR_INDEX);
+            const int64_t bh = ok ? (int64_t)blk * heads + kh : 0;
+            const float ks = ok ? __ldg(kv.ks + bh) : 0.0f, vs = ok ? __ldg(kv.vs + bh) : 1.0f;
+            const int next = lookup(j + 1);
+            // lane b < nb: the box of block rows at key b * br
+            const int src = lane < nb ? lane * br / 16 : 0;
+            const int bblk = __shfl_sync(0xffffffffu, blk, src);
+            const bool bok = __shfl_sync(0xffffffffu, (int)ok, src) && lane < nb;
+            const unsigned mask = __ballot_sync(0xffffffffu, bok);
+            const int row = bok ? (int)(((int64_t)bblk * heads + kh) * bs) : 0;
+#pragma unroll
+            for (int v = 0; v < 2; v++) {
+                if (j > 0 && !wait(bars.raw_empty[v], j - 1)) break;
+                const uint32_t bar = smem_u32(&bars.raw_full[v]);
+                if (lane == 0) tc::mbar_arrive_expect_tx(bar, __popc(mask) * br * D);
+                __syncwarp();
+                if (bok) tc::tma_2d(base + S::R0 + v * S::RAW + lane * br * D, v ? &vmap : &kmap, 0, row, bar);
+                issued++;
+            }
+            if (dead) break;
+            if (lane < 8) {
+                const float f = v_scale_floor(vs);
+                s_meta[j & 3][lane] = make_float4(ks, log2f(f), 1.0f / f, ok ? 0.0f : 1.0f);
+            }
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(smem_u32(&bars.meta_full[j & 3]));
+            blk = next;
+        }
+        if (dead)  // let the copies in flight land
+            for (int v = 0; v < 2; v++) {
+                const int c = (issued + 1 - v) / 2;  // copies into buffer v
+                if (c > 0) tc::mbar_wait(smem_u32(&bars.raw_full[v]), (c - 1) & 1);
+            }
+    } else if (w == 13) {
+        // ---- products ----
+        if (lane == 0 && nt > 0) {
+            constexpr uint32_t idS = tc::idesc_f16(128, PKV), idO = tc::idesc_f16(128, D) | tc::IDESC_B_MN;
+            auto mma_s = [&](int q, uint32_t d, int j) {  // S = Q K^T of key tile j; q: the Q tile (lo half next to it)
+                const uint32_t kb = base + S::K0 + (j % KN) * S::QB;
+#pragma unroll
+                for (int half = PAIR ? 1 : 0; half >= 0; half--)
+#pragma unroll
+                    for (int k = 0; k < D / 16; k++) {
+                        const uint32_t off = (k / 4) * 16384 + (k % 4) * 32;
+                        tc::mma_ss(d, tc::smem_desc_sw128(base + S::Q0 + (q + half) * S::QB + off), tc::smem_desc_sw128(kb + off), idS,
+                                   k > 0 || (PAIR && half == 0));
+                    }
+            };
+            auto mma_o = [&](uint32_t d, uint32_t p, int j, bool add) {  // O (+)= P V
+                const uint32_t vb = base + S::V0 + (j % VN) * S::QB;
+#pragma unroll
+                for (int half = PAIR ? 1 : 0; half >= 0; half--)
+#pragma unroll
+                    for (int k = 0; k < PKV / 16; k++)
+                        tc::mma_ts(d, p + (k / 2) * 32 + (k % 2) * 8 + half * 16, tc::smem_desc_mn_sw128(vb + k * 2048, PKV * 128), idO,
+                                   add || k > 0 || (PAIR && half == 0));
+            };
+            if (wait1(bars.q_full, 0) && wait1(bars.k_full[0], 0)) {
+                tc::fence_after_sync();
+                for (int t = 0; t < NRT; t++) {
+                    mma_s(t, tm + t * 128, 0);
+                    tc::mma_commit(smem_u32(&bars.s_full[t]));
+                }
+                tc::mma_commit(smem_u32(&bars.k_empty[0]));
+            }
+            for (int j = 0; j < nt && !dead; j++) {
+                if (PAIR) {
+                    if (j + 1 < nt) {
+                        if (!wait1(bars.k_full[(j + 1) % KN], (j + 1) / KN)) break;
+                        tc::fence_after_sync();
+                        mma_s(0, tm + ((j + 1) & 1) * 128, j + 1);
+                        tc::mma_commit(smem_u32(&bars.s_full[(j + 1) & 1]));
+                        tc::mma_commit(smem_u32(&bars.k_empty[(j + 1) % KN]));
+                    }
+                    if (!wait1(bars.v_full[j % VN], j / VN) || !wait1(bars.p_full[j & 1], j / 2)) break;
+                    if (j >= 2 && !wait1(bars.o_empty[j & 1], j / 2 - 1)) break;
+                    tc::fence_after_sync();
+                    mma_o(tm + 256 + (j & 1) * 128, tm + (j & 1) * 128, j, false);
+                    tc::mma_commit(smem_u32(&bars.o_full[j & 1]));
+                    tc::mma_commit(smem_u32(&bars.v_empty[j % VN]));
+                } else {
+                    for (int t = 0; t < NRT; t++) {
+                        if (t == 0 && !wait1(bars.v_full[j % VN], j / VN)) break;
+                        if (!wait1(bars.p_full[t], j)) break;
+                        tc::fence_after_sync();
+                        mma_o(tm + 256 + t * 128, tm + t * 128, j, j > 0);
+                        tc::mma_commit(smem_u32(&bars.o_full[t]));
+                        if (t == NRT - 1) tc::mma_commit(smem_u32(&bars.v_empty[j % VN]));
+                        if (j + 1 < nt) {
+                            if (t == 0 && !wait1(bars.k_full[(j + 1) % KN], (j + 1) / KN)) break;
+                            tc::fence_after_sync();
+                            mma_s(t, tm + t * 128, j + 1);
+                            tc::mma_commit(smem_u32(&bars.s_full[t]));
+                            if (t == NRT - 1) tc::mma_commit(smem_u32(&bars.k_empty[(j + 1) % KN]));
+                        }
+                    }
+                }
+            }
+            tc::mma_commit(smem_u32(&bars.drain));  // nothing may run into freed tensor memory
+            if (!tc::mbar_wait(smem_u32(&bars.drain), 0)) dead = true;
+        }
+    } else if (wg == 2) {
+        // ---- widening: one key per thread ----
+        const int row = tid - 256;
+        for (int j = 0; j < nt; j++) {
+            if (!wait(bars.meta_full[j & 3], j >> 2)) break;
+            const int key = (jt0 + j) * PKV + row;
+            // keys that no row sees may hold anything, NaN codes too, and 0 * NaN is NaN
+            const bool live = key < kmax && key >= kmin && s_meta[j & 3][row >> 4].w == 0.0f;
+#pragma unroll
+            for (int v = 0; v < 2; v++) {
+                const int nbuf = v ? VN : KN, b = j % nbuf;
+                if (!wait(bars.raw_full[v], j)) break;
+                if (j >= nbuf && !wait(v ? bars.v_empty[b] : bars.k_empty[b], j / nbuf - 1)) break;
+                const uint32_t src = base + S::R0 + v * S::RAW, dst = base + (v ? S::V0 : S::K0) + b * S::QB + row * 128;
+#pragma unroll
+                for (int c = 0; c < D / 16; c++) {
+                    const uint4 x = D == 64 ? lds128(src + row * 64 + ((c ^ ((row >> 1) & 3)) << 4))
+                                            : lds128(src + row * 128 + ((c ^ (row & 7)) << 4));
+                    uint32_t y[8];
+                    widen4<CODE>(x.x, y[0], y[1]);
+                    widen4<CODE>(x.y, y[2], y[3]);
+                    widen4<CODE>(x.z, y[4], y[5]);
+                    widen4<CODE>(x.w, y[6], y[7]);
+                    if (!live)
+#pragma unroll
+                        for (int i = 0; i < 8; i++) y[i] = 0;
+                    const uint32_t d = dst + (c / 4) * 16384;
+                    sts128(d + (((2 * c & 7) ^ (row & 7)) << 4), make_uint4(y[0], y[1], y[2], y[3]));
+                    sts128(d + (((2 * c + 1 & 7) ^ (row & 7)) << 4), make_uint4(y[4], y[5], y[6], y[7]));
+                }
+                tc::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    tc::mbar_arrive(smem_u32(v ? &bars.v_full[b] : &bars.k_full[b]));
+                    tc::mbar_arrive(smem_u32(&bars.raw_empty[v]));
+                }
+            }
+            if (dead) break;
+        }
+    } else if (wg < NRT || (PAIR && wg == 1)) {
+        const int rt = PAIR ? 0 : wg, lrow = tid & 127;
+        const uint32_t tl = tm + ((uint32_t)((w & 3) * 32) << 16);
+        const int row = row0 + rt * 128 + lrow, tok = row / group, h = kh * group + row % group;
+        const bool live = tok < n;
+        T* op = reinterpret_cast<T*>(a.out.p) + (int64_t)(q0 + (live ? tok : 0)) * a.out.st + (int64_t)h * a.out.sh;
+        auto finish = [&](int c, const float* v, float l) {  // 32 elements of the row
+            const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+            float y[32];
+#pragma unroll
+            for (int i = 0; i < 32; i++) y[i] = l == 0.0f ? 0.0f : v[i] * inv;
+            if (live)
+#pragma unroll
+                for (int i = 0; i < 4; i++) store8(op + c * 32 + i * 8, a.out.vec, y + i * 8);
+        };
+        auto put_lse = [&](float m, float l) {
+            if (live && a.lse) a.lse[(int64_t)(q0 + tok) * a.q.heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+        };
+        if (PAIR && wg == 1) {
+            // ---- f32: adding up the tiles' O ----
+            float acc[D];
+#pragma unroll
+            for (int i = 0; i < D; i++) acc[i] = 0.0f;
+            for (int j = 0; j < nt; j++) {
+                if (!wait(bars.o_full[j & 1], j / 2)) break;
+                tc::fence_after_sync();
+                const float al = s_alpha[PAIR ? j & 3 : 0][PAIR ? lrow : 0];
+#pragma unroll
+                for (int c = 0; c < CH; c++) {
+                    uint32_t v[32];
+                    tc::tmem_ld32(tl + 256 + (j & 1) * 128 + c * 32, v);
+                    tc::tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; i++) acc[c * 32 + i] = fmaf(acc[c * 32 + i], al, __uint_as_float(v[i]));
+                }
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(smem_u32(&bars.o_empty[j & 1]));
+            }
+            if (!dead) {
+                const float l = nt > 0 ? s_fin[1][PAIR ? lrow : 0] : 0.0f;
+#pragma unroll
+                for (int c = 0; c < CH; c++) finish(c, acc + c * 32, l);
+                put_lse(nt > 0 ? s_fin[0][PAIR ? lrow : 0] : 0.0f, l);
+            }
+        } else {
+            // ---- q to operand tiles ----
+            const T* qp = reinterpret_cast<const T*>(a.q.p) + (int64_t)(q0 + (live ? tok : 0)) * a.q.st + (int64_t)h * a.q.sh;
+            float mx = 0.0f;
+            for (int c = 0; c < D / 8; c++) {
+                float v[8];
+                load8(qp + c * 8, a.q.vec, v);
+#pragma unroll
+                for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(v[i]));
+            }
+            const int e = q_exponent(mx);
+            const float dn = exp2i(-e), qs = exp2i(e) * a.scale * LOG2E;
+            for (int c = 0; c < D / 8; c++) {
+                float v[8];
+                load8(qp + c * 8, a.q.vec, v);
+                uint32_t hh[4], ll[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float x = live ? v[2 * i] * dn : 0.0f, y = live ? v[2 * i + 1] * dn : 0.0f;
+                    hh[i] = pack_f16x2(x, y);
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hh[i]));
+                    ll[i] = pack_f16x2(x - f.x, y - f.y);
+                }
+                const uint32_t d = base + S::Q0 + rt * S::QB + (c / 8) * 16384 + lrow * 128 + (((c & 7) ^ (lrow & 7)) << 4);
+                sts128(d, make_uint4(hh[0], hh[1], hh[2], hh[3]));
+                if (PAIR) sts128(d + S::QB, make_uint4(ll[0], ll[1], ll[2], ll[3]));
+            }
+            tc::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(smem_u32(&bars.q_full));
+            // ---- softmax ----
+            const int vhi = live ? min(pos0 + tok + 1, hi) : 0, vlo = a.window ? max(0, pos0 + tok - a.window + 1) : 0;
+            // keys that every row of the tile sees
+            const int first = (row0 + rt * 128) / group, last = min(n - 1, (row0 + rt * 128 + 127) / group);
+            const int all_hi = min(pos0 + first + 1, hi), all_lo = a.window ? max(0, pos0 + last - a.window + 1) : 0;
+            float m = -INFINITY, l = 0.0f;
+            for (int j = 0; j < nt; j++) {
+                const int sb = PAIR ? j & 1 : rt, key0 = (jt0 + j) * PKV;
+                const uint32_t sp = tl + sb * 128;
+                if (!wait(bars.meta_full[j & 3], j >> 2)) break;
+                const float4* meta = s_meta[j & 3];
+                bool masked = key0 < all_lo || key0 + PKV > all_hi;
+#pragma unroll
+                for (int i = 0; i < 8; i++) masked |= meta[i].w != 0.0f;
+                if (!wait(bars.s_full[sb], PAIR ? j / 2 : j)) break;
+                tc::fence_after_sync();
+                float mx = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    uint32_t v[32];
+                    tc::tmem_ld32(sp + c * 32, v);
+                    tc::tmem_ld_wait();
+#pragma unroll
+                    for (int g = 0; g < 2; g++) {
+                        const float4 mt = meta[2 * c + g];
+                        float x = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const int key = key0 + c * 32 + g * 16 + i;
+                            const float y = __uint_as_float(v[g * 16 + i]);
+                            if (!masked || (key < vhi && key >= vlo && mt.w == 0.0f)) x = fmaxf(x, y);
+                        }
+                        if (x != -INFINITY) mx = fmaxf(mx, fmaf(x, qs * mt.x, mt.y));
+                    }
+                }
+                // f32: M is the maximum; else it only moves when P could leave 2^8
+                const bool grow = PAIR ? mx > m : mx > m + 8.0f;
+                const float mn = grow ? mx : m, mu = mn == -INFINITY ? 0.0f : mn;
+                const float al = grow ? ex2(m - mu) : 1.0f;
+                if (PAIR) {
+                    s_alpha[PAIR ? j & 3 : 0][PAIR ? lrow : 0] = al;
+                } else if (j > 0 && __any_sync(0xffffffffu, grow && m != -INFINITY)) {
+                    if (!wait(bars.o_full[rt], j - 1)) break;
+                    tc::fence_after_sync();
+#pragma unroll
+                    for (int c = 0; c < CH; c++) {
+                        uint32_t v[32];
+                        tc::tmem_ld32(tl + 256 + rt * 128 + c * 32, v);
+                        tc::tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * al);
+                        tc::tmem_st32(tl + 256 + rt * 128 + c * 32, v);
+                    }
+                }
+                m = mn;
+                l *= al;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    uint32_t v[32], ph[16], pl[16];
+                    tc::tmem_ld32(sp + c * 32, v);
+                    tc::tmem_ld_wait();
+#pragma unroll
+                    for (int g = 0; g < 2; g++) {
+                        const float4 mt = meta[2 * c + g];
+                        const float sc = qs * mt.x, off = mt.y - mu;
+                        float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            float p[2];
+#pragma unroll
+                            for (int z = 0; z < 2; z++) {
+                                const int key = key0 + c * 32 + g * 16 + 2 * i + z;
+                                p[z] = ex2(fmaf(__uint_as_float(v[g * 16 + 2 * i + z]), sc, off));
+                                if (masked && !(key < vhi && key >= vlo && mt.w == 0.0f)) p[z] = 0.0f;
+                                sum[z] += p[z];
+                            }
+                            const uint32_t hh = pack_f16x2(p[0], p[1]);
+                            ph[g * 8 + i] = hh;
+                            if (PAIR) {
+                                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hh));
+                                pl[g * 8 + i] = pack_f16x2(p[0] - f.x, p[1] - f.y);
+                            }
+                        }
+                        l = fmaf(sum[0] + sum[1], mt.z, l);
+                    }
+                    tc::tmem_st16(sp + c * 32, ph);
+                    if (PAIR) tc::tmem_st16(sp + c * 32 + 16, pl);
+                }
+                if (PAIR && j == nt - 1) s_fin[0][PAIR ? lrow : 0] = m, s_fin[1][PAIR ? lrow : 0] = l;
+                tc::tmem_st_wait();
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(smem_u32(&bars.p_full[sb]));
+            }
+            if (!PAIR && !dead) {
+                if (nt == 0 || wait(bars.o_full[rt], nt - 1)) {
+                    tc::fence_after_sync();
+#pragma unroll
+                    for (int c = 0; c < CH; c++) {
+                        uint32_t v[32];
+                        if (nt > 0) {
+                            tc::tmem_ld32(tl + 256 + rt * 128 + c * 32, v);
+                            tc::tmem_ld_wait();
+                        }
+                        float f[32];
+#pragma unroll
+                        for (int i = 0; i < 32; i++) f[i] = nt > 0 ? __uint_as_float(v[i]) : 0.0f;
+                        finish(c, f, l);
+                    }
+                    put_lse(m, l);
+                }
+            }
+        }
+    }
+    if (dead && lane == 0) atomicOr(kv.status, (unsigned)DERR_TIMEOUT);
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    if (w == 13) tc::tmem_dealloc(tm, 512);
+}
+
+template <typename T, int CODE, int D>
+static cudaError_t prompt_launch(const KvMaps& maps, const KvArg& kv, const AttendArg& a, cudaStream_t s) {
+    using S = PromptShape<D, sizeof(T) == 4>;
+    auto k = kv_prompt_kernel<T, CODE, D>;
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    if (e != cudaSuccess) return e;
+    const int64_t group = a.q.heads / kv.heads, per = 128 * S::NRT;
+    // an upper bound of the row tiles: whole ones, and a partial one per request
+    const int64_t ctas = ((int64_t)a.T * group / per + min(a.R, a.T)) * kv.heads;
+    if (ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    k<<<(unsigned)ctas, PT, S::SMEM, s>>>(maps.k, maps.v, kv, a);
+    return cudaGetLastError();
+}
+
+template <typename T, int CODE>
+static cudaError_t prompt_dims(const KvMaps& maps, const KvArg& kv, const AttendArg& a, cudaStream_t s) {
+    return kv.dim == 64 ? prompt_launch<T, CODE, 64>(maps, kv, a, s) : prompt_launch<T, CODE, 128>(maps, kv, a, s);
+}
+
+cudaError_t launch_prompt(const KvMaps& maps, const KvArg& kv, const AttendArg& a, uint32_t type, int code, cudaStream_t s) {
+    const bool i8 = code == RMOE_KV_INT8;
+    if (type == T_F32) return i8 ? prompt_dims<float, RMOE_KV_INT8>(maps, kv, a, s) : prompt_dims<float, RMOE_KV_E4M3>(maps, kv, a, s);
+    if (type == T_F16) return i8 ? prompt_dims<__half, RMOE_KV_INT8>(maps, kv, a, s) : prompt_dims<__half, RMOE_KV_E4M3>(maps, kv, a, s);
+    return i8 ? prompt_dims<__nv_bfloat16, RMOE_KV_INT8>(maps, kv, a, s) : prompt_dims<__nv_bfloat16, RMOE_KV_E4M3>(maps, kv, a, s);
+}
+
+}  // namespace rmoe

@@ -22,9 +22,9 @@
 // warps' pieces, and items that span CTAs go through a workspace slot per CTA, where the last
 // arriving CTA (an atomic count, nobody waits) joins them in CTA order: the result does not depend
 // on timing.
-#include "kv_code.cuh"
-#include "rope.cuh"
 #include "kv_attend.h"
+#include "kv_widen.cuh"
+#include "rope.cuh"
 #include "tc_ptx.cuh"
 
 namespace rmoe {
@@ -56,7 +56,8 @@ struct SplitReq {
     int items;       // row tiles x kv heads
 };
 
-__device__ __forceinline__ SplitReq split_req(const AttendArg& a, int r, int heads, int group, int bs, int nr, int tw) {
+__device__ __forceinline__ SplitReq split_req(const AttendArg& a, int r, int heads, int group, int bs, int nr, int tw,
+                                              int64_t max_rows) {
     SplitReq q;
     const int c0 = __ldg(a.cu + r), c1 = __ldg(a.cu + r + 1), len = __ldg(a.lens + r);
     q.q0 = min(max(c0, 0), a.T);
@@ -67,25 +68,8 @@ __device__ __forceinline__ SplitReq split_req(const AttendArg& a, int r, int hea
     const int lo = a.window ? max(0, q.pos0 - a.window + 1) : 0;
     q.t0 = min(lo, q.hi) / tw;
     q.tiles = max(1, (q.hi + tw - 1) / tw - q.t0);
-    q.items = rows > a.split_rows ? 0 : (int)((rows + nr - 1) / nr) * heads;
+    q.items = rows > max_rows ? 0 : (int)((rows + nr - 1) / nr) * heads;
     return q;
-}
-
-// 4 codes -> two registers of two fp16 each (elements 0, 1 and 2, 3 of the word), exactly.
-template <int CODE>
-__device__ __forceinline__ void widen4(uint32_t w, uint32_t& a, uint32_t& b) {
-    if (CODE == RMOE_KV_INT8) {
-        // 0x6400 | u is 1024 + u for a byte u; u = code + 128
-        const uint32_t u = w ^ 0x80808080u;
-        const uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
-        const __half2 c = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
-        const __half2 p = __hsub2(*reinterpret_cast<const __half2*>(&x), c), q = __hsub2(*reinterpret_cast<const __half2*>(&y), c);
-        a = *reinterpret_cast<const uint32_t*>(&p);
-        b = *reinterpret_cast<const uint32_t*>(&q);
-    } else {
-        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}\n"
-            : "=r"(a), "=r"(b) : "r"(w));
-    }
 }
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
@@ -94,17 +78,6 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     return y;
 }
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-    return y;
-}
-
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-    return v;
-}
 __device__ __forceinline__ uint2 lds64(uint32_t a) {
     uint2 v;
     asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(a));
@@ -156,9 +129,10 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
 
     // ---- this CTA's share of the units ----
     const int per = (a.R + NT - 1) / NT;
+    const int64_t max_rows = a.prompts ? split_max_rows(a, heads, group, s_tot) : INT64_MAX;
     int64_t mine = 0;
     for (int r = tid * per; r < min(a.R, (tid + 1) * per); r++) {
-        const SplitReq q = split_req(a, r, heads, group, bs, NR, TW);
+        const SplitReq q = split_req(a, r, heads, group, bs, NR, TW, max_rows);
         mine += (int64_t)q.items * q.tiles;
     }
     int64_t incl = mine;
@@ -198,10 +172,10 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         }
         int r = lo * per;
         int64_t rem = wu0 - s_pre[lo];
-        SplitReq rq = split_req(a, r, heads, group, bs, NR, TW);
+        SplitReq rq = split_req(a, r, heads, group, bs, NR, TW, max_rows);
         while (rem >= (int64_t)rq.items * rq.tiles) {
             rem -= (int64_t)rq.items * rq.tiles;
-            rq = split_req(a, ++r, heads, group, bs, NR, TW);
+            rq = split_req(a, ++r, heads, group, bs, NR, TW, max_rows);
         }
         int item = (int)(rem / rq.tiles), tile = (int)(rem % rq.tiles);
 
@@ -247,7 +221,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 ptile = 0;
                 if (++pitem == pq.items) {
                     pitem = 0;
-                    do pq = split_req(a, ++pr, heads, group, bs, NR, TW);
+                    do pq = split_req(a, ++pr, heads, group, bs, NR, TW, max_rows);
                     while (pq.items == 0);
                 }
             }
@@ -291,9 +265,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 }
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                // 2^e with mx 2^-e in [2^13, 2^14); nothing to scale at 0 and at infinities
-                const int ex = (int)((__float_as_uint(mx) >> 23) & 0xffu) - 127 - 13;
-                const int e = mx > 0.0f && mx <= 3.4e38f ? max(-126, min(113, ex)) : 0;
+                const int e = q_exponent(mx);
                 const float dn = exp2i(-e);
 #pragma unroll
                 for (int hf = 0; hf < HF; hf++)
@@ -309,7 +281,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                                 ql[nt][hf * 4 + i][p] = pack_f16x2(x - f.x, y - f.y);
                             }
                         }
-                const float up = exp2i(e) * a.scale * 1.4426950408889634f;
+                const float up = exp2i(e) * a.scale * LOG2E;
 #pragma unroll
                 for (int i = 0; i < 2; i++) {  // of the rows 2c, 2c + 1 whose sums this lane holds
                     qs[nt][i] = __shfl_sync(0xffffffffu, up, (2 * c + i) * 4);
@@ -334,7 +306,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             }
             for (int s = 0; s < seg; s++, cnt++) {
                 const int stage = cnt % DEPTH;
-                if (!tc::mbar_wait(smem_u32(&s_full[w][stage]), (cnt / DEPTH) & 1)) {
+                if (!__all_sync(0xffffffffu, tc::mbar_wait(smem_u32(&s_full[w][stage]), (cnt / DEPTH) & 1))) {
                     dead = true;
                     break;
                 }
@@ -346,7 +318,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 for (int i = 0; i < MT; i++) {
                     const int b = MT == 2 && br == 16 ? i : 0;
                     kscale[i] = s_scale[w][stage][b][0];
-                    const float vs = fmaxf(s_scale[w][stage][b][1], 7.8886090522101181e-31f);  // 2^-100
+                    const float vs = v_scale_floor(s_scale[w][stage][b][1]);
                     lv[i] = log2f(vs);
                     iv[i] = 1.0f / vs;
                     gone |= kscale[i] < 0.0f;
@@ -497,8 +469,15 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
 #pragma unroll
                                 for (int y = 0; y < 2; y++) {
                                     float* acc = o[nt][x * 8 + 2 * k + y];
-                                    mma_f16_16816(acc, f[y], ph[nt][i][0], ph[nt][i][1]);
-                                    if (PAIR) mma_f16_16816(acc, f[y], pl[nt][i][0], pl[nt][i][1]);
+                                    if (PAIR) {  // a chain of two, as above
+                                        float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                        mma_f16_16816(t, f[y], pl[nt][i][0], pl[nt][i][1]);
+                                        mma_f16_16816(t, f[y], ph[nt][i][0], ph[nt][i][1]);
+#pragma unroll
+                                        for (int e = 0; e < 4; e++) acc[e] += t[e];
+                                    } else {
+                                        mma_f16_16816(acc, f[y], ph[nt][i][0], ph[nt][i][1]);
+                                    }
                                 }
                         }
                     }
@@ -537,7 +516,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                             }
                         if (g == 0 && a.lse)
                             a.lse[(int64_t)(rq.q0 + tok) * a.q.heads + h] =
-                                l[nt][q] == 0.0f ? -INFINITY : (m[nt][q] + log2f(l[nt][q])) * 0.69314718055994531f;
+                                l[nt][q] == 0.0f ? -INFINITY : (m[nt][q] + log2f(l[nt][q])) * LN2;
                     }
             } else {
                 const bool into_first = firstseg && left > seg;  // the ring is still in use then
@@ -566,7 +545,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 tile = 0;
                 if (++item == rq.items) {
                     item = 0;
-                    do rq = split_req(a, ++r, heads, group, bs, NR, TW);
+                    do rq = split_req(a, ++r, heads, group, bs, NR, TW, max_rows);
                     while (rq.items == 0);
                 }
             }
@@ -604,7 +583,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         reinterpret_cast<T*>(a.out.p)[(int64_t)(pc.q0 + tok) * a.out.st + (int64_t)h * a.out.sh + d] =
             Elt<T>::put(ll > 0.0f ? oo / ll : (ll == 0.0f ? 0.0f : ll));
         if (d == 0 && a.lse)
-            a.lse[(int64_t)(pc.q0 + tok) * a.q.heads + h] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.69314718055994531f;
+            a.lse[(int64_t)(pc.q0 + tok) * a.q.heads + h] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * LN2;
     };
     for (int i = 0; i < 2 * NW;) {
         if (!(s_piece[i].flags & 1)) { i++; continue; }

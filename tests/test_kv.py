@@ -269,7 +269,8 @@ def test_append_edges(kv):
 
 
 # ---- attend --------------------------------------------------------------------------------------
-def run_attend(kv, code, dtype, lens, new, bs, nq, nkv, d, window=0, scale=None, pad=0, max_new=True, poison=False, seed=0):
+def run_attend(kv, code, dtype, lens, new, bs, nq, nkv, d, window=0, scale=None, pad=0, max_new=True, poison=False, seed=0,
+               far=0.0):
     blocks = sum(-(-max(n, 0) // bs) for n in lens) + 3
     c, k, v, ks, vs = cache_of(kv, code, blocks, nkv, bs, d, seed=seed)
     _, _, table = slots_of([max(n, 0) for n in lens], [0] * len(lens), bs, blocks)
@@ -293,10 +294,12 @@ def run_attend(kv, code, dtype, lens, new, bs, nq, nkv, d, window=0, scale=None,
     assert out.dtype == q.dtype and torch.isfinite(out.float()).all()
     e = rel(out, want)
     print(f"attend {code} {dtype} lens {lens[:4]} new {new[:4]}: rel-L2 {e:.2e}")
-    assert e <= REL[dtype], e
+    hidden = torch.isinf(wl)
+    loose = far * float(wl[~hidden].abs().max()) if far else 0.0
+    assert e <= REL[dtype] + loose, e
     hidden = torch.isinf(wl)
     assert torch.equal(torch.isinf(lse.cpu()), hidden) and not out.cpu()[hidden].any()
-    assert (lse.cpu().double() - wl)[~hidden].abs().max().item() <= 2e-5 if (~hidden).any() else True
+    assert (lse.cpu().double() - wl)[~hidden].abs().max().item() <= 2e-5 + loose if (~hidden).any() else True
 
 
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
@@ -316,6 +319,43 @@ def test_attend_decode(kv, code, dtype, lens, new, bs, nq, nkv, d):
     ([129, 90, 260], [129, 1, 130], 32, 16, 2, 128), ([1000], [333], 64, 5, 1, 128)])
 def test_attend_prompts(kv, code, dtype, lens, new, bs, nq, nkv, d):
     run_attend(kv, code, dtype, lens, new, bs, nq, nkv, d, seed=len(lens))
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("lens,new,bs,nq,nkv,d,window", [
+    ([300], [300], 16, 32, 8, 128, 0), ([520, 7, 140, 0], [300, 1, 140, 0], 64, 16, 8, 64, 0),
+    ([129, 700], [128, 129], 128, 40, 8, 128, 0), ([70, 90, 64, 33], [64, 64, 64, 33], 32, 8, 8, 64, 0),
+    ([600, 40], [257, 40], 64, 24, 8, 128, 100), ([400, 300], [140, 1], 16, 48, 12, 128, 33)])
+def test_attend_prompts_of_many_rows(kv, code, dtype, lens, new, bs, nq, nkv, d, window):
+    """Enough rows for the tensor-core prompt kernel (24 CTAs of 256 rows), beside short requests."""
+    run_attend(kv, code, dtype, lens, new, bs, nq, nkv, d, window=window, seed=len(lens))
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attend_many_rows_edges(kv, code, dtype):
+    """The prompt kernel's rows that see nothing, garbage past the ends, scores near to each other,
+    and repeats bit for bit."""
+    run_attend(kv, code, dtype, [3, 200, 0], [300, 280, 90], 16, 16, 8, 64, pad=50, poison=True, max_new=False)
+    run_attend(kv, code, dtype, [190, 333], [190, 150], 64, 16, 8, 128, pad=3, poison=True)
+    run_attend(kv, code, dtype, [700], [200], 64, 32, 8, 64, scale=0.001)
+    c, *_ = cache_of(kv, code, 40, 8, 64, 128)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    q = torch.randn((500, 32, 128), generator=g, device="cuda").to(R.DT[dtype])
+    args = (ints([list(range(0, 20)), list(range(20, 40))]), ints([1200, 900]), ints([0, 300, 500]))
+    a, b = c.attend(q, *args), c.attend(q, *args)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attend_scores_in_the_hundreds(kv, code, dtype):
+    """Scores so far apart that the maximum grows from tile to tile.  A score of size s is a sum of
+    128 products whose running sums the tensor cores cut to 24 bits at most 16 times, and is rounded
+    three more times at 1.44 s: off by at most 2^-19 s, and so are lse and, relatively, the weights."""
+    run_attend(kv, code, dtype, [700], [200], 64, 32, 8, 128, scale=1.0, far=2.0 ** -19)
+    run_attend(kv, code, dtype, [700, 90], [1, 2], 64, 32, 8, 128, scale=1.0, far=2.0 ** -19)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
