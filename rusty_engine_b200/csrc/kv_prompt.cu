@@ -43,6 +43,28 @@ struct PromptBars {
         o_empty[2], meta_full[4], drain;
 };
 
+// Registers a thread of this warpgroup (all four warps execute it).
+template <int N> __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
+
+// Two f32 in one register pair.
+__device__ __forceinline__ uint64_t f2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void un2(uint64_t r, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(x), "=f"(y) : "l"(r)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 template <typename T, int CODE, int D>
 __global__ void __launch_bounds__(PT, 1)
 kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, KvArg kv, AttendArg a) {
@@ -141,6 +163,10 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
         return !dead;
     };
 
+    // Registers go to the roles that hold rows: 192 + 192 + 72 + 56 a thread (f32: 184 + 184 + 80 +
+    // 64), of 128 x 4 at launch.  Each role's branch begins with its warpgroup's share.
+    if (wg == 3) {
+    reg_dec<PAIR ? 64 : 56>();
     if (w == 12) {
         // ---- producer: raw tiles and the scales of their blocks ----
         const int br = min(bs, PKV), nb = PKV / br;
@@ -253,8 +279,10 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
             tc::mma_commit(smem_u32(&bars.drain));  // nothing may run into freed tensor memory
             if (!tc::mbar_wait(smem_u32(&bars.drain), 0)) dead = true;
         }
+    }
     } else if (wg == 2) {
         // ---- widening: one key per thread ----
+        reg_dec<PAIR ? 80 : 72>();
         const int row = tid - 256;
         for (int j = 0; j < nt; j++) {
             if (!wait(bars.meta_full[j & 3], j >> 2)) break;
@@ -292,7 +320,8 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
             }
             if (dead) break;
         }
-    } else if (wg < NRT || (PAIR && wg == 1)) {
+    } else {
+        reg_inc<PAIR ? 184 : 192>();
         const int rt = PAIR ? 0 : wg, lrow = tid & 127;
         const uint32_t tl = tm + ((uint32_t)((w & 3) * 32) << 16);
         const int row = row0 + rt * 128 + lrow, tok = row / group, h = kh * group + row % group;
@@ -383,24 +412,30 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
                 for (int i = 0; i < 8; i++) masked |= meta[i].w != 0.0f;
                 if (!wait(bars.s_full[sb], PAIR ? j / 2 : j)) break;
                 tc::fence_after_sync();
+                // the row of S, masked where a key is not this row's
+                uint32_t v[PKV];
+#pragma unroll
+                for (int c = 0; c < 4; c++) tc::tmem_ld32(sp + c * 32, v + c * 32);
+                tc::tmem_ld_wait();
+                if (masked) {
+#pragma unroll
+                    for (int g = 0; g < 8; g++) {
+                        const bool gone = meta[g].w != 0.0f;
+                        const int b = gone ? 0 : vhi - (key0 + 16 * g), t = vlo - (key0 + 16 * g);  // keys t .. b - 1 of the 16
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            if (i >= b || i < t) v[g * 16 + i] = 0xff800000u;  // -infinity
+                    }
+                }
                 float mx = -INFINITY;
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    uint32_t v[32];
-                    tc::tmem_ld32(sp + c * 32, v);
-                    tc::tmem_ld_wait();
+                for (int g = 0; g < 8; g++) {
+                    const float4 mt = meta[g];
+                    float x[2] = {__uint_as_float(v[g * 16]), __uint_as_float(v[g * 16 + 1])};
 #pragma unroll
-                    for (int g = 0; g < 2; g++) {
-                        const float4 mt = meta[2 * c + g];
-                        float x = -INFINITY;
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const int key = key0 + c * 32 + g * 16 + i;
-                            const float y = __uint_as_float(v[g * 16 + i]);
-                            if (!masked || (key < vhi && key >= vlo && mt.w == 0.0f)) x = fmaxf(x, y);
-                        }
-                        if (x != -INFINITY) mx = fmaxf(mx, fmaf(x, qs * mt.x, mt.y));
-                    }
+                    for (int i = 2; i < 16; i++) x[i & 1] = fmaxf(x[i & 1], __uint_as_float(v[g * 16 + i]));
+                    // a scale of 0 times -infinity is NaN, which fmaxf drops
+                    mx = fmaxf(mx, fmaf(fmaxf(x[0], x[1]), qs * mt.x, mt.y));
                 }
                 // f32: M is the maximum; else it only moves when P could leave 2^8
                 const bool grow = PAIR ? mx > m : mx > m + 8.0f;
@@ -412,45 +447,48 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
                     if (!wait(bars.o_full[rt], j - 1)) break;
                     tc::fence_after_sync();
 #pragma unroll
-                    for (int c = 0; c < CH; c++) {
-                        uint32_t v[32];
-                        tc::tmem_ld32(tl + 256 + rt * 128 + c * 32, v);
+                    for (int c = 0; c < CH * 2; c++) {
+                        uint32_t o[16];
+                        tc::tmem_ld16(tl + 256 + rt * 128 + c * 16, o);
                         tc::tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * al);
-                        tc::tmem_st32(tl + 256 + rt * 128 + c * 32, v);
+                        for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
+                        tc::tmem_st16(tl + 256 + rt * 128 + c * 16, o);
                     }
                 }
                 m = mn;
                 l *= al;
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    uint32_t v[32], ph[16], pl[16];
-                    tc::tmem_ld32(sp + c * 32, v);
-                    tc::tmem_ld_wait();
+                    uint32_t ph[16], pl[16];
 #pragma unroll
                     for (int g = 0; g < 2; g++) {
                         const float4 mt = meta[2 * c + g];
                         const float sc = qs * mt.x, off = mt.y - mu;
-                        float sum[2] = {0.0f, 0.0f};
+                        const uint64_t sc2 = f2(sc, sc), off2 = f2(off, off);
+                        uint64_t sum = 0;
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
-                            float p[2];
-#pragma unroll
-                            for (int z = 0; z < 2; z++) {
-                                const int key = key0 + c * 32 + g * 16 + 2 * i + z;
-                                p[z] = ex2(fmaf(__uint_as_float(v[g * 16 + 2 * i + z]), sc, off));
-                                if (masked && !(key < vhi && key >= vlo && mt.w == 0.0f)) p[z] = 0.0f;
-                                sum[z] += p[z];
+                            const int e = c * 32 + g * 16 + 2 * i;
+                            float x, y;
+                            un2(fma2(f2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sc2, off2), x, y);
+                            x = ex2(x);
+                            y = ex2(y);
+                            if (masked) {  // 0 * -infinity above
+                                if (v[e] == 0xff800000u) x = 0.0f;
+                                if (v[e + 1] == 0xff800000u) y = 0.0f;
                             }
-                            const uint32_t hh = pack_f16x2(p[0], p[1]);
+                            sum = add2(sum, f2(x, y));
+                            const uint32_t hh = pack_f16x2(x, y);
                             ph[g * 8 + i] = hh;
                             if (PAIR) {
                                 const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hh));
-                                pl[g * 8 + i] = pack_f16x2(p[0] - f.x, p[1] - f.y);
+                                pl[g * 8 + i] = pack_f16x2(x - f.x, y - f.y);
                             }
                         }
-                        l = fmaf(sum[0] + sum[1], mt.z, l);
+                        float x, y;
+                        un2(sum, x, y);
+                        l = fmaf(x + y, mt.z, l);
                     }
                     tc::tmem_st16(sp + c * 32, ph);
                     if (PAIR) tc::tmem_st16(sp + c * 32 + 16, pl);
