@@ -39,7 +39,7 @@ struct PromptShape {
 };
 
 struct PromptBars {
-    uint64_t q_full, raw_full[2], raw_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2],
+    uint64_t q_full, raw_full[2], raw_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_half[2], p_full[2], o_full[2],
         o_empty[2], meta_full[4], drain;
 };
 
@@ -64,6 +64,9 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+
+// The factor from a product of codes to the exponent: positive, so that -infinity stays it.
+__device__ __forceinline__ float score_scale(float qs, float ks) { return fmaxf(qs * ks, 1.17549435e-38f); }
 
 template <typename T, int CODE, int D>
 __global__ void __launch_bounds__(PT, 1)
@@ -139,6 +142,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
             tc::mbar_init(smem_u32(&bars.v_full[i]), 4);
             tc::mbar_init(smem_u32(&bars.v_empty[i]), 1);
             tc::mbar_init(smem_u32(&bars.s_full[i]), 1);
+            tc::mbar_init(smem_u32(&bars.p_half[i]), 4);
             tc::mbar_init(smem_u32(&bars.p_full[i]), 4);
             tc::mbar_init(smem_u32(&bars.o_full[i]), 1);
             tc::mbar_init(smem_u32(&bars.o_empty[i]), 4);
@@ -155,11 +159,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     // tensor memory columns: S (and P) of tile / buffer i at 128 i, O at 256 + 128 i
     bool dead = false;
     auto wait = [&](uint64_t& b, uint32_t parity) {  // by whole warps: all lanes go on, or none
-        if (!dead) dead = !__all_sync(0xffffffffu, tc::mbar_wait(smem_u32(&b), parity & 1));
-        return !dead;
-    };
-    auto wait1 = [&](uint64_t& b, uint32_t parity) {  // by one thread
-        if (!dead) dead = !tc::mbar_wait(smem_u32(&b), parity & 1);
+        if (!dead) dead = !__all_sync(0xffffffffu, tc::mbar_wait_tries(smem_u32(&b), parity & 1));
         return !dead;
     };
 
@@ -213,71 +213,81 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
             }
     } else if (w == 13) {
         // ---- products ----
-        if (lane == 0 && nt > 0) {
+        if (nt > 0) {
+            const uint32_t lead = lane == 0;
             constexpr uint32_t idS = tc::idesc_f16(128, PKV), idO = tc::idesc_f16(128, D) | tc::IDESC_B_MN;
-            auto mma_s = [&](int q, uint32_t d, int j) {  // S = Q K^T of key tile j; q: the Q tile (lo half next to it)
-                const uint32_t kb = base + S::K0 + (j % KN) * S::QB;
+            const uint64_t qd = tc::smem_desc_sw128(base + S::Q0), kd = tc::smem_desc_sw128(base + S::K0),
+                           vd = tc::smem_desc_mn_sw128(base + S::V0, PKV * 128);
+            const uint32_t dh = (uint32_t)(kd >> 32), vh = (uint32_t)(vd >> 32);
+            auto mma_s = [&](int q, uint32_t d, int buf) {  // S = Q K^T; q: the Q tile (lo half next to it)
+                const uint32_t qa = (uint32_t)qd + q * (S::QB >> 4), kb = (uint32_t)kd + buf * (S::QB >> 4);
 #pragma unroll
                 for (int half = PAIR ? 1 : 0; half >= 0; half--)
 #pragma unroll
                     for (int k = 0; k < D / 16; k++) {
-                        const uint32_t off = (k / 4) * 16384 + (k % 4) * 32;
-                        tc::mma_ss(d, tc::smem_desc_sw128(base + S::Q0 + (q + half) * S::QB + off), tc::smem_desc_sw128(kb + off), idS,
-                                   k > 0 || (PAIR && half == 0));
+                        const uint32_t off = ((k / 4) * 16384 + (k % 4) * 32) >> 4;
+                        tc::mma_ss_lead(lead, d, qa + (half * (S::QB >> 4) + off), dh, kb + off, dh, idS, k > 0 || (PAIR && half == 0));
                     }
             };
-            auto mma_o = [&](uint32_t d, uint32_t p, int j, bool add) {  // O (+)= P V
-                const uint32_t vb = base + S::V0 + (j % VN) * S::QB;
+            auto mma_o = [&](uint32_t d, uint32_t p, int buf, uint32_t add, int part) {  // O (+)= P V of half the keys
+                const uint32_t vb = (uint32_t)vd + buf * (S::QB >> 4) + part * (4 * 2048 >> 4);
+                p += part * 64;
 #pragma unroll
                 for (int half = PAIR ? 1 : 0; half >= 0; half--)
 #pragma unroll
-                    for (int k = 0; k < PKV / 16; k++)
-                        tc::mma_ts(d, p + (k / 2) * 32 + (k % 2) * 8 + half * 16, tc::smem_desc_mn_sw128(vb + k * 2048, PKV * 128), idO,
-                                   add || k > 0 || (PAIR && half == 0));
+                    for (int k = 0; k < PKV / 32; k++)
+                        tc::mma_ts_lead(lead, d, p + (k / 2) * 32 + (k % 2) * 8 + half * 16, vb + (k * 2048 >> 4), vh, idO,
+                                        k > 0 || (PAIR && half == 0) ? 1u : add);
             };
-            if (wait1(bars.q_full, 0) && wait1(bars.k_full[0], 0)) {
+            if (wait(bars.q_full, 0) && wait(bars.k_full[0], 0)) {
                 tc::fence_after_sync();
                 for (int t = 0; t < NRT; t++) {
                     mma_s(t, tm + t * 128, 0);
-                    tc::mma_commit(smem_u32(&bars.s_full[t]));
+                    tc::mma_commit_lead(lead, smem_u32(&bars.s_full[t]));
                 }
-                tc::mma_commit(smem_u32(&bars.k_empty[0]));
+                tc::mma_commit_lead(lead, smem_u32(&bars.k_empty[0]));
             }
             for (int j = 0; j < nt && !dead; j++) {
                 if (PAIR) {
                     if (j + 1 < nt) {
-                        if (!wait1(bars.k_full[(j + 1) % KN], (j + 1) / KN)) break;
+                        if (!wait(bars.k_full[(j + 1) % KN], (j + 1) / KN)) break;
                         tc::fence_after_sync();
-                        mma_s(0, tm + ((j + 1) & 1) * 128, j + 1);
-                        tc::mma_commit(smem_u32(&bars.s_full[(j + 1) & 1]));
-                        tc::mma_commit(smem_u32(&bars.k_empty[(j + 1) % KN]));
+                        mma_s(0, tm + ((j + 1) & 1) * 128, (j + 1) % KN);
+                        tc::mma_commit_lead(lead, smem_u32(&bars.s_full[(j + 1) & 1]));
+                        tc::mma_commit_lead(lead, smem_u32(&bars.k_empty[(j + 1) % KN]));
                     }
-                    if (!wait1(bars.v_full[j % VN], j / VN) || !wait1(bars.p_full[j & 1], j / 2)) break;
-                    if (j >= 2 && !wait1(bars.o_empty[j & 1], j / 2 - 1)) break;
+                    if (!wait(bars.v_full[j % VN], j / VN) || !wait(bars.p_half[j & 1], j / 2)) break;
+                    if (j >= 2 && !wait(bars.o_empty[j & 1], j / 2 - 1)) break;
                     tc::fence_after_sync();
-                    mma_o(tm + 256 + (j & 1) * 128, tm + (j & 1) * 128, j, false);
-                    tc::mma_commit(smem_u32(&bars.o_full[j & 1]));
-                    tc::mma_commit(smem_u32(&bars.v_empty[j % VN]));
+                    mma_o(tm + 256 + (j & 1) * 128, tm + (j & 1) * 128, j % VN, 0, 0);
+                    if (!wait(bars.p_full[j & 1], j / 2)) break;
+                    tc::fence_after_sync();
+                    mma_o(tm + 256 + (j & 1) * 128, tm + (j & 1) * 128, j % VN, 1, 1);
+                    tc::mma_commit_lead(lead, smem_u32(&bars.o_full[j & 1]));
+                    tc::mma_commit_lead(lead, smem_u32(&bars.v_empty[j % VN]));
                 } else {
                     for (int t = 0; t < NRT; t++) {
-                        if (t == 0 && !wait1(bars.v_full[j % VN], j / VN)) break;
-                        if (!wait1(bars.p_full[t], j)) break;
+                        if (t == 0 && !wait(bars.v_full[j % VN], j / VN)) break;
+                        if (!wait(bars.p_half[t], j)) break;
                         tc::fence_after_sync();
-                        mma_o(tm + 256 + t * 128, tm + t * 128, j, j > 0);
-                        tc::mma_commit(smem_u32(&bars.o_full[t]));
-                        if (t == NRT - 1) tc::mma_commit(smem_u32(&bars.v_empty[j % VN]));
+                        mma_o(tm + 256 + t * 128, tm + t * 128, j % VN, j > 0, 0);
+                        if (!wait(bars.p_full[t], j)) break;
+                        tc::fence_after_sync();
+                        mma_o(tm + 256 + t * 128, tm + t * 128, j % VN, 1, 1);
+                        tc::mma_commit_lead(lead, smem_u32(&bars.o_full[t]));
+                        if (t == NRT - 1) tc::mma_commit_lead(lead, smem_u32(&bars.v_empty[j % VN]));
                         if (j + 1 < nt) {
-                            if (t == 0 && !wait1(bars.k_full[(j + 1) % KN], (j + 1) / KN)) break;
+                            if (t == 0 && !wait(bars.k_full[(j + 1) % KN], (j + 1) / KN)) break;
                             tc::fence_after_sync();
-                            mma_s(t, tm + t * 128, j + 1);
-                            tc::mma_commit(smem_u32(&bars.s_full[t]));
-                            if (t == NRT - 1) tc::mma_commit(smem_u32(&bars.k_empty[(j + 1) % KN]));
+                            mma_s(t, tm + t * 128, (j + 1) % KN);
+                            tc::mma_commit_lead(lead, smem_u32(&bars.s_full[t]));
+                            if (t == NRT - 1) tc::mma_commit_lead(lead, smem_u32(&bars.k_empty[(j + 1) % KN]));
                         }
                     }
                 }
             }
-            tc::mma_commit(smem_u32(&bars.drain));  // nothing may run into freed tensor memory
-            if (!tc::mbar_wait(smem_u32(&bars.drain), 0)) dead = true;
+            tc::mma_commit_lead(lead, smem_u32(&bars.drain));  // nothing may run into freed tensor memory
+            if (!__all_sync(0xffffffffu, tc::mbar_wait(smem_u32(&bars.drain), 0))) dead = true;
         }
     }
     } else if (wg == 2) {
@@ -289,24 +299,26 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
             const int key = (jt0 + j) * PKV + row;
             // keys that no row sees may hold anything, NaN codes too, and 0 * NaN is NaN
             const bool live = key < kmax && key >= kmin && s_meta[j & 3][row >> 4].w == 0.0f;
-#pragma unroll
+#pragma unroll 1
             for (int v = 0; v < 2; v++) {
                 const int nbuf = v ? VN : KN, b = j % nbuf;
                 if (!wait(bars.raw_full[v], j)) break;
                 if (j >= nbuf && !wait(v ? bars.v_empty[b] : bars.k_empty[b], j / nbuf - 1)) break;
                 const uint32_t src = base + S::R0 + v * S::RAW, dst = base + (v ? S::V0 : S::K0) + b * S::QB + row * 128;
+uint4 x[D / 16];
+#pragma unroll
+                for (int c = 0; c < D / 16; c++)
+                    x[c] = D == 64 ? lds128(src + row * 64 + ((c ^ ((row >> 1) & 3)) << 4)) : lds128(src + row * 128 + ((c ^ (row & 7)) << 4));
+                if (!__all_sync(0xffffffffu, live) && !live)
+#pragma unroll
+                    for (int c = 0; c < D / 16; c++) x[c] = make_uint4(0, 0, 0, 0);
 #pragma unroll
                 for (int c = 0; c < D / 16; c++) {
-                    const uint4 x = D == 64 ? lds128(src + row * 64 + ((c ^ ((row >> 1) & 3)) << 4))
-                                            : lds128(src + row * 128 + ((c ^ (row & 7)) << 4));
                     uint32_t y[8];
-                    widen4<CODE>(x.x, y[0], y[1]);
-                    widen4<CODE>(x.y, y[2], y[3]);
-                    widen4<CODE>(x.z, y[4], y[5]);
-                    widen4<CODE>(x.w, y[6], y[7]);
-                    if (!live)
-#pragma unroll
-                        for (int i = 0; i < 8; i++) y[i] = 0;
+                    widen4<CODE>(x[c].x, y[0], y[1]);
+                    widen4<CODE>(x[c].y, y[2], y[3]);
+                    widen4<CODE>(x[c].z, y[4], y[5]);
+                    widen4<CODE>(x[c].w, y[6], y[7]);
                     const uint32_t d = dst + (c / 4) * 16384;
                     sts128(d + (((2 * c & 7) ^ (row & 7)) << 4), make_uint4(y[0], y[1], y[2], y[3]));
                     sts128(d + (((2 * c + 1 & 7) ^ (row & 7)) << 4), make_uint4(y[4], y[5], y[6], y[7]));
@@ -377,7 +389,9 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
                 for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(v[i]));
             }
             const int e = q_exponent(mx);
-            const float dn = exp2i(-e), qs = exp2i(e) * a.scale * LOG2E;
+            // the sign of the scale goes to q, and a scale of 0 makes q 0: qs is positive
+            const float dn = exp2i(-e) * (a.scale < 0.0f ? -1.0f : a.scale == 0.0f ? 0.0f : 1.0f);
+            const float qs = exp2i(e) * (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * LOG2E;
             for (int c = 0; c < D / 8; c++) {
                 float v[8];
                 load8(qp + c * 8, a.q.vec, v);
@@ -425,6 +439,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
 #pragma unroll
                         for (int i = 0; i < 16; i++)
                             if (i >= b || i < t) v[g * 16 + i] = 0xff800000u;  // -infinity
+                        asm volatile("" ::: "memory");  // a branch: few tiles are masked
                     }
                 }
                 float mx = -INFINITY;
@@ -434,8 +449,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
                     float x[2] = {__uint_as_float(v[g * 16]), __uint_as_float(v[g * 16 + 1])};
 #pragma unroll
                     for (int i = 2; i < 16; i++) x[i & 1] = fmaxf(x[i & 1], __uint_as_float(v[g * 16 + i]));
-                    // a scale of 0 times -infinity is NaN, which fmaxf drops
-                    mx = fmaxf(mx, fmaf(fmaxf(x[0], x[1]), qs * mt.x, mt.y));
+                    mx = fmaxf(mx, fmaf(fmaxf(x[0], x[1]), score_scale(qs, mt.x), mt.y));
                 }
                 // f32: M is the maximum; else it only moves when P could leave 2^8
                 const bool grow = PAIR ? mx > m : mx > m + 8.0f;
@@ -464,7 +478,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
 #pragma unroll
                     for (int g = 0; g < 2; g++) {
                         const float4 mt = meta[2 * c + g];
-                        const float sc = qs * mt.x, off = mt.y - mu;
+                        const float sc = score_scale(qs, mt.x), off = mt.y - mu;
                         const uint64_t sc2 = f2(sc, sc), off2 = f2(off, off);
                         uint64_t sum = 0;
 #pragma unroll
@@ -474,10 +488,6 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
                             un2(fma2(f2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sc2, off2), x, y);
                             x = ex2(x);
                             y = ex2(y);
-                            if (masked) {  // 0 * -infinity above
-                                if (v[e] == 0xff800000u) x = 0.0f;
-                                if (v[e + 1] == 0xff800000u) y = 0.0f;
-                            }
                             sum = add2(sum, f2(x, y));
                             const uint32_t hh = pack_f16x2(x, y);
                             ph[g * 8 + i] = hh;
@@ -492,6 +502,12 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
                     }
                     tc::tmem_st16(sp + c * 32, ph);
                     if (PAIR) tc::tmem_st16(sp + c * 32 + 16, pl);
+                    if (c == 1) {  // the products of the first half of the keys can begin
+                        tc::tmem_st_wait();
+                        tc::fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(smem_u32(&bars.p_half[sb]));
+                    }
                 }
                 if (PAIR && j == nt - 1) s_fin[0][PAIR ? lrow : 0] = m, s_fin[1][PAIR ? lrow : 0] = l;
                 tc::tmem_st_wait();
