@@ -44,6 +44,33 @@ def _nccl_flags():
     return [], ["-lnccl"]
 
 
+BINDING_SRC = os.path.join(HERE, "binding", "kv_ops.cpp")
+BINDING = os.path.join(HERE, "_kv_ops.so")
+
+
+def build_binding() -> str:
+    """The torch-tensor entry of kv.py (binding/kv_ops.cpp), linked against librmoe.so and torch."""
+    deps = [BINDING_SRC, os.path.join(HERE, "..", "include", "rmoe.h")]
+    if os.path.exists(BINDING) and os.path.getmtime(BINDING) >= max(os.path.getmtime(d) for d in deps):
+        return BINDING
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cuda_inc = os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I" + sysconfig.get_paths()["include"], "-I" + cuda_inc] + ["-I" + p for p in include_paths()] + [
+        BINDING_SRC, "-o", BINDING, "-L" + lib, "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda",
+        OUT, "-Wl,-rpath," + lib, "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {BINDING_SRC}:\n{r.stderr}")
+    return BINDING
+
+
 def build(verbose: bool = False, jobs: int = 8) -> str:
     nvcc = _nvcc()
     os.makedirs(OBJ, exist_ok=True)
@@ -71,10 +98,11 @@ def build(verbose: bool = False, jobs: int = 8) -> str:
                 print(log, file=sys.stderr)
     objs = [o for o, _ in results]
     if not os.path.exists(OUT) or os.path.getmtime(OUT) < max(os.path.getmtime(o) for o in objs):
-        cmd = [nvcc] + ARCH + ["-shared", "-o", OUT] + objs + link_nccl
+        cmd = [nvcc] + ARCH + ["-shared", "-Xlinker", "-soname=librmoe.so", "-o", OUT] + objs + link_nccl
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stderr}")
+    build_binding()
     return OUT
 
 

@@ -3,6 +3,8 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "layer_impl.h"
 
 struct rmoe_rope {
@@ -51,6 +53,19 @@ inline rmoe_status check_device(int32_t device) {
         return fail(RMOE_ERR_CUDA, "no CUDA device");
     }
     return device >= 0 && device < n ? RMOE_OK : fail(RMOE_ERR_INVALID, "device %d out of range", device);
+}
+
+// Raises a kernel's dynamic shared-memory limit on the current device, the first time only (a call
+// of its own took longer than the launch).
+template <typename K>
+inline cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_relaxed) & bit))) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 inline uint32_t elt_size(uint32_t type) { return type == T_F32 ? 4 : 2; }

@@ -546,7 +546,8 @@ template <typename T, int CODE, int D>
 static cudaError_t prompt_launch(const KvMaps& maps, const KvArg& kv, const AttendArg& a, cudaStream_t s) {
     using S = PromptShape<D, sizeof(T) == 4>;
     auto k = kv_prompt_kernel<T, CODE, D>;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_smem(k, S::SMEM, done);
     if (e != cudaSuccess) return e;
     const int64_t group = a.q.heads / kv.heads, per = 128 * S::NRT;
     // an upper bound of the row tiles: whole ones, and a partial one per request

@@ -649,7 +649,8 @@ static cudaError_t split_launch(const KvMaps& maps, const KvArg& kv, const Atten
     constexpr int smem = SplitSmem<D, NR>::TOTAL;
     static_assert(SplitSmem<D, NR>::PIECE * 4 <= SPLIT_DEPTH * SplitShape<D>::STAGE, "a last piece takes the place of the ring");
     auto k = kv_split_kernel<T, CODE, D, NR>;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_smem(k, smem, done);
     if (e != cudaSuccess) return e;
     k<<<sms, SPLIT_NW * 32, smem, s>>>(maps.k, maps.v, kv, a, ws);
     return cudaGetLastError();

@@ -168,7 +168,8 @@ rmoe_status rmoe_kv_extend(const rmoe_kv_extend_args* a, void* stream) {
     if (a->lens_out == a->lens || a->n_free_out == a->n_free)
         return fail(RMOE_ERR_INVALID, "kv extend: lens_out / n_free_out alias their inputs");
     const size_t smem = (2 * (size_t)a->R + 1) * 4;
-    cudaError_t e = cudaFuncSetAttribute(kv_extend_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 132 << 10);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_smem(kv_extend_kernel, 132 << 10, done);
     if (e != cudaSuccess) return cuda_fail(e, "kv extend");
     const unsigned grid = (unsigned)((a->T + EXT_THREADS - 1) / EXT_THREADS);
     kv_extend_kernel<<<grid < 1 ? 1 : grid < 148 ? grid : 148, EXT_THREADS, smem, static_cast<cudaStream_t>(stream)>>>(*a);
@@ -182,7 +183,8 @@ rmoe_status rmoe_kv_release(const rmoe_kv_release_args* a, void* stream) {
     if (!a->n_free || !a->n_free_out || (a->R && (!a->table || !a->lens || !a->done)) || (a->free_cap && !a->free_list))
         return fail(RMOE_ERR_INVALID, "kv release: null pointer");
     if (a->n_free_out == a->n_free) return fail(RMOE_ERR_INVALID, "kv release: n_free_out aliases n_free");
-    cudaError_t e = cudaFuncSetAttribute(kv_release_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 132 << 10);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_smem(kv_release_kernel, 132 << 10, done);
     if (e != cudaSuccess) return cuda_fail(e, "kv release");
     kv_release_kernel<<<1, EXT_THREADS, (size_t)a->R * 4 + 4, static_cast<cudaStream_t>(stream)>>>(*a);
     e = cudaGetLastError();

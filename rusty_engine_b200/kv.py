@@ -19,6 +19,7 @@ float16 or bfloat16 CUDA tensors [tokens, heads, head_dim] whose last dimension 
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import enum
 import math
@@ -28,11 +29,39 @@ from typing import Optional, Sequence
 import numpy as np
 
 from . import _lib
-from .moe import EngineError, _call, _require_cuda, torch
+from .moe import EngineError, _call, _require_cuda, _stream, torch
 
-if torch is not None:
-    _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}  # ggml codes
-    _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+_binding = None
+
+
+def _ops():
+    """The native entry for torch tensors (binding/kv_ops.cpp); raises if it was not built."""
+    global _binding
+    if _binding is None:
+        import importlib.util
+        import os
+
+        _lib.load()
+        path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_kv_ops.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is missing: build it with `python -m rusty_engine_b200.build`")
+        spec = importlib.util.spec_from_file_location("_kv_ops", path)
+        m = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(m)
+        m.setup(EngineError, _call)
+        _binding = m
+    return _binding
+
+
+@contextlib.contextmanager
+def _on(stream, *tensors):
+    """Calls made here run on `stream` and allocate their outputs there; the tensors' memory is kept
+    from being reused before the stream is done with it."""
+    for t in tensors:
+        if t is not None:
+            t.record_stream(stream)
+    with torch.cuda.stream(stream):
+        yield
 
 
 class RopeLayout(enum.IntEnum):
@@ -67,47 +96,10 @@ class RopeConfig:
     freq_factors: Optional[Sequence[float]] = None
 
 
-def _stream_of(x, stream, *others):
-    """The raw stream a call runs on.  With an explicit stream, the tensors' memory is also kept
-    from being reused before that stream is done with it."""
-    if stream is None:
-        return _raw_stream(x.device.index) if _raw_stream else torch.cuda.current_stream(x.device).cuda_stream
-    for t in (x, *others):
-        if t is not None:
-            t.record_stream(stream)
-    return stream.cuda_stream
-
-
-def _rows(x, what):
-    """(data, token stride, head stride, heads, 0) of an rmoe_rows."""
-    if x.dim() != 3 or x.stride(2) != 1 and x.shape[2] != 1:
-        raise EngineError(f"{what}: a [tokens, heads, head_dim] tensor with contiguous heads, got {tuple(x.shape)} "
-                          f"strides {tuple(x.stride())}")
-    st = x.stride()
-    return x.data_ptr(), st[0], st[1], x.shape[1], 0
-
-
-_NO_ROWS = (0, 0, 0, 0, 0)
-
-
-def _type_of(x, what):
-    t = _TYPES.get(x.dtype)
-    if t is None or not x.is_cuda:
-        raise EngineError(f"{what}: a float32, float16 or bfloat16 CUDA tensor, got {x.dtype} on {x.device}")
-    return t
-
-
-def _int32(x, what, like, n=None):
-    if x.dtype != torch.int32 or not x.is_contiguous() or x.device != like.device:
-        raise EngineError(f"{what}: a contiguous int32 tensor on {like.device}, got {x.dtype} on {x.device}")
-    if n is not None and x.numel() != n:
-        raise EngineError(f"{what}: {x.numel()} entries, expected {n}")
+def _int32(x, what, like, n):
+    if x.dtype != torch.int32 or not x.is_contiguous() or x.device != like.device or x.numel() != n:
+        raise EngineError(f"{what}: {n} contiguous int32 on {like.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
     return x.data_ptr()
-
-
-def _same(x, like, what):
-    if x.dtype != like.dtype or x.device != like.device:
-        raise EngineError(f"{what}: {x.dtype} on {x.device}, expected {like.dtype} on {like.device}")
 
 
 class Rope:
@@ -129,37 +121,15 @@ class Rope:
         h = C.c_void_p()
         L = _lib.load()
         _call(L.rmoe_rope_create(C.byref(d), C.byref(h)))
-        self._h, self._apply = h, L.rmoe_rope_apply
+        self._h, self._p, self._apply = h, h.value, _ops().rope_apply
 
     def apply(self, q, positions, k=None, *, out=None, k_out=None, inverse: bool = False, stream=None):
         """q (and k) [tokens, heads, head_dim] turned by positions [tokens] (int32); returns the
         turned q, or (q, k) when k is given.  `out=q` turns in place.  inverse: turns back."""
-        ty = _type_of(q, "q")
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        qr, orow = _rows(q, "q"), _rows(out, "out")
-        _same(out, q, "out")
-        T, _, dim = q.shape
-        if out.shape != q.shape:
-            raise EngineError(f"out: {tuple(out.shape)}, expected {tuple(q.shape)}")
-        if k is not None:
-            _same(k, q, "k")
-            if k_out is None:
-                k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-            _same(k_out, q, "k_out")
-            kr, kor = _rows(k, "k"), _rows(k_out, "k_out")
-            if k.shape[0] != T or k.shape[2] != dim or k_out.shape != k.shape:
-                raise EngineError(f"k: {tuple(k.shape)} / {tuple(k_out.shape)} beside q {tuple(q.shape)}")
-        else:
-            kr = kor = _NO_ROWS
-        if q.device.index != self.device:
-            raise EngineError(f"q is on {q.device}, the rope on device {self.device}")
-        args = _lib.ROPE_ARGS.pack(*qr, *orow, *kr, *kor, _int32(positions, "positions", q, T), T, dim, ty,
-                                   1 if inverse else 0)
-        st = self._apply(self._h, args, _stream_of(q, stream, out, k, k_out, positions))
-        if st:
-            _call(st)
-        return out if k is None else (out, k_out)
+        if stream is not None:
+            with _on(stream, q, positions, k, out, k_out):
+                return self.apply(q, positions, k, out=out, k_out=k_out, inverse=inverse)
+        return self._apply(self._p, self.device, q, positions, k, out, k_out, inverse)
 
     def check(self):
         """Raises if a call so far met a position outside the table (synchronises)."""
@@ -168,7 +138,7 @@ class Rope:
     def close(self):
         if getattr(self, "_h", None) is not None and self._h.value:
             _lib.load().rmoe_rope_destroy(self._h)
-            self._h = C.c_void_p()
+            self._h, self._p = C.c_void_p(), 0
 
     def __del__(self):
         try:
@@ -194,26 +164,10 @@ def extend_tables(table, lens, new_lens, free, n_free, total: int, block_size: i
     token count (slots past the requests' tokens are -1).  New blocks come off the stack
     free[:n_free] in request order and are written into `table` [R, max_blocks]; a request that
     cannot have all its blocks gets none: its slots are -1 and its length stays."""
-    if table.dim() != 2:
-        raise EngineError(f"table: [requests, blocks], got {tuple(table.shape)}")
-    if not table.is_cuda:
-        raise EngineError(f"table: a CUDA tensor, got {table.device}")
-    if total < 0:
-        raise EngineError(f"total {total}")
-    R, mb = table.shape
-    # one allocation: cu, then the [R] and [total] outputs
-    buf = torch.empty(2 * R + 2 + 2 * total, dtype=torch.int32, device=table.device)
-    cu, out_lens, out_free, positions, slots = buf.split((R + 1, R, 1, total, total))
-    base = buf.data_ptr()
-    args = _lib.KV_EXTEND_ARGS.pack(
-        _int32(table, "table", table), _int32(lens, "lens", table, R), _int32(new_lens, "new_lens", table, R),
-        _int32(free, "free", table), _int32(n_free, "n_free", table, 1), base, base + 4 * (2 * R + 2),
-        base + 4 * (2 * R + 2 + total), base + 4 * (R + 1), base + 4 * (2 * R + 1), R, mb, total, block_size, free.numel(), 0)
-    with torch.cuda.device(table.device):
-        st = _lib.load().rmoe_kv_extend(args, _stream_of(table, stream, lens, new_lens, free, n_free, buf))
-    if st:
-        _call(st)
-    return KVStep(cu, positions, slots, out_lens, out_free)
+    if stream is not None:
+        with _on(stream, table, lens, new_lens, free, n_free):
+            return extend_tables(table, lens, new_lens, free, n_free, total, block_size)
+    return KVStep(*_ops().extend(table, lens, new_lens, free, n_free, total, block_size))
 
 
 class KVBatch:
@@ -236,14 +190,16 @@ class KVBatch:
 
     def release(self, done, *, stream=None):
         """rmoe_kv_release: requests with done[r] != 0 (int32 [R]) give their blocks back."""
+        if stream is not None:
+            with _on(stream, self.table, self.lens, self.free, done, self.n_free):
+                return self.release(done)
         R, mb = self.table.shape
-        out = torch.empty_like(self.n_free)
-        args = _lib.KV_RELEASE_ARGS.pack(self.table.data_ptr(), self.lens.data_ptr(), self.free.data_ptr(),
-                                         _int32(done, "done", self.table, R), self.n_free.data_ptr(), out.data_ptr(), R, mb,
-                                         self.block_size, self.free.numel())
         with torch.cuda.device(self.table.device):
-            _call(_lib.load().rmoe_kv_release(args, _stream_of(self.table, stream, self.lens, self.free, done, self.n_free,
-                                                               out)))
+            out = torch.empty_like(self.n_free)
+            args = _lib.KV_RELEASE_ARGS.pack(self.table.data_ptr(), self.lens.data_ptr(), self.free.data_ptr(),
+                                             _int32(done, "done", self.table, R), self.n_free.data_ptr(), out.data_ptr(),
+                                             R, mb, self.block_size, self.free.numel())
+            _call(_lib.load().rmoe_kv_release(args, _stream()))
         self.n_free = out
 
 
@@ -291,55 +247,29 @@ class KVCache:
         h = C.c_void_p()
         L = _lib.load()
         _call(L.rmoe_kv_create(C.byref(d), C.byref(h)))
-        self._h, self._append, self._read, self._attend = h, L.rmoe_kv_append, L.rmoe_kv_read, L.rmoe_kv_attend
+        ops = _ops()
+        self._h, self._p, self._append, self._read, self._attend = h, h.value, ops.append, ops.read, ops.attend
+        self._scale = 1.0 / math.sqrt(self.head_dim)
+        self._like = {dt: torch.empty(0, dtype=dt, device=k.device) for dt in (torch.float32, torch.float16, torch.bfloat16)}
 
     def append(self, k, v, slots, *, rope: Optional[Rope] = None, positions=None, q=None, q_out=None, stream=None):
         """Writes k and v [tokens, n_kv_heads, head_dim] at `slots` (int32, -1 skips).  With a
         rope, k is turned by `positions` first, and so is q where given; returns the turned q."""
-        ty = _type_of(k, "k")
-        T = k.shape[0]
-        _same(v, k, "v")
-        kr, vr = _rows(k, "k"), _rows(v, "v")
-        want = (T, self.n_kv_heads, self.head_dim)
-        if k.shape != want or v.shape != want:
-            raise EngineError(f"k {tuple(k.shape)} / v {tuple(v.shape)}, expected {want}")
-        if k.device.index != self.device:
-            raise EngineError(f"k is on {k.device}, the cache on device {self.device}")
-        qr = qor = _NO_ROWS
-        pp = rh = 0
-        if rope is not None:
-            if positions is None:
-                raise EngineError("rope needs positions")
-            pp, rh = _int32(positions, "positions", k, T), rope._h.value
-            if q is not None:
-                _same(q, k, "q")
-                if q_out is None:
-                    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-                _same(q_out, q, "q_out")
-                qr, qor = _rows(q, "q"), _rows(q_out, "q_out")
-                if q.shape[0] != T or q.shape[2] != self.head_dim or q_out.shape != q.shape:
-                    raise EngineError(f"q {tuple(q.shape)} / {tuple(q_out.shape)} beside k {tuple(k.shape)}")
-        elif q is not None:
-            raise EngineError("q is only taken with a rope")
-        args = _lib.KV_APPEND_ARGS.pack(*kr, *vr, *qr, *qor, _int32(slots, "slots", k, T), pp, rh, T, ty)
-        st = self._append(self._h, args, _stream_of(k, stream, v, slots, positions, q, q_out))
-        if st:
-            _call(st)
-        return q_out
+        if stream is not None:
+            with _on(stream, k, v, slots, positions, q, q_out):
+                return self.append(k, v, slots, rope=rope, positions=positions, q=q, q_out=q_out)
+        return self._append(self._p, self.device, self.n_kv_heads, self.head_dim, k, v, slots, 0 if rope is None else rope._p,
+                            positions, q, q_out)
 
     def read(self, slots, dtype=None, *, stream=None):
         """(k, v) of cached tokens [slots, n_kv_heads, head_dim], code * scale, as `dtype` (float32)."""
-        dtype = torch.float32 if dtype is None else dtype
-        if dtype not in _TYPES:
-            raise EngineError(f"read as {dtype}")
-        n = slots.numel()
-        p = _int32(slots, "slots", self.k)
-        both = torch.empty((2, n, self.n_kv_heads, self.head_dim), dtype=dtype, device=self.k.device)
-        k, v = both.unbind(0)
-        st = self._read(self._h, p, n, _TYPES[dtype], k.data_ptr(), v.data_ptr(), _stream_of(both, stream, slots))
-        if st:
-            _call(st)
-        return k, v
+        like = self._like.get(torch.float32 if dtype is None else dtype)
+        if like is None:
+            raise EngineError(f"read as {dtype}: float32, float16 or bfloat16")
+        if stream is not None:
+            with _on(stream, slots):
+                return self.read(slots, dtype)
+        return self._read(self._p, self.k, slots, like)
 
     def attend(self, q, table, lens, cu, *, scale: Optional[float] = None, window: int = 0, max_new: Optional[int] = None,
                out=None, return_lse: bool = False, stream=None):
@@ -348,31 +278,12 @@ class KVCache:
         window, each query sees that many keys at most.  scale: 1 / sqrt(head_dim) by default.
         max_new: an upper bound of any request's new tokens, where known (chooses kernels only).
         Returns out (as q), or (out, lse [tokens, q heads] f32)."""
-        ty = _type_of(q, "q")
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        else:
-            _same(out, q, "out")
-        qr, orow = _rows(q, "q"), _rows(out, "out")
-        T, nq, dim = q.shape
-        if dim != self.head_dim or out.shape != q.shape:
-            raise EngineError(f"q {tuple(q.shape)} / out {tuple(out.shape)} with head_dim {self.head_dim}")
-        if q.device.index != self.device:
-            raise EngineError(f"q is on {q.device}, the cache on device {self.device}")
-        if table.dim() != 2:
-            raise EngineError(f"table: [requests, blocks], got {tuple(table.shape)}")
-        R, mb = table.shape
-        if window < 0 or (max_new is not None and max_new < 0):
-            raise EngineError(f"window {window}, max_new {max_new}")
-        lse = torch.empty((T, nq), dtype=torch.float32, device=q.device) if return_lse else None
-        args = _lib.KV_ATTEND_ARGS.pack(
-            *qr, *orow, _int32(table, "table", q), _int32(lens, "lens", q, R), _int32(cu, "cu", q, R + 1),
-            lse.data_ptr() if return_lse else 0, R, mb, T, ty, 1.0 / math.sqrt(dim) if scale is None else scale, window,
-            max_new or 0, 0)
-        st = self._attend(self._h, args, _stream_of(q, stream, out, table, lens, cu, lse))
-        if st:
-            _call(st)
-        return (out, lse) if return_lse else out
+        if stream is not None:
+            with _on(stream, q, table, lens, cu, out):
+                return self.attend(q, table, lens, cu, scale=scale, window=window, max_new=max_new, out=out,
+                                   return_lse=return_lse)
+        return self._attend(self._p, self.device, self.head_dim, q, table, lens, cu, self._scale if scale is None else scale,
+                            window, max_new or 0, out, return_lse)
 
     def check(self):
         """Raises if a call so far met a device error (synchronises and clears it)."""
@@ -381,7 +292,7 @@ class KVCache:
     def close(self):
         if getattr(self, "_h", None) is not None and self._h.value:
             _lib.load().rmoe_kv_destroy(self._h)
-            self._h = C.c_void_p()
+            self._h, self._p = C.c_void_p(), 0
 
     def __del__(self):
         try:
