@@ -17,6 +17,8 @@ template <typename T, int CODE>
 __global__ void __launch_bounds__(128) kv_append_kernel(KvArg kv, AppendArg a) {
     const int t0 = blockIdx.x, h = blockIdx.y, isv = blockIdx.z, tid = threadIdx.x;
     const int bs = kv.bs, dim = kv.dim;
+    pdl_trigger();
+    pdl_wait();
     const int slot = __ldg(a.slots + t0);
     if (slot < 0) return;
     const int first = slot & (bs - 1), block = slot / bs;
@@ -98,6 +100,8 @@ __global__ void __launch_bounds__(128) kv_append_kernel(KvArg kv, AppendArg a) {
 // One thread per 16 elements of a slot and head, K then V.
 template <typename T, int CODE>
 __global__ void __launch_bounds__(256) kv_read_kernel(KvArg kv, const int32_t* slots, int n, T* ko, T* vo) {
+    pdl_trigger();
+    pdl_wait();
     const int units = kv.dim / 16;
     const uint64_t per = (uint64_t)n * kv.heads * units, all = 2 * per;
     for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < all; i += gridDim.x * 256ull) {
@@ -128,15 +132,14 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvArg kv, const int32_t* s
 
 template <typename T, int CODE>
 static cudaError_t append_launch(const KvArg& kv, const AppendArg& a, cudaStream_t s) {
-    kv_append_kernel<T, CODE><<<dim3((unsigned)a.T, (unsigned)kv.heads, 2), 128, 0, s>>>(kv, a);
-    return cudaGetLastError();
+    return launch_pdl(kv_append_kernel<T, CODE>, dim3((unsigned)a.T, (unsigned)kv.heads, 2), dim3(128), 0, s, kv, a);
 }
 
 template <typename T, int CODE>
 static cudaError_t read_launch(const KvArg& kv, const int32_t* slots, int n, void* ko, void* vo, cudaStream_t s) {
     const uint64_t all = 2ull * n * kv.heads * (kv.dim / 16), ctas = (all + 255) / 256;
-    kv_read_kernel<T, CODE><<<(unsigned)(ctas < 148 * 64 ? ctas : 148 * 64), 256, 0, s>>>(kv, slots, n, (T*)ko, (T*)vo);
-    return cudaGetLastError();
+    return launch_pdl(kv_read_kernel<T, CODE>, dim3((unsigned)(ctas < 148 * 64 ? ctas : 148 * 64)), dim3(256), 0, s, kv, slots, n,
+                      (T*)ko, (T*)vo);
 }
 
 }  // namespace rmoe

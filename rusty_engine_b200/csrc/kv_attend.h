@@ -9,6 +9,7 @@ struct AttendArg {
     const int32_t *table, *lens, *cu;
     float* lse;
     int R, max_blocks, T;
+    int group;  // query heads per kv head
     float scale;
     int window;
     bool prompts;  // the prompt kernel runs too and takes the requests of more than split_max_rows rows

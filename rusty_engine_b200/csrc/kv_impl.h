@@ -88,9 +88,11 @@ struct KvArg {
     float *ks, *vs;
     int n_blocks, bs, heads, dim;  // bs a power of two
     unsigned* status;
+    int shift;                     // log2 bs
 };
 inline KvArg kv_arg(const rmoe_kv* kv) {
-    return KvArg{kv->k, kv->v, kv->ks, kv->vs, (int)kv->n_blocks, (int)kv->bs, (int)kv->heads, (int)kv->dim, kv->status};
+    return KvArg{kv->k, kv->v, kv->ks, kv->vs, (int)kv->n_blocks, (int)kv->bs, (int)kv->heads, (int)kv->dim, kv->status,
+                 kv->bs == 16 ? 4 : kv->bs == 32 ? 5 : kv->bs == 64 ? 6 : 7};
 }
 inline bool block_size_ok(uint32_t bs) { return bs == 16 || bs == 32 || bs == 64 || bs == 128; }
 

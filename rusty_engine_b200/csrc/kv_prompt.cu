@@ -84,9 +84,11 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     __shared__ float s_fin[2][PAIR ? 128 : 1];            // f32: M and l of the rows
 
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, wg = w >> 2;
-    const int heads = kv.heads, bs = kv.bs, group = a.q.heads / heads;
+    const int heads = kv.heads, bs = kv.bs, group = a.group;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
 
+    pdl_trigger();
+    pdl_wait();
     // ---- which request, head and rows ----
     const int64_t max_rows = split_max_rows(a, heads, group, s_sum);
     if (max_rows == INT64_MAX) return;
@@ -172,7 +174,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
         const int br = min(bs, PKV), nb = PKV / br;
         auto lookup = [&](int j) {
             const int t = (jt0 + j) * PKV + 16 * lane;
-            return j < nt && lane < 8 && t < kmax ? __ldg(a.table + (int64_t)r * a.max_blocks + t / bs) : -1;
+            return j < nt && lane < 8 && t < kmax ? __ldg(a.table + (int64_t)r * a.max_blocks + (t >> kv.shift)) : -1;
         };
         int blk = lookup(0), issued = 0;
         for (int j = 0; j < nt; j++) {
@@ -553,8 +555,7 @@ static cudaError_t prompt_launch(const KvMaps& maps, const KvArg& kv, const Atte
     // an upper bound of the row tiles: whole ones, and a partial one per request
     const int64_t ctas = ((int64_t)a.T * group / per + min(a.R, a.T)) * kv.heads;
     if (ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    k<<<(unsigned)ctas, PT, S::SMEM, s>>>(maps.k, maps.v, kv, a);
-    return cudaGetLastError();
+    return launch_pdl(k, dim3((unsigned)ctas), dim3(PT), S::SMEM, s, maps.k, maps.v, kv, a);
 }
 
 template <typename T, int CODE>

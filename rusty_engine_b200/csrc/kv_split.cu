@@ -91,6 +91,11 @@ struct SplitPiece {   // where a piece belongs
     int flags;        // 1: valid, 2: holds the item's first tile, 4: holds its last
 };
 
+// a / b for a >= 0, b > 0: in 32 bits where they fit (a 64-bit division is a hundred instructions).
+__device__ __forceinline__ int64_t quot(int64_t a, int64_t b) {
+    return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 template <typename T, int CODE, int D, int NR>
 __global__ void __launch_bounds__(SPLIT_NW * 32, 1)
 kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, KvArg kv, AttendArg a,
@@ -104,7 +109,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     constexpr int BX = D == 256 ? 2 : 1;       // 128-byte boxes per row
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t s_full[NW][DEPTH];
-    __shared__ float s_scale[NW][DEPTH][2][2];  // per box of the tile: K scale (-1: no such block), V scale
+    __shared__ __align__(8) float s_scale[NW][DEPTH][2][2];  // per box of the tile: K scale (-1: no such block), V scale
     __shared__ int64_t s_pre[NT];
     __shared__ int64_t s_tot[NW];
     __shared__ SplitPiece s_piece[2 * NW];
@@ -113,19 +118,11 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, c = lane & 3;
     const uint32_t ring0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* ring_ptr = smem_raw + (ring0 - smem_u32(smem_raw));
-    const int heads = kv.heads, bs = kv.bs, group = a.q.heads / heads;
+    const int heads = kv.heads, bs = kv.bs, group = a.group;
 
-    // ---- tokens of no request ----
-    {
-        const int first = min(max(__ldg(a.cu), 0), a.T), end = min(max(__ldg(a.cu + a.R), first), a.T);
-        const int64_t rest = (int64_t)(a.T - (end - first)) * a.q.heads;
-        for (int64_t i = (int64_t)blockIdx.x * NW + w; i < rest; i += (int64_t)gridDim.x * NW) {
-            const int k = (int)(i / a.q.heads), h = (int)(i % a.q.heads), t = k < first ? k : end + (k - first);
-            T* o = reinterpret_cast<T*>(a.out.p) + t * a.out.st + h * a.out.sh;
-            for (int d = lane; d < D; d += 32) o[d] = Elt<T>::put(0.0f);
-            if (lane == 0 && a.lse) a.lse[(int64_t)t * a.q.heads + h] = -INFINITY;
-        }
-    }
+    const int br = min(bs, TW), nb = TW / br;  // rows and number of a tile's boxes
+    pdl_trigger();
+    pdl_wait();
 
     // ---- this CTA's share of the units ----
     const int per = (a.R + NT - 1) / NT;
@@ -144,7 +141,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     if (lane == 31) s_tot[w] = incl;
     if (tid < 2 * NW) s_piece[tid].flags = 0;
     if (lane == 0) {
-        for (int i = 0; i < DEPTH; i++) tc::mbar_init(smem_u32(&s_full[w][i]), 1 + (bs < TW ? TW / bs : 1));
+        for (int i = 0; i < DEPTH; i++) tc::mbar_init(smem_u32(&s_full[w][i]), 1 + nb);
         tc::fence_mbar_init();
     }
     __syncthreads();
@@ -158,9 +155,9 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     __syncthreads();
     // a share of less than a tile per warp would only add joining
     const int64_t active = min((int64_t)gridDim.x, (W + NW - 1) / NW);
-    if (blockIdx.x >= active) return;
-    auto share = [&](int64_t cta) { return W * cta / active; };
-    const int64_t u0 = share(blockIdx.x), u1 = share(blockIdx.x + 1);
+    const int64_t each = active ? quot(W, active) : 0, extra = W - each * active;  // the first `extra` CTAs take one more
+    auto share = [&](int64_t cta) { return each * cta + min(cta, extra); };
+    const int64_t u0 = share(blockIdx.x), u1 = blockIdx.x < active ? share(blockIdx.x + 1) : u0;
     const int64_t wu0 = u0 + (u1 - u0) * w / NW, wu1 = u0 + (u1 - u0) * (w + 1) / NW;
 
     if (wu0 < wu1) {
@@ -177,10 +174,9 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             rem -= (int64_t)rq.items * rq.tiles;
             rq = split_req(a, ++r, heads, group, bs, NR, TW, max_rows);
         }
-        int item = (int)(rem / rq.tiles), tile = (int)(rem % rq.tiles);
+        int item = (int)quot(rem, rq.tiles), tile = (int)(rem - (int64_t)item * rq.tiles);
 
         // ---- the issuing side: runs DEPTH tiles ahead ----
-        const int br = min(bs, TW), nb = TW / br;  // rows and number of a tile's boxes
         SplitReq pq = rq;
         int pr = r, pitem = item, ptile = tile;
         int64_t pleft = wu1 - wu0;
@@ -188,7 +184,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         auto lookup = [&]() {  // lane b < nb: the block of box b of the tile to issue next
             const int j = (pq.t0 + ptile) * TW + lane * br;
             pblk = -1;
-            if (lane < nb && pleft > 0 && j < pq.hi) pblk = __ldg(a.table + (int64_t)pr * a.max_blocks + j / bs);
+            if (lane < nb && pleft > 0 && j < pq.hi) pblk = __ldg(a.table + (int64_t)pr * a.max_blocks + (j >> kv.shift));
         };
         lookup();
         auto issue = [&](int stage) {
@@ -306,7 +302,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             }
             for (int s = 0; s < seg; s++, cnt++) {
                 const int stage = cnt % DEPTH;
-                if (!__all_sync(0xffffffffu, tc::mbar_wait(smem_u32(&s_full[w][stage]), (cnt / DEPTH) & 1))) {
+                if (!__all_sync(0xffffffffu, tc::mbar_wait_tries(smem_u32(&s_full[w][stage]), (cnt / DEPTH) & 1))) {
                     dead = true;
                     break;
                 }
@@ -316,11 +312,11 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 bool gone = false;
 #pragma unroll
                 for (int i = 0; i < MT; i++) {
-                    const int b = MT == 2 && br == 16 ? i : 0;
-                    kscale[i] = s_scale[w][stage][b][0];
-                    const float vs = v_scale_floor(s_scale[w][stage][b][1]);
-                    lv[i] = log2f(vs);
-                    iv[i] = 1.0f / vs;
+                    const float2 sc = *reinterpret_cast<const float2*>(s_scale[w][stage][MT == 2 && br == 16 ? i : 0]);
+                    const float vs = v_scale_floor(sc.y);
+                    kscale[i] = sc.x;
+                    lv[i] = lg2(vs);
+                    iv[i] = rcp(vs);
                     gone |= kscale[i] < 0.0f;
                 }
                 const bool masked = gone || j0 < all_lo || j0 + TW > all_hi;
@@ -386,15 +382,26 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 for (int nt = 0; nt < QT; nt++) {
                     float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
+                    for (int i = 0; i < MT; i++) {
+                        const float sc[2] = {qs[nt][0] * kscale[i], qs[nt][1] * kscale[i]};
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            st[nt][i][e] = fmaf(PAIR ? st[nt][i][e] + su[nt][i][e] : st[nt][i][e], sc[e & 1], lv[i]);
+                    }
+                    if (masked) {
+#pragma unroll
+                        for (int i = 0; i < MT; i++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const int q = e & 1, j = j0 + 16 * i + 8 * (e >> 1) + tg;
+                                if (j >= vhi[nt][q] || j < vlo[nt][q] || kscale[i] < 0.0f) st[nt][i][e] = -INFINITY;
+                            }
+                        asm volatile("" ::: "memory");  // a branch: few tiles are masked
+                    }
+#pragma unroll
                     for (int i = 0; i < MT; i++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int q = e & 1, j = j0 + 16 * i + 8 * (e >> 1) + tg;
-                            float x = fmaf(PAIR ? st[nt][i][e] + su[nt][i][e] : st[nt][i][e], qs[nt][q] * kscale[i], lv[i]);
-                            if (masked && (j >= vhi[nt][q] || j < vlo[nt][q] || kscale[i] < 0.0f)) x = -INFINITY;
-                            st[nt][i][e] = x;
-                            mx[q] = fmaxf(mx[q], x);
-                        }
+                        for (int e = 0; e < 4; e++) mx[e & 1] = fmaxf(mx[e & 1], st[nt][i][e]);
                     float al[2], mu[2];
 #pragma unroll
                     for (int q = 0; q < 2; q++) {
@@ -553,7 +560,19 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         if (dead) {  // a copy did not arrive: say so, and let what is in flight land
             if (lane == 0) atomicOr(kv.status, (unsigned)DERR_TIMEOUT);
             for (int64_t k = (wu1 - wu0) - pleft; (int64_t)cnt < k; cnt++)
-                tc::mbar_wait(smem_u32(&s_full[w][cnt % DEPTH]), (cnt / DEPTH) & 1);
+                tc::mbar_wait_tries(smem_u32(&s_full[w][cnt % DEPTH]), (cnt / DEPTH) & 1);
+        }
+    }
+
+    // ---- tokens of no request ----
+    {
+        const int first = min(max(__ldg(a.cu), 0), a.T), end = min(max(__ldg(a.cu + a.R), first), a.T);
+        const int64_t rest = (int64_t)(a.T - (end - first)) * a.q.heads;
+        for (int64_t i = (int64_t)blockIdx.x * NW + w; i < rest; i += (int64_t)gridDim.x * NW) {
+            const int k = (int)(i / a.q.heads), h = (int)(i % a.q.heads), t = k < first ? k : end + (k - first);
+            T* o = reinterpret_cast<T*>(a.out.p) + t * a.out.st + h * a.out.sh;
+            for (int d = lane; d < D; d += 32) o[d] = Elt<T>::put(0.0f);
+            if (lane == 0 && a.lse) a.lse[(int64_t)t * a.q.heads + h] = -INFINITY;
         }
     }
 
@@ -620,10 +639,8 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         if (whole) continue;
         // the CTAs that hold the item's first and last unit
         auto cta_of = [&](int64_t u) {
-            int64_t x = u * active / W;
-            while (share(x + 1) <= u) x++;
-            while (share(x) > u) x--;
-            return (int)x;
+            const int64_t big = extra * (each + 1);
+            return (int)(u < big ? quot(u, each + 1) : extra + quot(u - big, each));
         };
         const int c0 = cta_of(pc.a), c1 = cta_of(pc.a + pc.tiles - 1);
         __threadfence();
@@ -652,8 +669,7 @@ static cudaError_t split_launch(const KvMaps& maps, const KvArg& kv, const Atten
     static std::atomic<uint64_t> done{0};
     cudaError_t e = allow_smem(k, smem, done);
     if (e != cudaSuccess) return e;
-    k<<<sms, SPLIT_NW * 32, smem, s>>>(maps.k, maps.v, kv, a, ws);
-    return cudaGetLastError();
+    return launch_pdl(k, dim3(sms), dim3(SPLIT_NW * 32), smem, s, maps.k, maps.v, kv, a, ws);
 }
 
 // nr: 8 or 16 rows per item (16 only up to head_dim 128: the accumulators of 256 would spill)

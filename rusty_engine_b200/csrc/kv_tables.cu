@@ -43,6 +43,8 @@ __global__ void __launch_bounds__(EXT_THREADS) kv_extend_kernel(rmoe_kv_extend_a
     __shared__ int s_used;
     const int tid = threadIdx.x, R = (int)a.R, bs = (int)a.block_size;
     const int per = (R + EXT_THREADS - 1) / EXT_THREADS, r0 = min(R, tid * per), r1 = min(R, r0 + per);
+    pdl_trigger();
+    pdl_wait();
     const int height = max(0, min(__ldg(a.n_free), (int)a.free_cap));
     if (tid == 0) s_used = 0;
     int64_t mine = 0, total = 0;
@@ -172,8 +174,8 @@ rmoe_status rmoe_kv_extend(const rmoe_kv_extend_args* a, void* stream) {
     cudaError_t e = allow_smem(kv_extend_kernel, 132 << 10, done);
     if (e != cudaSuccess) return cuda_fail(e, "kv extend");
     const unsigned grid = (unsigned)((a->T + EXT_THREADS - 1) / EXT_THREADS);
-    kv_extend_kernel<<<grid < 1 ? 1 : grid < 148 ? grid : 148, EXT_THREADS, smem, static_cast<cudaStream_t>(stream)>>>(*a);
-    e = cudaGetLastError();
+    e = launch_pdl(kv_extend_kernel, dim3(grid < 1 ? 1 : grid < 148 ? grid : 148), dim3(EXT_THREADS), smem,
+                   static_cast<cudaStream_t>(stream), *a);
     return e == cudaSuccess ? RMOE_OK : cuda_fail(e, "kv extend launch");
 }
 

@@ -28,6 +28,17 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
@@ -38,7 +49,8 @@ __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
 }
 
 // The V scale enters the exponent: log2 of it is added to the score, and a row's sum takes its
-// reciprocal.  A scale below 2^-100 (zero included) counts as 2^-100.
+// reciprocal (to 2^-22: an error of the logarithm changes a block's weights alike in both sums and
+// is as small as the weights' own).  A scale below 2^-100 (zero included) counts as 2^-100.
 __device__ __forceinline__ float v_scale_floor(float vs) { return fmaxf(vs, 7.8886090522101181e-31f); }
 
 // The exponent e that brings a row of q whose largest magnitude is mx to mx 2^-e in [2^13, 2^14);

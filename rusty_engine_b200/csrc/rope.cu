@@ -25,6 +25,8 @@ __global__ void __launch_bounds__(256) rope_table_kernel(float2* table, const do
 template <typename T>
 __global__ void __launch_bounds__(256) rope_units_kernel(Rows q, Rows qo, Rows k, Rows ko, RopeArg ra, int T_, int dim,
                                                          unsigned* status) {
+    pdl_trigger();
+    pdl_wait();
     const int per_head = dim / 16, per_tok = (q.heads + k.heads) * per_head;
     const uint64_t n = (uint64_t)T_ * per_tok;
     for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += gridDim.x * 256ull) {
@@ -54,6 +56,8 @@ __global__ void __launch_bounds__(256) rope_units_kernel(Rows q, Rows qo, Rows k
 template <typename T>
 __global__ void __launch_bounds__(256) rope_pairs_kernel(Rows q, Rows qo, Rows k, Rows ko, RopeArg ra, int T_, int dim,
                                                          unsigned* status) {
+    pdl_trigger();
+    pdl_wait();
     const int per_head = ra.rot / 2 + (dim - ra.rot), per_tok = (q.heads + k.heads) * per_head;
     const uint64_t n = (uint64_t)T_ * per_tok;
     for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += gridDim.x * 256ull) {
@@ -89,11 +93,8 @@ static cudaError_t rope_launch(const Rows& q, const Rows& qo, const Rows& k, con
     const bool units = dim % 16 == 0 && ra.rot % 16 == 0;
     const uint64_t n = (uint64_t)T_ * (q.heads + k.heads) * (units ? dim / 16 : dim - ra.rot / 2);
     const unsigned grid = (unsigned)((n + 255) / 256 < 148 * 64 ? (n + 255) / 256 : 148 * 64);
-    if (units)
-        rope_units_kernel<T><<<grid, 256, 0, s>>>(q, qo, k, ko, ra, T_, dim, status);
-    else
-        rope_pairs_kernel<T><<<grid, 256, 0, s>>>(q, qo, k, ko, ra, T_, dim, status);
-    return cudaGetLastError();
+    return launch_pdl(units ? rope_units_kernel<T> : rope_pairs_kernel<T>, dim3(grid), dim3(256), 0, s, q, qo, k, ko, ra, T_, dim,
+                      status);
 }
 
 cudaError_t launch_rope_apply(const Rows& q, const Rows& qo, const Rows& k, const Rows& ko, const RopeArg& ra, int T,
