@@ -27,6 +27,8 @@ extern "C" rmoe_status rmoe_kv_attend(rmoe_kv* kv, const rmoe_kv_attend_args* a,
     const KvArg ka = kv_arg(kv);
     const uint64_t group = a->q.heads / kv->heads;
     p.group = (int)group;
+    p.group_inv = group > 1 ? (uint32_t)((0xffffffffull + group) / group) : 0;
+    if (group > 32768) return fail(RMOE_ERR_UNSUPPORTED, "%llu query heads per kv head", (unsigned long long)group);
     // Without a bound on any request's new tokens: one each when there are as many tokens as
     // requests.  A wrong guess costs time only, the split kernel takes whatever the other does not.
     const uint64_t longest = std::min<uint64_t>(a->max_new ? a->max_new : a->T > a->R ? a->T : 1, a->T);

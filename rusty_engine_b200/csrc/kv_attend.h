@@ -9,7 +9,8 @@ struct AttendArg {
     const int32_t *table, *lens, *cu;
     float* lse;
     int R, max_blocks, T;
-    int group;  // query heads per kv head
+    int group;           // query heads per kv head
+    uint32_t group_inv;  // ceil(2^32 / group): x / group = mulhi(x, group_inv) for x < 2^16; 0 for group 1
     float scale;
     int window;
     bool prompts;  // the prompt kernel runs too and takes the requests of more than split_max_rows rows

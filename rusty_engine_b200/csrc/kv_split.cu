@@ -22,6 +22,8 @@
 // warps' pieces, and items that span CTAs go through a workspace slot per CTA, where the last
 // arriving CTA (an atomic count, nobody waits) joins them in CTA order: the result does not depend
 // on timing.
+#include <algorithm>
+
 #include "kv_attend.h"
 #include "kv_widen.cuh"
 #include "rope.cuh"
@@ -31,6 +33,7 @@ namespace rmoe {
 
 static constexpr int SPLIT_NW = 8;      // warps per CTA
 static constexpr int SPLIT_DEPTH = 2;   // tiles in a warp's ring
+static constexpr int SPLIT_MAX_SMS = 160;  // CTAs at most
 
 template <int D>
 struct SplitShape {
@@ -41,7 +44,8 @@ struct SplitShape {
 
 template <int D, int NR>
 struct SplitSmem {
-    static constexpr int PIECE = NR * (D + 2);        // floats: M[NR], l[NR], O[NR][D]
+    static constexpr int ROW = D + 4;                 // floats between the rows of a piece (bank offset)
+    static constexpr int PIECE = NR * (ROW + 2);      // O[NR][ROW], M[NR], l[NR]
     static constexpr int RING = SPLIT_NW * SPLIT_DEPTH * SplitShape<D>::STAGE;
     static constexpr int FIRST = SPLIT_NW * PIECE * 4;
     static constexpr int TOTAL = RING + FIRST + 1024;  // + alignment of the ring
@@ -96,6 +100,12 @@ __device__ __forceinline__ int64_t quot(int64_t a, int64_t b) {
     return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
+struct SplitStart {   // where a warp's share begins
+    SplitReq rq;
+    int r;
+    int64_t rem;      // units of the request before it
+};
+
 template <typename T, int CODE, int D, int NR>
 __global__ void __launch_bounds__(SPLIT_NW * 32, 1)
 kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, KvArg kv, AttendArg a,
@@ -110,7 +120,8 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t s_full[NW][DEPTH];
     __shared__ __align__(8) float s_scale[NW][DEPTH][2][2];  // per box of the tile: K scale (-1: no such block), V scale
-    __shared__ int64_t s_pre[NT];
+    __shared__ SplitStart s_start[NW];
+    __shared__ float s_f[SPLIT_MAX_SMS][NR], s_m[NR], s_l[NR];  // joining: factors of the pieces, the joined M and l
     __shared__ int64_t s_tot[NW];
     __shared__ SplitPiece s_piece[2 * NW];
     __shared__ int s_last;
@@ -128,9 +139,10 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     const int per = (a.R + NT - 1) / NT;
     const int64_t max_rows = a.prompts ? split_max_rows(a, heads, group, s_tot) : INT64_MAX;
     int64_t mine = 0;
+    SplitReq rq{};
     for (int r = tid * per; r < min(a.R, (tid + 1) * per); r++) {
-        const SplitReq q = split_req(a, r, heads, group, bs, NR, TW, max_rows);
-        mine += (int64_t)q.items * q.tiles;
+        rq = split_req(a, r, heads, group, bs, NR, TW, max_rows);
+        mine += (int64_t)rq.items * rq.tiles;
     }
     int64_t incl = mine;
 #pragma unroll
@@ -151,29 +163,40 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         if (i < w) before += s_tot[i];
         W += s_tot[i];
     }
-    s_pre[tid] = before + incl - mine;
-    __syncthreads();
     // a share of less than a tile per warp would only add joining
     const int64_t active = min((int64_t)gridDim.x, (W + NW - 1) / NW);
     const int64_t each = active ? quot(W, active) : 0, extra = W - each * active;  // the first `extra` CTAs take one more
     auto share = [&](int64_t cta) { return each * cta + min(cta, extra); };
     const int64_t u0 = share(blockIdx.x), u1 = blockIdx.x < active ? share(blockIdx.x + 1) : u0;
-    const int64_t wu0 = u0 + (u1 - u0) * w / NW, wu1 = u0 + (u1 - u0) * (w + 1) / NW;
+    auto warp_unit = [&](int i) { return u0 + (u1 - u0) * i / NW; };
+    const int64_t wu0 = warp_unit(w), wu1 = warp_unit(w + 1);
+    // the thread that holds a warp's first unit tells it where that is
+    {
+        const int64_t at = before + incl - mine;
+#pragma unroll
+        for (int i = 0; i < NW; i++) {
+            const int64_t u = warp_unit(i);
+            if (u >= at && u < at + mine) {
+                int64_t rem = u - at;
+                int r = tid * per;
+                SplitReq q = rq;
+                if (per > 1) {
+                    q = split_req(a, r, heads, group, bs, NR, TW, max_rows);
+                    while (rem >= (int64_t)q.items * q.tiles) {
+                        rem -= (int64_t)q.items * q.tiles;
+                        q = split_req(a, ++r, heads, group, bs, NR, TW, max_rows);
+                    }
+                }
+                s_start[i] = SplitStart{q, r, rem};
+            }
+        }
+    }
+    __syncthreads();
 
     if (wu0 < wu1) {
-        // ---- the request, item and tile of the warp's first unit ----
-        int lo = 0, hi = NT - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (s_pre[mid] <= wu0) lo = mid; else hi = mid - 1;
-        }
-        int r = lo * per;
-        int64_t rem = wu0 - s_pre[lo];
-        SplitReq rq = split_req(a, r, heads, group, bs, NR, TW, max_rows);
-        while (rem >= (int64_t)rq.items * rq.tiles) {
-            rem -= (int64_t)rq.items * rq.tiles;
-            rq = split_req(a, ++r, heads, group, bs, NR, TW, max_rows);
-        }
+        rq = s_start[w].rq;
+        int r = s_start[w].r;
+        const int64_t rem = s_start[w].rem;
         int item = (int)quot(rem, rq.tiles), tile = (int)(rem - (int64_t)item * rq.tiles);
 
         // ---- the issuing side: runs DEPTH tiles ahead ----
@@ -238,16 +261,19 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         while (left > 0 && !dead) {
             const int seg = (int)min(left, (int64_t)(rq.tiles - tile));
             const int kh = item % heads, row0 = item / heads * NR;
+            // row row0 + i is token tok0 + (rem0 + i) / group, head (rem0 + i) % group of the group
+            const int tok0 = row0 / group, rem0 = row0 - tok0 * group;
+            auto tok_of = [&](int i) { return tok0 + (group == 1 ? i : (int)__umulhi((uint32_t)(rem0 + i), a.group_inv)); };
             // q rows as B operands, scaled to the fp16 range row by row
             uint32_t qh[QT][KS][2], ql[PAIR ? QT : 1][PAIR ? KS : 1][2];
             float qs[QT][2];
             int vhi[QT][2], vlo[QT][2];
 #pragma unroll
             for (int nt = 0; nt < QT; nt++) {
-                const int row = row0 + nt * 8 + g, tok = row / group;
+                const int tok = tok_of(nt * 8 + g), gh = row0 + nt * 8 + g - tok * group;
                 const bool live = tok < rq.n;
                 const T* qp = reinterpret_cast<const T*>(a.q.p) + (int64_t)(rq.q0 + (live ? tok : 0)) * a.q.st +
-                              (int64_t)(kh * group + row % group) * a.q.sh;
+                              (int64_t)(kh * group + gh) * a.q.sh;
                 float v[HF][16], mx = 0.0f;
 #pragma unroll
                 for (int hf = 0; hf < HF; hf++) {
@@ -281,13 +307,13 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
 #pragma unroll
                 for (int i = 0; i < 2; i++) {  // of the rows 2c, 2c + 1 whose sums this lane holds
                     qs[nt][i] = __shfl_sync(0xffffffffu, up, (2 * c + i) * 4);
-                    const int t2 = (row0 + nt * 8 + 2 * c + i) / group, p = rq.pos0 + t2;
+                    const int t2 = tok_of(nt * 8 + 2 * c + i), p = rq.pos0 + t2;
                     vhi[nt][i] = t2 < rq.n ? min(p + 1, rq.hi) : 0;
                     vlo[nt][i] = a.window ? max(0, p - a.window + 1) : 0;
                 }
             }
             // keys that every row of the tile sees: no masks there
-            const int last = min(rq.n - 1, (row0 + NR - 1) / group), firstt = row0 / group;
+            const int last = min(rq.n - 1, tok_of(NR - 1)), firstt = tok0;
             const int all_hi = min(rq.pos0 + firstt + 1, rq.hi);
             const int all_lo = a.window ? max(0, rq.pos0 + last - a.window + 1) : 0;
             const int any_lo = a.window ? max(0, rq.pos0 + firstt - a.window + 1) : 0;
@@ -507,9 +533,9 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 for (int nt = 0; nt < QT; nt++)
 #pragma unroll
                     for (int q = 0; q < 2; q++) {
-                        const int row = row0 + nt * 8 + 2 * c + q, tok = row / group;
+                        const int tok = tok_of(nt * 8 + 2 * c + q);
                         if (tok >= rq.n) continue;
-                        const int h = kh * group + row % group;
+                        const int h = kh * group + row0 + nt * 8 + 2 * c + q - tok * group;
                         const float inv = l[nt][q] > 0.0f ? 1.0f / l[nt][q] : (l[nt][q] == 0.0f ? 0.0f : l[nt][q]);
                         T* op = reinterpret_cast<T*>(a.out.p) + (int64_t)(rq.q0 + tok) * a.out.st + h * a.out.sh;
 #pragma unroll
@@ -534,12 +560,14 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
 #pragma unroll
                     for (int q = 0; q < 2; q++) {
                         const int row = nt * 8 + 2 * c + q;
-                        if (g == 0) pc[row] = m[nt][q], pc[NR + row] = l[nt][q];
-                        float* po = pc + 2 * NR + row * D;
+                        if (g == 0) pc[NR * M::ROW + row] = m[nt][q], pc[NR * (M::ROW + 1) + row] = l[nt][q];
 #pragma unroll
                         for (int x = 0; x < BX; x++)
 #pragma unroll
-                            for (int e = 0; e < VB; e++) po[x * 128 + vg * VB + e] = o[nt][x * 8 + e / 2][(e & 1) * 2 + q];
+                            for (int e = 0; e < VB; e += 4)
+                                *reinterpret_cast<float4*>(pc + row * M::ROW + x * 128 + vg * VB + e) =
+                                    make_float4(o[nt][x * 8 + e / 2][q], o[nt][x * 8 + e / 2][2 + q], o[nt][x * 8 + e / 2 + 1][q],
+                                                o[nt][x * 8 + e / 2 + 1][2 + q]);
                     }
                 if (lane == 0)
                     s_piece[2 * w + (into_first ? 0 : 1)] =
@@ -578,86 +606,120 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
 
     // ---- joining ----
     __syncthreads();
-    auto piece_ptr = [&](int i) {
-        return (i & 1) ? reinterpret_cast<const float*>(ring_ptr + (i >> 1) * DEPTH * S::STAGE)
-                       : reinterpret_cast<const float*>(ring_ptr + M::RING) + (i >> 1) * M::PIECE;
+    auto piece = [&](int i) {
+        return (i & 1) ? reinterpret_cast<float*>(ring_ptr + (i >> 1) * DEPTH * S::STAGE)
+                       : reinterpret_cast<float*>(ring_ptr + M::RING) + (i >> 1) * M::PIECE;
     };
-    // (M, l, o) of element (row, d) over n pieces at get(i)
-    auto join = [&](int n, auto get, int row, int d, float& mm, float& ll, float& oo) {
-        mm = -INFINITY;
-        for (int i = 0; i < n; i++) mm = fmaxf(mm, __ldcg(get(i) + row));
-        const float mu = mm == -INFINITY ? 0.0f : mm;
-        ll = oo = 0.0f;
-        for (int i = 0; i < n; i++) {
-            const float* p = get(i);
-            const float f = ex2(__ldcg(p + row) - mu);
-            ll = fmaf(__ldcg(p + NR + row), f, ll);
-            oo = fmaf(__ldcg(p + 2 * NR + row * D + d), f, oo);
-        }
-    };
-    auto emit = [&](const SplitPiece& pc, int row, int d, float mm, float ll, float oo) {
-        const int rr = pc.row0 + row, tok = rr / group;
+    constexpr int E4 = NR * D / 4;  // a thread joins four neighbouring elements
+    auto emit = [&](const SplitPiece& pc, int e, float4 o) {
+        const int row = e / (D / 4), d = e % (D / 4) * 4, rr = pc.row0 + row, tok = rr / group;
         if (tok >= pc.n) return;
-        const int h = pc.head * group + rr % group;
-        reinterpret_cast<T*>(a.out.p)[(int64_t)(pc.q0 + tok) * a.out.st + (int64_t)h * a.out.sh + d] =
-            Elt<T>::put(ll > 0.0f ? oo / ll : (ll == 0.0f ? 0.0f : ll));
+        const int h = pc.head * group + rr - tok * group;
+        const float l = s_l[row], inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+        T* op = reinterpret_cast<T*>(a.out.p) + (int64_t)(pc.q0 + tok) * a.out.st + (int64_t)h * a.out.sh + d;
+        T y[4] = {Elt<T>::put(o.x * inv), Elt<T>::put(o.y * inv), Elt<T>::put(o.z * inv), Elt<T>::put(o.w * inv)};
+        if (a.out.vec) {
+            if (sizeof(T) == 4) *reinterpret_cast<uint4*>(op) = *reinterpret_cast<const uint4*>(y);
+            else *reinterpret_cast<uint2*>(op) = *reinterpret_cast<const uint2*>(y);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) op[i] = y[i];
+        }
         if (d == 0 && a.lse)
-            a.lse[(int64_t)(pc.q0 + tok) * a.q.heads + h] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * LN2;
+            a.lse[(int64_t)(pc.q0 + tok) * a.q.heads + h] = l == 0.0f ? -INFINITY : (s_m[row] + log2f(l)) * LN2;
     };
     for (int i = 0; i < 2 * NW;) {
-        if (!(s_piece[i].flags & 1)) { i++; continue; }
+        if (!(s_piece[i].flags & 1)) {
+            i++;
+            continue;
+        }
         const SplitPiece pc = s_piece[i];
-        int idx[2 * NW], n = 0, k = i;
         int flags = 0;
-        for (; k < 2 * NW; k++) {
-            if (!(s_piece[k].flags & 1)) continue;
-            if (s_piece[k].a != pc.a) break;
-            idx[n++] = k;
-            flags |= s_piece[k].flags;
+        unsigned set = 0;  // the slots that hold pieces of this item
+        for (; i < 2 * NW; i++) {
+            if (!(s_piece[i].flags & 1)) continue;
+            if (s_piece[i].a != pc.a) break;
+            set |= 1u << i;
+            flags |= s_piece[i].flags;
         }
-        i = k;
         const bool whole = (flags & 6) == 6;
-        float* slot = ws.part + (size_t)(2 * blockIdx.x + ((flags & 2) ? 1 : 0)) * M::PIECE;
-        for (int e = tid; e < NR * D; e += NT) {
-            const int row = e / D, d = e % D;
-            float mm = -INFINITY, ll = 0.0f, oo = 0.0f;
-            for (int x = 0; x < n; x++) mm = fmaxf(mm, piece_ptr(idx[x])[row]);
+        if (tid < NR) {
+            float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 2 * NW; k++)
+                if (set >> k & 1) mm = fmaxf(mm, piece(k)[NR * M::ROW + tid]);
             const float mu = mm == -INFINITY ? 0.0f : mm;
-            for (int x = 0; x < n; x++) {
-                const float* p = piece_ptr(idx[x]);
-                const float f = ex2(p[row] - mu);
-                ll = fmaf(p[NR + row], f, ll);
-                oo = fmaf(p[2 * NR + row * D + d], f, oo);
-            }
-            if (whole) {
-                emit(pc, row, d, mm, ll, oo);
-            } else {
-                if (d == 0) slot[row] = mm, slot[NR + row] = ll;
-                slot[2 * NR + row * D + d] = oo;
-            }
+#pragma unroll
+            for (int k = 0; k < 2 * NW; k++)
+                if (set >> k & 1) {
+                    const float f = ex2(piece(k)[NR * M::ROW + tid] - mu);
+                    s_f[k][tid] = f;
+                    ll = fmaf(piece(k)[NR * (M::ROW + 1) + tid], f, ll);
+                }
+            s_m[tid] = mm;
+            s_l[tid] = ll;
         }
-        if (whole) continue;
-        // the CTAs that hold the item's first and last unit
-        auto cta_of = [&](int64_t u) {
-            const int64_t big = extra * (each + 1);
-            return (int)(u < big ? quot(u, each + 1) : extra + quot(u - big, each));
-        };
-        const int c0 = cta_of(pc.a), c1 = cta_of(pc.a + pc.tiles - 1);
-        __threadfence();
         __syncthreads();
-        if (tid == 0) s_last = atomicAdd(ws.ticket + c0, 1u) == (unsigned)(c1 - c0);
-        __syncthreads();
-        if (s_last) {
+        float* slot = ws.part + (size_t)(2 * blockIdx.x + ((flags & 2) ? 1 : 0)) * M::PIECE;
+        for (int e = tid; e < E4; e += NT) {
+            const int row = e / (D / 4), at = row * M::ROW + e % (D / 4) * 4;
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int k = 0; k < 2 * NW; k++)
+                if (set >> k & 1) {
+                    const float4 v = *reinterpret_cast<const float4*>(piece(k) + at);
+                    const float f = s_f[k][row];
+                    o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
+                }
+            if (whole) emit(pc, e, o);
+            else __stcg(reinterpret_cast<float4*>(slot + at), o);
+        }
+        if (!whole) {
+            if (tid < NR) __stcg(slot + NR * M::ROW + tid, s_m[tid]), __stcg(slot + NR * (M::ROW + 1) + tid, s_l[tid]);
+            // the CTAs that hold the item's first and last unit
+            auto cta_of = [&](int64_t u) {
+                const int64_t big = extra * (each + 1);
+                return (int)(u < big ? quot(u, each + 1) : extra + quot(u - big, each));
+            };
+            const int c0 = cta_of(pc.a), n = cta_of(pc.a + pc.tiles - 1) - c0 + 1;
             __threadfence();
-            auto get = [&](int x) { return ws.part + (size_t)(2 * (c0 + x) + (x == 0 ? 1 : 0)) * M::PIECE; };
-            for (int e = tid; e < NR * D; e += NT) {
-                float mm, ll, oo;
-                join(c1 - c0 + 1, get, e / D, e % D, mm, ll, oo);
-                emit(pc, e / D, e % D, mm, ll, oo);
+            __syncthreads();
+            if (tid == 0) s_last = atomicAdd(ws.ticket + c0, 1u) == (unsigned)(n - 1);
+            __syncthreads();
+            if (s_last) {
+                __threadfence();
+                auto part = [&](int k) { return ws.part + (size_t)(2 * (c0 + k) + (k == 0 ? 1 : 0)) * M::PIECE; };
+                for (int row = w; row < NR; row += NW) {  // a warp per row, lanes over the CTAs
+                    float mm = -INFINITY, ll = 0.0f;
+                    for (int k = lane; k < n; k += 32) mm = fmaxf(mm, __ldcg(part(k) + NR * M::ROW + row));
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+                    const float mu = mm == -INFINITY ? 0.0f : mm;
+                    for (int k = lane; k < n; k += 32) {
+                        const float f = ex2(__ldcg(part(k) + NR * M::ROW + row) - mu);
+                        s_f[k][row] = f;
+                        ll = fmaf(__ldcg(part(k) + NR * (M::ROW + 1) + row), f, ll);
+                    }
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
+                    if (lane == 0) s_m[row] = mm, s_l[row] = ll;
+                }
+                __syncthreads();
+                for (int e = tid; e < E4; e += NT) {
+                    const int row = e / (D / 4), at = row * M::ROW + e % (D / 4) * 4;
+                    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+                    for (int k = 0; k < n; k++) {
+                        const float4 v = __ldcg(reinterpret_cast<const float4*>(part(k) + at));
+                        const float f = s_f[k][row];
+                        o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
+                    }
+                    emit(pc, e, o);
+                }
+                if (tid == 0) ws.ticket[c0] = 0;
             }
-            if (tid == 0) ws.ticket[c0] = 0;
         }
-        __syncthreads();
+        __syncthreads();  // s_f, s_m and s_l are used again
     }
 }
 
@@ -669,7 +731,7 @@ static cudaError_t split_launch(const KvMaps& maps, const KvArg& kv, const Atten
     static std::atomic<uint64_t> done{0};
     cudaError_t e = allow_smem(k, smem, done);
     if (e != cudaSuccess) return e;
-    return launch_pdl(k, dim3(sms), dim3(SPLIT_NW * 32), smem, s, maps.k, maps.v, kv, a, ws);
+    return launch_pdl(k, dim3(std::min(sms, SPLIT_MAX_SMS)), dim3(SPLIT_NW * 32), smem, s, maps.k, maps.v, kv, a, ws);
 }
 
 // nr: 8 or 16 rows per item (16 only up to head_dim 128: the accumulators of 256 would spill)
@@ -684,7 +746,7 @@ static cudaError_t split_dims(const KvMaps& maps, const KvArg& kv, const AttendA
 }
 
 int split_tile_tokens(int dim) { return dim == 256 ? SplitShape<256>::TW : SplitShape<128>::TW; }
-size_t split_part_bytes(int dim) { return (size_t)(dim == 256 ? 8 : 16) * (dim + 2) * 4 * 2; }
+size_t split_part_bytes(int dim) { return (size_t)(dim == 256 ? 8 : 16) * (dim + 4 + 2) * 4 * 2; }
 
 cudaError_t launch_split(const KvMaps& maps, const KvArg& kv, const AttendArg& a, const SplitWs& ws, int sms, int nr,
                          uint32_t type, int code, cudaStream_t s) {
