@@ -115,13 +115,14 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     constexpr int NW = SPLIT_NW, NT = NW * 32, DEPTH = SPLIT_DEPTH, TW = S::TW, MT = S::MT, KS = S::KS, HF = S::HF;
     constexpr int QT = NR / 8;                 // n-tiles of 8 rows
     constexpr bool PAIR = sizeof(T) == 4;      // f32: hi + lo
+    constexpr bool PRE = !PAIR && NR * D <= 1024;  // q is asked for ahead where registers allow
     constexpr int VB = D == 64 ? 8 : 16;       // V bytes per lane, token and 128-byte box
     constexpr int BX = D == 256 ? 2 : 1;       // 128-byte boxes per row
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t s_full[NW][DEPTH];
     __shared__ __align__(8) float s_scale[NW][DEPTH][2][2];  // per box of the tile: K scale (-1: no such block), V scale
     __shared__ SplitStart s_start[NW];
-    __shared__ float s_f[SPLIT_MAX_SMS][NR], s_m[NR], s_l[NR];  // joining: factors of the pieces, the joined M and l
+    __shared__ int64_t s_first[NW];
     __shared__ int64_t s_tot[NW];
     __shared__ SplitPiece s_piece[2 * NW];
     __shared__ int s_last;
@@ -164,45 +165,82 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         W += s_tot[i];
     }
     // a share of less than a tile per warp would only add joining
-    const int64_t active = min((int64_t)gridDim.x, (W + NW - 1) / NW);
-    const int64_t each = active ? quot(W, active) : 0, extra = W - each * active;  // the first `extra` CTAs take one more
-    auto share = [&](int64_t cta) { return each * cta + min(cta, extra); };
-    const int64_t u0 = share(blockIdx.x), u1 = blockIdx.x < active ? share(blockIdx.x + 1) : u0;
-    auto warp_unit = [&](int i) { return u0 + (u1 - u0) * i / NW; };
-    const int64_t wu0 = warp_unit(w), wu1 = warp_unit(w + 1);
+    const int active = (int)min((int64_t)gridDim.x, (W + NW - 1) / NW);
+    const int64_t each = active ? quot(W, active) : 0;
+    const int extra = (int)(W - each * active);  // the first `extra` CTAs take one unit more
+    const int bx = blockIdx.x;
+    const int64_t u0 = each * bx + min(bx, extra);
+    const int64_t cnt_u = bx < active ? each + (bx < extra) : 0;
+    const int64_t wbase = u0 + cnt_u / NW * w + min(w, (int)(cnt_u % NW)), wlen = cnt_u / NW + (w < cnt_u % NW);
     // the thread that holds a warp's first unit tells it where that is
+    if (lane == 0) s_first[w] = wlen > 0 ? wbase : -1;
+    __syncthreads();
     {
         const int64_t at = before + incl - mine;
-#pragma unroll
-        for (int i = 0; i < NW; i++) {
-            const int64_t u = warp_unit(i);
-            if (u >= at && u < at + mine) {
-                int64_t rem = u - at;
-                int r = tid * per;
-                SplitReq q = rq;
-                if (per > 1) {
-                    q = split_req(a, r, heads, group, bs, NR, TW, max_rows);
-                    while (rem >= (int64_t)q.items * q.tiles) {
-                        rem -= (int64_t)q.items * q.tiles;
-                        q = split_req(a, ++r, heads, group, bs, NR, TW, max_rows);
+        if (at + mine > u0 && at < u0 + cnt_u)
+#pragma unroll 1
+            for (int i = 0; i < NW; i++) {
+                const int64_t u = s_first[i];
+                if (u >= at && u < at + mine) {
+                    int64_t rem = u - at;
+                    int r = tid * per;
+                    SplitReq q = rq;
+                    if (per > 1) {
+                        q = split_req(a, r, heads, group, bs, NR, TW, max_rows);
+                        while (rem >= (int64_t)q.items * q.tiles) {
+                            rem -= (int64_t)q.items * q.tiles;
+                            q = split_req(a, ++r, heads, group, bs, NR, TW, max_rows);
+                        }
                     }
+                    s_start[i] = SplitStart{q, r, rem};
                 }
-                s_start[i] = SplitStart{q, r, rem};
             }
-        }
     }
     __syncthreads();
 
-    if (wu0 < wu1) {
+    if (wlen > 0) {
         rq = s_start[w].rq;
         int r = s_start[w].r;
         const int64_t rem = s_start[w].rem;
         int item = (int)quot(rem, rq.tiles), tile = (int)(rem - (int64_t)item * rq.tiles);
 
+        // the rows of the current item, and its q
+        int kh, row0, tok0, rem0;
+        uint4 qraw[QT][HF][sizeof(T)];
+        // row row0 + i is token tok0 + (rem0 + i) / group, head (rem0 + i) % group of the group
+        auto tok_of = [&](int i) { return tok0 + (group == 1 ? i : (int)__umulhi((uint32_t)(rem0 + i), a.group_inv)); };
+        auto next_rows = [&]() {
+            kh = item % heads;
+            row0 = item / heads * NR;
+            tok0 = row0 / group;
+            rem0 = row0 - tok0 * group;
+#pragma unroll
+            for (int nt = 0; nt < QT; nt++) {
+                const int tok = tok_of(nt * 8 + g), gh = row0 + nt * 8 + g - tok * group;
+                const T* qp = reinterpret_cast<const T*>(a.q.p) + (int64_t)(rq.q0 + (tok < rq.n ? tok : 0)) * a.q.st +
+                              (int64_t)(kh * group + gh) * a.q.sh;
+#pragma unroll
+                for (int hf = 0; hf < HF; hf++) {
+                    const T* x = qp + (hf * 4 + c) * 16;
+                    if (a.q.vec) {
+#pragma unroll
+                        for (int i = 0; i < (int)sizeof(T); i++) qraw[nt][hf][i] = *(reinterpret_cast<const uint4*>(x) + i);
+                    } else {
+                        T y[16];
+#pragma unroll
+                        for (int i = 0; i < 16; i++) y[i] = x[i];
+#pragma unroll
+                        for (int i = 0; i < (int)sizeof(T); i++) qraw[nt][hf][i] = *(reinterpret_cast<const uint4*>(y) + i);
+                    }
+                }
+            }
+        };
+        if (PRE) next_rows();
+
         // ---- the issuing side: runs DEPTH tiles ahead ----
         SplitReq pq = rq;
         int pr = r, pitem = item, ptile = tile;
-        int64_t pleft = wu1 - wu0;
+        int64_t pleft = wlen;
         int pblk = -1;
         auto lookup = [&]() {  // lane b < nb: the block of box b of the tile to issue next
             const int j = (pq.t0 + ptile) * TW + lane * br;
@@ -255,33 +293,28 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         const int tg = D == 64 ? g : (g >> 1) + 4 * (g & 1);
         const int t2c = D == 64 ? 2 * c : c, t2c1 = D == 64 ? 2 * c + 1 : c + 4;  // rows 2c and 2c + 1
         const int vg = (g >> 1) + 4 * (g & 1);
-        int64_t left = wu1 - wu0;
+        int64_t left = wlen;
         uint32_t cnt = 0;
         bool dead = false, firstseg = true;
         while (left > 0 && !dead) {
             const int seg = (int)min(left, (int64_t)(rq.tiles - tile));
-            const int kh = item % heads, row0 = item / heads * NR;
-            // row row0 + i is token tok0 + (rem0 + i) / group, head (rem0 + i) % group of the group
-            const int tok0 = row0 / group, rem0 = row0 - tok0 * group;
-            auto tok_of = [&](int i) { return tok0 + (group == 1 ? i : (int)__umulhi((uint32_t)(rem0 + i), a.group_inv)); };
+            if (!PRE) next_rows();
             // q rows as B operands, scaled to the fp16 range row by row
             uint32_t qh[QT][KS][2], ql[PAIR ? QT : 1][PAIR ? KS : 1][2];
             float qs[QT][2];
             int vhi[QT][2], vlo[QT][2];
 #pragma unroll
             for (int nt = 0; nt < QT; nt++) {
-                const int tok = tok_of(nt * 8 + g), gh = row0 + nt * 8 + g - tok * group;
-                const bool live = tok < rq.n;
-                const T* qp = reinterpret_cast<const T*>(a.q.p) + (int64_t)(rq.q0 + (live ? tok : 0)) * a.q.st +
-                              (int64_t)(kh * group + gh) * a.q.sh;
+                const bool live = tok_of(nt * 8 + g) < rq.n;
                 float v[HF][16], mx = 0.0f;
 #pragma unroll
                 for (int hf = 0; hf < HF; hf++) {
-                    load8(qp + (hf * 4 + c) * 16, a.q.vec, v[hf]);
-                    load8(qp + (hf * 4 + c) * 16 + 8, a.q.vec, v[hf] + 8);
+                    T y[16];
+#pragma unroll
+                    for (int i = 0; i < (int)sizeof(T); i++) *(reinterpret_cast<uint4*>(y) + i) = qraw[nt][hf][i];
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
-                        if (!live) v[hf][e] = 0.0f;
+                        v[hf][e] = live ? Elt<T>::get(y[e]) : 0.0f;
                         mx = fmaxf(mx, fabsf(v[hf][e]));
                     }
                 }
@@ -571,7 +604,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     }
                 if (lane == 0)
                     s_piece[2 * w + (into_first ? 0 : 1)] =
-                        SplitPiece{wu1 - left - tile, rq.tiles, rq.q0, rq.n, row0, kh, 1 | (starts ? 2 : 0) | (ends ? 4 : 0)};
+                        SplitPiece{wbase + wlen - left - tile, rq.tiles, rq.q0, rq.n, row0, kh, 1 | (starts ? 2 : 0) | (ends ? 4 : 0)};
             }
             firstseg = false;
             left -= seg;
@@ -583,11 +616,12 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     do rq = split_req(a, ++r, heads, group, bs, NR, TW, max_rows);
                     while (rq.items == 0);
                 }
+                if (PRE) next_rows();
             }
         }
         if (dead) {  // a copy did not arrive: say so, and let what is in flight land
             if (lane == 0) atomicOr(kv.status, (unsigned)DERR_TIMEOUT);
-            for (int64_t k = (wu1 - wu0) - pleft; (int64_t)cnt < k; cnt++)
+            for (int64_t k = wlen - pleft; (int64_t)cnt < k; cnt++)
                 tc::mbar_wait_tries(smem_u32(&s_full[w][cnt % DEPTH]), (cnt / DEPTH) & 1);
         }
     }
@@ -596,7 +630,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     {
         const int first = min(max(__ldg(a.cu), 0), a.T), end = min(max(__ldg(a.cu + a.R), first), a.T);
         const int64_t rest = (int64_t)(a.T - (end - first)) * a.q.heads;
-        for (int64_t i = (int64_t)blockIdx.x * NW + w; i < rest; i += (int64_t)gridDim.x * NW) {
+        for (int64_t i = (int64_t)bx * NW + w; i < rest; i += (int64_t)gridDim.x * NW) {
             const int k = (int)(i / a.q.heads), h = (int)(i % a.q.heads), t = k < first ? k : end + (k - first);
             T* o = reinterpret_cast<T*>(a.out.p) + t * a.out.st + h * a.out.sh;
             for (int d = lane; d < D; d += 32) o[d] = Elt<T>::put(0.0f);
@@ -610,116 +644,124 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         return (i & 1) ? reinterpret_cast<float*>(ring_ptr + (i >> 1) * DEPTH * S::STAGE)
                        : reinterpret_cast<float*>(ring_ptr + M::RING) + (i >> 1) * M::PIECE;
     };
-    constexpr int E4 = NR * D / 4;  // a thread joins four neighbouring elements
-    auto emit = [&](const SplitPiece& pc, int e, float4 o) {
-        const int row = e / (D / 4), d = e % (D / 4) * 4, rr = pc.row0 + row, tok = rr / group;
+    // A warp joins a row: lanes hold the pieces' M and l first, then D / 32 neighbouring elements each.
+    constexpr int VE = D / 32;
+    auto emit = [&](const SplitPiece& pc, int row, float m, float l, const float* o) {
+        const int rr = pc.row0 + row, tok = rr / group;
         if (tok >= pc.n) return;
         const int h = pc.head * group + rr - tok * group;
-        const float l = s_l[row], inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-        T* op = reinterpret_cast<T*>(a.out.p) + (int64_t)(pc.q0 + tok) * a.out.st + (int64_t)h * a.out.sh + d;
-        T y[4] = {Elt<T>::put(o.x * inv), Elt<T>::put(o.y * inv), Elt<T>::put(o.z * inv), Elt<T>::put(o.w * inv)};
+        const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+        T* op = reinterpret_cast<T*>(a.out.p) + (int64_t)(pc.q0 + tok) * a.out.st + (int64_t)h * a.out.sh + lane * VE;
+        T y[VE];
+#pragma unroll
+        for (int i = 0; i < VE; i++) y[i] = Elt<T>::put(o[i] * inv);
         if (a.out.vec) {
-            if (sizeof(T) == 4) *reinterpret_cast<uint4*>(op) = *reinterpret_cast<const uint4*>(y);
-            else *reinterpret_cast<uint2*>(op) = *reinterpret_cast<const uint2*>(y);
+            constexpr int B = VE * (int)sizeof(T);  // 4 to 32 bytes
+#pragma unroll
+            for (int i = 0; i < (B + 15) / 16; i++)
+                if (B >= 16) *(reinterpret_cast<uint4*>(op) + i) = *(reinterpret_cast<const uint4*>(y) + i);
+                else if (B == 8) *reinterpret_cast<uint2*>(op) = *reinterpret_cast<const uint2*>(y);
+                else *reinterpret_cast<uint32_t*>(op) = *reinterpret_cast<const uint32_t*>(y);
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; i++) op[i] = y[i];
+            for (int i = 0; i < VE; i++) op[i] = y[i];
         }
-        if (d == 0 && a.lse)
-            a.lse[(int64_t)(pc.q0 + tok) * a.q.heads + h] = l == 0.0f ? -INFINITY : (s_m[row] + log2f(l)) * LN2;
+        if (lane == 0 && a.lse)
+            a.lse[(int64_t)(pc.q0 + tok) * a.q.heads + h] = l == 0.0f ? -INFINITY : (m + lg2(l)) * LN2;
     };
-    for (int i = 0; i < 2 * NW;) {
-        if (!(s_piece[i].flags & 1)) {
-            i++;
-            continue;
-        }
-        const SplitPiece pc = s_piece[i];
-        int flags = 0;
-        unsigned set = 0;  // the slots that hold pieces of this item
-        for (; i < 2 * NW; i++) {
-            if (!(s_piece[i].flags & 1)) continue;
-            if (s_piece[i].a != pc.a) break;
-            set |= 1u << i;
-            flags |= s_piece[i].flags;
-        }
+    auto vec = [&](const float* p, float* v) {  // VE floats
+        if (VE == 2) *reinterpret_cast<float2*>(v) = __ldcg(reinterpret_cast<const float2*>(p));
+        else
+#pragma unroll
+            for (int i = 0; i < VE / 4; i++) *(reinterpret_cast<float4*>(v) + i) = __ldcg(reinterpret_cast<const float4*>(p) + i);
+    };
+    auto wmax = [&](float x) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+        return x;
+    };
+    auto wsum = [&](float x) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        return x;
+    };
+    const unsigned valid = __ballot_sync(0xffffffffu, lane < 2 * NW && (s_piece[lane & (2 * NW - 1)].flags & 1));
+    for (unsigned todo = valid; todo;) {
+        const SplitPiece& pc = s_piece[__ffs(todo) - 1];
+        // the slots that hold pieces of this item
+        const SplitPiece& mp = s_piece[lane & (2 * NW - 1)];
+        const unsigned set = __ballot_sync(0xffffffffu, (todo >> lane & 1) && mp.a == pc.a);
+        const bool in = set >> lane & 1;
+        const int flags = __reduce_or_sync(0xffffffffu, in ? mp.flags : 0);
+        todo &= ~set;
         const bool whole = (flags & 6) == 6;
-        if (tid < NR) {
-            float mm = -INFINITY, ll = 0.0f;
+        float* slot = ws.part + (size_t)(2 * bx + ((flags & 2) ? 1 : 0)) * M::PIECE;
+#pragma unroll 1
+        for (int row = w; row < NR; row += NW) {
+            const float* mine_p = in ? piece(lane) : piece(0);
+            const float pm = in ? mine_p[NR * M::ROW + row] : -INFINITY, mm = wmax(pm), mu = mm == -INFINITY ? 0.0f : mm;
+            const float f = ex2(pm - mu), ll = wsum(in ? mine_p[NR * (M::ROW + 1) + row] * f : 0.0f);
+            float o[VE];
 #pragma unroll
-            for (int k = 0; k < 2 * NW; k++)
-                if (set >> k & 1) mm = fmaxf(mm, piece(k)[NR * M::ROW + tid]);
-            const float mu = mm == -INFINITY ? 0.0f : mm;
+            for (int i = 0; i < VE; i++) o[i] = 0.0f;
+            for (unsigned rest = set; rest; rest &= rest - 1) {
+                const int k = __ffs(rest) - 1;
+                const float fk = __shfl_sync(0xffffffffu, f, k);
+                const float* p = piece(k) + row * M::ROW + lane * VE;
 #pragma unroll
-            for (int k = 0; k < 2 * NW; k++)
-                if (set >> k & 1) {
-                    const float f = ex2(piece(k)[NR * M::ROW + tid] - mu);
-                    s_f[k][tid] = f;
-                    ll = fmaf(piece(k)[NR * (M::ROW + 1) + tid], f, ll);
-                }
-            s_m[tid] = mm;
-            s_l[tid] = ll;
-        }
-        __syncthreads();
-        float* slot = ws.part + (size_t)(2 * blockIdx.x + ((flags & 2) ? 1 : 0)) * M::PIECE;
-        for (int e = tid; e < E4; e += NT) {
-            const int row = e / (D / 4), at = row * M::ROW + e % (D / 4) * 4;
-            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int i = 0; i < VE; i++) o[i] = fmaf(p[i], fk, o[i]);
+            }
+            if (whole) {
+                emit(pc, row, mm, ll, o);
+            } else {
 #pragma unroll
-            for (int k = 0; k < 2 * NW; k++)
-                if (set >> k & 1) {
-                    const float4 v = *reinterpret_cast<const float4*>(piece(k) + at);
-                    const float f = s_f[k][row];
-                    o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
-                }
-            if (whole) emit(pc, e, o);
-            else __stcg(reinterpret_cast<float4*>(slot + at), o);
-        }
-        if (!whole) {
-            if (tid < NR) __stcg(slot + NR * M::ROW + tid, s_m[tid]), __stcg(slot + NR * (M::ROW + 1) + tid, s_l[tid]);
-            // the CTAs that hold the item's first and last unit
-            auto cta_of = [&](int64_t u) {
-                const int64_t big = extra * (each + 1);
-                return (int)(u < big ? quot(u, each + 1) : extra + quot(u - big, each));
-            };
-            const int c0 = cta_of(pc.a), n = cta_of(pc.a + pc.tiles - 1) - c0 + 1;
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) s_last = atomicAdd(ws.ticket + c0, 1u) == (unsigned)(n - 1);
-            __syncthreads();
-            if (s_last) {
-                __threadfence();
-                auto part = [&](int k) { return ws.part + (size_t)(2 * (c0 + k) + (k == 0 ? 1 : 0)) * M::PIECE; };
-                for (int row = w; row < NR; row += NW) {  // a warp per row, lanes over the CTAs
-                    float mm = -INFINITY, ll = 0.0f;
-                    for (int k = lane; k < n; k += 32) mm = fmaxf(mm, __ldcg(part(k) + NR * M::ROW + row));
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-                    const float mu = mm == -INFINITY ? 0.0f : mm;
-                    for (int k = lane; k < n; k += 32) {
-                        const float f = ex2(__ldcg(part(k) + NR * M::ROW + row) - mu);
-                        s_f[k][row] = f;
-                        ll = fmaf(__ldcg(part(k) + NR * (M::ROW + 1) + row), f, ll);
-                    }
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
-                    if (lane == 0) s_m[row] = mm, s_l[row] = ll;
-                }
-                __syncthreads();
-                for (int e = tid; e < E4; e += NT) {
-                    const int row = e / (D / 4), at = row * M::ROW + e % (D / 4) * 4;
-                    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-                    for (int k = 0; k < n; k++) {
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(part(k) + at));
-                        const float f = s_f[k][row];
-                        o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
-                    }
-                    emit(pc, e, o);
-                }
-                if (tid == 0) ws.ticket[c0] = 0;
+                for (int i = 0; i < VE; i += 2) __stcg(reinterpret_cast<float2*>(slot + row * M::ROW + lane * VE + i), make_float2(o[i], o[i + 1]));
+                if (lane == 0) __stcg(slot + NR * M::ROW + row, mm), __stcg(slot + NR * (M::ROW + 1) + row, ll);
             }
         }
-        __syncthreads();  // s_f, s_m and s_l are used again
+        if (whole) continue;
+        // the CTAs that hold the item's first and last unit
+        auto cta_of = [&](int64_t u) {
+            const int64_t big = extra * (each + 1);
+            return (int)(u < big ? quot(u, each + 1) : extra + quot(u - big, each));
+        };
+        const int c0 = cta_of(pc.a), n = cta_of(pc.a + pc.tiles - 1) - c0 + 1;
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) s_last = atomicAdd(ws.ticket + c0, 1u) == (unsigned)(n - 1);
+        __syncthreads();
+        if (s_last) {
+            __threadfence();
+            auto part = [&](int k) { return ws.part + (size_t)(2 * (c0 + k) + (k == 0 ? 1 : 0)) * M::PIECE; };
+#pragma unroll 1
+            for (int row = w; row < NR; row += NW) {
+                float mm = -INFINITY;
+                for (int k = lane; k < n; k += 32) mm = fmaxf(mm, __ldcg(part(k) + NR * M::ROW + row));
+                mm = wmax(mm);
+                const float mu = mm == -INFINITY ? 0.0f : mm;
+                float o[VE], ll = 0.0f;
+#pragma unroll
+                for (int i = 0; i < VE; i++) o[i] = 0.0f;
+                for (int k0 = 0; k0 < n; k0 += 32) {
+                    const int k1 = min(32, n - k0);
+                    const float* mine_p = part(k0 + min(lane, k1 - 1));
+                    const float f = lane < k1 ? ex2(__ldcg(mine_p + NR * M::ROW + row) - mu) : 0.0f;
+                    ll = fmaf(__ldcg(mine_p + NR * (M::ROW + 1) + row), f, ll);
+#pragma unroll 4
+                    for (int k = 0; k < k1; k++) {
+                        float v[VE];
+                        vec(part(k0 + k) + row * M::ROW + lane * VE, v);
+                        const float fk = __shfl_sync(0xffffffffu, f, k);
+#pragma unroll
+                        for (int i = 0; i < VE; i++) o[i] = fmaf(v[i], fk, o[i]);
+                    }
+                }
+                ll = wsum(ll);
+                emit(pc, row, mm, ll, o);
+            }
+            if (tid == 0) ws.ticket[c0] = 0;
+        }
+        __syncthreads();  // s_last is used again
     }
 }
 
