@@ -1,40 +1,38 @@
 // kv_append.cu -- writing new keys and values into the 8-bit paged cache, and reading them back.
+#include <algorithm>
+
 #include "kv_code.cuh"
 #include "rope.cuh"
 
 namespace rmoe {
 
 struct AppendArg {
-    Rows k, v;
+    Rows k, v, q, qo;
     const int32_t* slots;
     RopeArg rope;
     int T;
+    int window;   // tokens of a CTA's window
+    int kv_ctas;  // the CTAs from here on turn q
 };
 
-// One CTA per (token, head, K or V); the CTA of a run's first token writes the whole run, the
-// others return.  Two passes over the run's elements: the largest magnitude, then the codes.
-template <typename T, int CODE>
-__global__ void __launch_bounds__(128) kv_append_kernel(KvArg kv, AppendArg a) {
-    const int t0 = blockIdx.x, h = blockIdx.y, isv = blockIdx.z, tid = threadIdx.x;
-    const int bs = kv.bs, dim = kv.dim;
-    pdl_trigger();
-    pdl_wait();
-    const int slot = __ldg(a.slots + t0);
-    if (slot < 0) return;
-    const int first = slot & (bs - 1), block = slot / bs;
-    if (block >= kv.n_blocks) {
-        if (tid == 0 && h == 0) atomicOr(kv.status, (unsigned)DERR_INDEX);
-        return;
-    }
-    if (first != 0 && t0 > 0 && __ldg(a.slots + t0 - 1) == slot - 1) return;  // inside a run
-    int n = 1;
-    while (first + n < bs && t0 + n < a.T && __ldg(a.slots + t0 + n) == slot + n) n++;
+// A run is the tokens of one call that go to consecutive slots of one block: they share a scale.
+// A CTA looks at `window` tokens for one head of K or V and writes the runs that begin there: all
+// threads together where few begin (prompts), a warp per run where many do (decoded tokens).
+// A run is bound by reading its elements once; up to HOLD units of 16 stay in registers between the
+// pass that finds the largest magnitude and the pass that rounds, the rest is read again (L2).
+static constexpr int APT = 256, HOLD = 2;
 
+// Writes the run of n tokens from t0 on, at slot; thread i of NT.  red: a word per warp (NT > 32).
+template <typename T, int CODE, int NT>
+__device__ __forceinline__ void write_run(const KvArg& kv, const AppendArg& a, bool isv, int h, int t0, int n, int slot, int tid,
+                                          float* red) {
+    const int bs = kv.bs, dim = kv.dim, units = dim >> 4, lu = 31 - __clz(units);  // dim is a power of two
+    const int first = slot & (bs - 1), block = slot >> kv.shift;
     const Rows& in = isv ? a.v : a.k;
-    const int units = dim / 16;
     const bool rot = !isv && a.rope.table;
     auto load = [&](int i, float* v, int& ca, int& cb) {  // unit i of the run
-        const int j = i / units, u = i - j * units, t = t0 + j;
+        const int j = i >> lu, u = i & (units - 1);
+        const int64_t t = t0 + j;
         unit_chunks(u, rot ? a.rope.rot : 0, a.rope.half, ca, cb);
         const T* x = reinterpret_cast<const T*>(in.p) + t * in.st + h * in.sh;
         load8(x + ca, in.vec, v);
@@ -48,53 +46,125 @@ __global__ void __launch_bounds__(128) kv_append_kernel(KvArg kv, AppendArg a) {
         }
         return j;
     };
-    float amax = 0.0f;
+    float* sp = (isv ? kv.vs : kv.ks) + (size_t)block * kv.heads + h;
+    const float old = first ? *sp : 0.0f;
+    float amax = 0.0f, held[HOLD][16];
     bool bad = false;
-    for (int i = tid; i < n * units; i += 128) {
-        float v[16];
-        int ca, cb;
-        load(i, v, ca, cb);
+    auto top = [&](const float* v) {
 #pragma unroll
         for (int e = 0; e < 16; e++) {
             const float m = fabsf(v[e]);
             if (m <= 3.4028234663852886e38f) amax = fmaxf(amax, m); else bad = true;
         }
+    };
+    int ca, cb;
+#pragma unroll
+    for (int k = 0; k < HOLD; k++)
+        if (tid + k * NT < n * units) load(tid + k * NT, held[k], ca, cb);
+#pragma unroll
+    for (int k = 0; k < HOLD; k++)
+        if (tid + k * NT < n * units) top(held[k]);
+    for (int i = tid + HOLD * NT; i < n * units; i += NT) {
+        float v[16];
+        load(i, v, ca, cb);
+        top(v);
     }
-    __shared__ float red[4];
+    if (bad) atomicOr(kv.status, (unsigned)DERR_NONFINITE);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if (bad) atomicOr(kv.status, (unsigned)DERR_NONFINITE);
-    if ((tid & 31) == 0) red[tid >> 5] = amax;
-    float* sp = (isv ? kv.vs : kv.ks) + (size_t)block * kv.heads + h;
-    const float old = first ? *sp : 0.0f;
-    __syncthreads();
-    amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    if (NT > 32) {
+        if ((tid & 31) == 0) red[tid >> 5] = amax;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NT / 32; i++) amax = fmaxf(amax, red[i]);
+    }
     float want = __fmul_rn(amax, Code<CODE>::PER);
     if (want < 1.1754943508222875e-38f) want = 0.0f;  // 1 / want must stay finite
     const float scale = fmaxf(old, want), inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
     uint8_t* base = (isv ? kv.v : kv.k) + ((size_t)block * kv.heads + h) * bs * dim;
     if (scale > old && first) {  // the block's earlier tokens, rounded again to the new scale
         const float ratio = __fmul_rn(old, inv);
-        for (int i = tid; i < first * dim / 4; i += 128) {
-            uint32_t w = reinterpret_cast<uint32_t*>(base)[i], o = 0;
+        for (int i = tid; i < first * dim / 4; i += NT) {
+            const uint32_t w = reinterpret_cast<uint32_t*>(base)[i];
+            uint32_t o = 0;
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                o |= Code<CODE>::put(__fmul_rn(Code<CODE>::get(w >> (8 * e)), ratio)) << (8 * e);
+            for (int e = 0; e < 4; e++) o |= Code<CODE>::put(__fmul_rn(Code<CODE>::get(w >> (8 * e)), ratio)) << (8 * e);
             reinterpret_cast<uint32_t*>(base)[i] = o;
         }
     }
-    for (int i = tid; i < n * units; i += 128) {
-        float v[16];
-        int ca, cb;
-        const int j = load(i, v, ca, cb);
+    auto store = [&](int i, const float* v) {
+        const int j = i >> lu, u = i & (units - 1);
+        unit_chunks(u, rot ? a.rope.rot : 0, a.rope.half, ca, cb);
         uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int e = 0; e < 16; e++) w[e / 4] |= Code<CODE>::put(__fmul_rn(v[e], inv)) << (8 * (e & 3));
         uint8_t* row = base + (size_t)(first + j) * dim;
         *reinterpret_cast<uint2*>(row + ca) = make_uint2(w[0], w[1]);
         *reinterpret_cast<uint2*>(row + cb) = make_uint2(w[2], w[3]);
+    };
+#pragma unroll
+    for (int k = 0; k < HOLD; k++)
+        if (tid + k * NT < n * units) store(tid + k * NT, held[k]);
+    for (int i = tid + HOLD * NT; i < n * units; i += NT) {
+        float v[16];
+        load(i, v, ca, cb);
+        store(i, v);
     }
-    if (tid == 0) *sp = scale;  // every thread read the old one before the barrier
+    if (NT > 32) __syncthreads();  // red is used again; every thread has read the old scale
+    else __syncwarp();
+    if (tid == 0) *sp = scale;
+}
+
+template <typename T, int CODE>
+__global__ void __launch_bounds__(APT, 3) kv_append_kernel(KvArg kv, AppendArg a) {
+    __shared__ float red[APT / 32];
+    __shared__ int s_run[128], s_n;  // first tokens of the runs that begin in the window
+    const int tid = threadIdx.x;
+    pdl_trigger();
+    pdl_wait();
+    if ((int)blockIdx.x >= a.kv_ctas) {  // q, as the rope kernel turns it
+        Rows none{};
+        turn_items<T>(a.q, a.qo, none, none, a.rope, a.T, kv.dim, (int64_t)(blockIdx.x - a.kv_ctas) * APT + tid,
+                      (int64_t)(gridDim.x - a.kv_ctas) * APT, kv.status);
+        return;
+    }
+    const int per = 2 * kv.heads, win = blockIdx.x / per, hv = blockIdx.x - win * per, h = hv >> 1, bs = kv.bs;
+    const bool isv = hv & 1;
+    if (tid == 0) s_n = 0;
+    __syncthreads();
+    const int t = win * a.window + tid;
+    if (tid < a.window && t < a.T) {
+        const int slot = __ldg(a.slots + t), prev = t > 0 ? __ldg(a.slots + t - 1) : -2;
+        if (slot >= 0) {
+            if ((slot >> kv.shift) >= kv.n_blocks) {
+                if (hv == 0) atomicOr(kv.status, (unsigned)DERR_INDEX);
+            } else if ((slot & (bs - 1)) == 0 || prev != slot - 1) {
+                s_run[atomicAdd(&s_n, 1)] = t;
+            }
+        }
+    }
+    __syncthreads();
+    const int runs = s_n, lane = tid & 31, w = tid >> 5;
+    // the run's length: up to 32 slots at a time, by a warp
+    auto length = [&](int t0, int slot) {
+        const int room = min(bs - (slot & (bs - 1)), a.T - t0);
+        for (int n = 0;; n += 32) {
+            const bool same = n + lane < room && __ldg(a.slots + t0 + n + lane) == slot + n + lane;
+            const unsigned m = __ballot_sync(0xffffffffu, same);
+            if (m != 0xffffffffu) return n + __ffs(~m) - 1;
+        }
+    };
+    if (runs <= 2) {
+        for (int i = 0; i < runs; i++) {
+            const int t0 = s_run[i], slot = __ldg(a.slots + t0);
+            write_run<T, CODE, APT>(kv, a, isv, h, t0, length(t0, slot), slot, tid, red);
+        }
+    } else {
+        for (int i = w; i < runs; i += APT / 32) {
+            const int t0 = s_run[i], slot = __ldg(a.slots + t0);
+            write_run<T, CODE, 32>(kv, a, isv, h, t0, length(t0, slot), slot, lane, nullptr);
+        }
+    }
 }
 
 // One thread per 16 elements of a slot and head, K then V.
@@ -102,26 +172,25 @@ template <typename T, int CODE>
 __global__ void __launch_bounds__(256) kv_read_kernel(KvArg kv, const int32_t* slots, int n, T* ko, T* vo) {
     pdl_trigger();
     pdl_wait();
-    const int units = kv.dim / 16;
-    const uint64_t per = (uint64_t)n * kv.heads * units, all = 2 * per;
-    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < all; i += gridDim.x * 256ull) {
-        const bool isv = i >= per;
-        const uint64_t r = isv ? i - per : i;
-        const int u = (int)(r % units);
-        const uint64_t th = r / units;
-        const int h = (int)(th % kv.heads), t = (int)(th / kv.heads);
+    const int units = kv.dim / 16, lu = 31 - __clz(units);
+    const bool isv = blockIdx.y;
+    const uint64_t per = (uint64_t)n * kv.heads << lu;
+    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < per; i += gridDim.x * 256ull) {
+        const int u = (int)i & (units - 1);
+        const uint64_t th = i >> lu;
+        const int t = (th >> 32) == 0 ? (int)((uint32_t)th / (uint32_t)kv.heads) : (int)(th / kv.heads), h = (int)(th - (uint64_t)t * kv.heads);
         const int slot = __ldg(slots + t);
         float v[16];
 #pragma unroll
         for (int e = 0; e < 16; e++) v[e] = 0.0f;
-        if (slot >= 0 && slot / kv.bs < kv.n_blocks) {
-            const size_t bh = (size_t)(slot / kv.bs) * kv.heads + h;
+        if (slot >= 0 && (slot >> kv.shift) < kv.n_blocks) {
+            const size_t bh = (size_t)(slot >> kv.shift) * kv.heads + h;
             const float s = __ldg((isv ? kv.vs : kv.ks) + bh);
             const uint4 w = __ldg(reinterpret_cast<const uint4*>((isv ? kv.v : kv.k) + (bh * kv.bs + (slot & (kv.bs - 1))) * kv.dim) + u);
             const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
             for (int e = 0; e < 16; e++) v[e] = __fmul_rn(Code<CODE>::get(ww[e / 4] >> (8 * (e & 3))), s);
-        } else if (slot >= 0 && u == 0 && h == 0) {
+        } else if (slot >= 0 && u == 0 && h == 0 && !isv) {
             atomicOr(kv.status, (unsigned)DERR_INDEX);
         }
         T* y = (isv ? vo : ko) + th * kv.dim + 16 * u;
@@ -131,14 +200,30 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvArg kv, const int32_t* s
 }
 
 template <typename T, int CODE>
-static cudaError_t append_launch(const KvArg& kv, const AppendArg& a, cudaStream_t s) {
-    return launch_pdl(kv_append_kernel<T, CODE>, dim3((unsigned)a.T, (unsigned)kv.heads, 2), dim3(128), 0, s, kv, a);
+static cudaError_t append_launch(const KvArg& kv, AppendArg a, cudaStream_t s) {
+    // Decoded tokens are a run each: windows of 8 give every warp one, until such windows fill the
+    // chip; then a block's worth of tokens, in which a prompt begins one or two runs.
+    a.window = a.T <= 1024 ? 8 : kv.bs;
+    const int64_t kvc = ((int64_t)a.T + a.window - 1) / a.window * kv.heads * 2;
+    const int64_t qn = (int64_t)a.T * a.q.heads * (kv.dim / 16);
+    // One launch for both where it is the launch that costs; for prompts q's stream goes through the
+    // rope kernel, whose threads need half the registers and keep more loads in flight.
+    const bool apart = qn > 148 * APT * 4;
+    if (apart) {
+        const Rows none{};
+        cudaError_t e = launch_rope_apply(a.q, a.qo, none, none, a.rope, a.T, kv.dim, Elt<T>::TYPE, kv.status, s);
+        if (e != cudaSuccess) return e;
+    }
+    const int64_t qc = apart ? 0 : (qn + APT - 1) / APT;
+    if (kvc + qc > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    a.kv_ctas = (int)kvc;
+    return launch_pdl(kv_append_kernel<T, CODE>, dim3((unsigned)(kvc + qc)), dim3(APT), 0, s, kv, a);
 }
 
 template <typename T, int CODE>
 static cudaError_t read_launch(const KvArg& kv, const int32_t* slots, int n, void* ko, void* vo, cudaStream_t s) {
-    const uint64_t all = 2ull * n * kv.heads * (kv.dim / 16), ctas = (all + 255) / 256;
-    return launch_pdl(kv_read_kernel<T, CODE>, dim3((unsigned)(ctas < 148 * 64 ? ctas : 148 * 64)), dim3(256), 0, s, kv, slots, n,
+    const uint64_t ctas = ((uint64_t)n * kv.heads * (kv.dim / 16) + 255) / 256;
+    return launch_pdl(kv_read_kernel<T, CODE>, dim3((unsigned)(ctas < 148 * 64 ? ctas : 148 * 64), 2), dim3(256), 0, s, kv, slots, n,
                       (T*)ko, (T*)vo);
 }
 
@@ -153,15 +238,14 @@ rmoe_status rmoe_kv_append(rmoe_kv* kv, const rmoe_kv_append_args* a, void* stre
     if (!elt_ok(a->type)) return fail(RMOE_ERR_UNSUPPORTED, "kv append: ggml type %u (F32, F16 or BF16)", a->type);
     if (a->T > 0x7fffffffu) return fail(RMOE_ERR_UNSUPPORTED, "%u tokens", a->T);
     AppendArg p{};
-    Rows q, qo;
     rmoe_status st;
     if ((st = check_rows(a->k, a->T, a->type, "k", p.k)) || (st = check_rows(a->v, a->T, a->type, "v", p.v)) ||
-        (st = check_rows(a->q, a->T, a->type, "q", q)) || (st = check_rows(a->q_out, a->T, a->type, "q_out", qo)))
+        (st = check_rows(a->q, a->T, a->type, "q", p.q)) || (st = check_rows(a->q_out, a->T, a->type, "q_out", p.qo)))
         return st;
     if (a->k.heads != kv->heads || a->v.heads != kv->heads)
         return fail(RMOE_ERR_INVALID, "k / v have %u / %u heads, the cache %u", a->k.heads, a->v.heads, kv->heads);
-    if (q.heads != qo.heads) return fail(RMOE_ERR_INVALID, "q_out has %d heads, q %d", qo.heads, q.heads);
-    if (q.heads && !a->rope) return fail(RMOE_ERR_INVALID, "q is only taken with a rope");
+    if (p.q.heads != p.qo.heads) return fail(RMOE_ERR_INVALID, "q_out has %d heads, q %d", p.qo.heads, p.q.heads);
+    if (p.q.heads && !a->rope) return fail(RMOE_ERR_INVALID, "q is only taken with a rope");
     if (a->rope) {
         if (a->rope->device != kv->device) return fail(RMOE_ERR_INVALID, "the rope is on another device");
         if (a->rope->rot > kv->dim || a->rope->rot % 16)
@@ -181,20 +265,13 @@ rmoe_status rmoe_kv_append(rmoe_kv* kv, const rmoe_kv_append_args* a, void* stre
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const KvArg ka = kv_arg(kv);
     const bool i8 = kv->code == RMOE_KV_INT8;
-    cudaError_t e = cudaSuccess;
-    if (q.heads) {
-        Rows none{};
-        e = launch_rope_apply(q, qo, none, none, p.rope, p.T, ka.dim, a->type, kv->status, s);
-    }
-    if (e == cudaSuccess) {
-        if (a->type == T_F32)
-            e = i8 ? append_launch<float, RMOE_KV_INT8>(ka, p, s) : append_launch<float, RMOE_KV_E4M3>(ka, p, s);
-        else if (a->type == T_F16)
-            e = i8 ? append_launch<__half, RMOE_KV_INT8>(ka, p, s) : append_launch<__half, RMOE_KV_E4M3>(ka, p, s);
-        else
-            e = i8 ? append_launch<__nv_bfloat16, RMOE_KV_INT8>(ka, p, s)
-                   : append_launch<__nv_bfloat16, RMOE_KV_E4M3>(ka, p, s);
-    }
+    cudaError_t e;
+    if (a->type == T_F32)
+        e = i8 ? append_launch<float, RMOE_KV_INT8>(ka, p, s) : append_launch<float, RMOE_KV_E4M3>(ka, p, s);
+    else if (a->type == T_F16)
+        e = i8 ? append_launch<__half, RMOE_KV_INT8>(ka, p, s) : append_launch<__half, RMOE_KV_E4M3>(ka, p, s);
+    else
+        e = i8 ? append_launch<__nv_bfloat16, RMOE_KV_INT8>(ka, p, s) : append_launch<__nv_bfloat16, RMOE_KV_E4M3>(ka, p, s);
     return e == cudaSuccess ? RMOE_OK : cuda_fail(e, "kv append launch");
 }
 

@@ -21,35 +21,13 @@ __global__ void __launch_bounds__(256) rope_table_kernel(float2* table, const do
     }
 }
 
-// One thread per unit of 16 elements (rope.cuh); a token's units are neighbours, q heads first.
+// Units of 16 elements (rope.cuh), spread over all threads.
 template <typename T>
-__global__ void __launch_bounds__(256) rope_units_kernel(Rows q, Rows qo, Rows k, Rows ko, RopeArg ra, int T_, int dim,
-                                                         unsigned* status) {
+__global__ void __launch_bounds__(256, 3) rope_units_kernel(Rows q, Rows qo, Rows k, Rows ko, RopeArg ra, int T_, int dim,
+                                                            unsigned* status) {
     pdl_trigger();
     pdl_wait();
-    const int per_head = dim / 16, per_tok = (q.heads + k.heads) * per_head;
-    const uint64_t n = (uint64_t)T_ * per_tok;
-    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += gridDim.x * 256ull) {
-        const int t = (int)(i / per_tok), r = (int)(i - (uint64_t)t * per_tok), h = r / per_head, u = r - h * per_head;
-        const bool isq = h < q.heads;
-        const Rows& in = isq ? q : k;
-        const Rows& out = isq ? qo : ko;
-        const int hh = isq ? h : h - q.heads;
-        const T* x = reinterpret_cast<const T*>(in.p) + t * in.st + hh * in.sh;
-        T* y = reinterpret_cast<T*>(out.p) + t * out.st + hh * out.sh;
-        int a, b;
-        unit_chunks(u, ra.rot, ra.half, a, b);
-        float v[16];
-        load8(x + a, in.vec, v);
-        load8(x + b, in.vec, v + 8);
-        const int p = __ldg(ra.pos + t);
-        if ((unsigned)p < (unsigned)ra.max_pos)
-            turn_unit(v, u, ra.table + (size_t)p * (ra.rot / 2), ra.rot, ra.half, ra.sign);
-        else if (u == 0 && h == 0)
-            atomicOr(status, (unsigned)DERR_INDEX);
-        store8(y + a, out.vec, v);
-        store8(y + b, out.vec, v + 8);
-    }
+    turn_items<T>(q, qo, k, ko, ra, T_, dim, blockIdx.x * 256ll + threadIdx.x, gridDim.x * 256ll, status);
 }
 
 // Head and rotary sizes that are not multiples of 16: one thread per pair, then per copied element.
@@ -91,10 +69,10 @@ template <typename T>
 static cudaError_t rope_launch(const Rows& q, const Rows& qo, const Rows& k, const Rows& ko, const RopeArg& ra, int T_,
                                int dim, unsigned* status, cudaStream_t s) {
     const bool units = dim % 16 == 0 && ra.rot % 16 == 0;
-    const uint64_t n = (uint64_t)T_ * (q.heads + k.heads) * (units ? dim / 16 : dim - ra.rot / 2);
-    const unsigned grid = (unsigned)((n + 255) / 256 < 148 * 64 ? (n + 255) / 256 : 148 * 64);
-    return launch_pdl(units ? rope_units_kernel<T> : rope_pairs_kernel<T>, dim3(grid), dim3(256), 0, s, q, qo, k, ko, ra, T_, dim,
-                      status);
+    const uint64_t n = (uint64_t)T_ * (q.heads + k.heads) * (units ? dim / 16 : dim - ra.rot / 2), ctas = (n + 255) / 256;
+    const unsigned most = units ? 148 * 3 : 148 * 64;  // units: the CTAs that are resident, each thread walks over many
+    return launch_pdl(units ? rope_units_kernel<T> : rope_pairs_kernel<T>, dim3((unsigned)(ctas < most ? ctas : most)), dim3(256), 0,
+                      s, q, qo, k, ko, ra, T_, dim, status);
 }
 
 cudaError_t launch_rope_apply(const Rows& q, const Rows& qo, const Rows& k, const Rows& ko, const RopeArg& ra, int T,
