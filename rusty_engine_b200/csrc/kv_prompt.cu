@@ -33,7 +33,8 @@ struct PromptShape {
     static constexpr int NRT = PAIR ? 1 : 2;             // row tiles
     static constexpr int QB = 128 * D * 2;               // fp16 bytes of a Q, K or V tile
     static constexpr int RAW = PKV * D;
-    static constexpr int KN = 2, VN = PAIR ? 1 : 2;      // operand buffers
+    // operand buffers; f32 has room for three: K's is free again as soon as S is made, V's only after P V
+    static constexpr int KN = PAIR ? 1 : 2, VN = 2;
     static constexpr int Q0 = 0, K0 = 2 * QB, V0 = K0 + KN * QB, R0 = V0 + VN * QB, END = R0 + 2 * RAW;
     static constexpr int SMEM = END + 1024;              // + alignment
 };
