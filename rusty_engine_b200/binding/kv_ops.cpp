@@ -181,14 +181,21 @@ PyObject* extend(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         e.free_list = ints(fr, "free", dev);
         e.n_free = ints(nf, "n_free", dev, 1);
         const c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
-        const auto opt = table.options();
-        at::Tensor cu = at::empty({R + 1}, opt), pos = at::empty({T}, opt), slots = at::empty({T}, opt), lo = at::empty({R}, opt),
-                   no = at::empty({1}, opt);
-        e.cu = cu.data_ptr<int32_t>();
-        e.positions = pos.data_ptr<int32_t>();
-        e.slots = slots.data_ptr<int32_t>();
-        e.lens_out = lo.data_ptr<int32_t>();
-        e.n_free_out = no.data_ptr<int32_t>();
+        // one allocation, five tensors of it
+        const int64_t sizes[5] = {R + 1, T, T, R, 1};
+        const at::Tensor buf = at::empty({2 * R + 2 + 2 * T}, table.options());
+        at::Tensor out[5];
+        int32_t* at_[5];
+        for (int64_t i = 0, off = 0; i < 5; off += sizes[i++]) {
+            out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(), buf.dtype());
+            out[i].unsafeGetTensorImpl()->set_sizes_and_strides(c10::IntArrayRef(&sizes[i], 1), c10::IntArrayRef({1}), off);
+            at_[i] = buf.data_ptr<int32_t>() + off;
+        }
+        e.cu = at_[0];
+        e.positions = at_[1];
+        e.slots = at_[2];
+        e.lens_out = at_[3];
+        e.n_free_out = at_[4];
         e.R = (uint32_t)R;
         e.max_blocks = (uint32_t)table.size(1);
         e.T = (uint32_t)T;
@@ -197,8 +204,7 @@ PyObject* extend(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         check(rmoe_kv_extend(&e, stream_of(dev)));
         PyObject* t = PyTuple_New(5);
         if (!t) throw Raised();
-        const at::Tensor* o[5] = {&cu, &pos, &slots, &lo, &no};
-        for (int i = 0; i < 5; i++) PyTuple_SET_ITEM(t, i, THPVariable_Wrap(*o[i]));
+        for (int i = 0; i < 5; i++) PyTuple_SET_ITEM(t, i, THPVariable_Wrap(out[i]));
         return t;
     });
 }

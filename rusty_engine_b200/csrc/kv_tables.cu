@@ -13,36 +13,37 @@ namespace rmoe {
 static constexpr int EXT_THREADS = 1024;
 static constexpr uint32_t EXT_MAX_R = 16384;
 
-// Exclusive prefix sums of one 64-bit value per thread over the CTA; total in `sum`.
-__device__ __forceinline__ int64_t cta_scan(int64_t v, int64_t* warp_tot, int64_t& sum) {
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    int64_t x = v;
+// Exclusive prefix sums of one 64-bit value per thread over the CTA; total in `sum`.  warp_tot: 32
+// words, those past the CTA's warps 0.
+__device__ __forceinline__ int64_t warp_scan(int64_t x) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
+    return x;
+}
+__device__ __forceinline__ int64_t cta_scan(int64_t v, int64_t* warp_tot, int64_t& sum) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int64_t x = warp_scan(v);
     __syncthreads();  // warp_tot may still be read from the previous call
     if (lane == 31) warp_tot[w] = x;
     __syncthreads();
-    int64_t before = 0, all = 0;
-    for (int i = 0; i < nw; i++) {
-        const int64_t t = warp_tot[i];
-        if (i < w) before += t;
-        all += t;
-    }
-    sum = all;
-    return before + x - v;
+    const int64_t t = warp_tot[lane], all = warp_scan(t);  // every warp scans the warps' totals
+    sum = __shfl_sync(0xffffffffu, all, 31);
+    return __shfl_sync(0xffffffffu, all - t, w) + x - v;
 }
 
 __global__ void __launch_bounds__(EXT_THREADS) kv_extend_kernel(rmoe_kv_extend_args a) {
     extern __shared__ int32_t sm[];
     int32_t* s_cu = sm;                // [R + 1] first token of each request
     int32_t* s_first = sm + a.R + 1;   // [R] blocks that earlier requests take, -1: refused
-    __shared__ int64_t warp_tot[EXT_THREADS / 32];
+    __shared__ int64_t warp_tot[32];
     __shared__ int s_used;
-    const int tid = threadIdx.x, R = (int)a.R, bs = (int)a.block_size;
-    const int per = (R + EXT_THREADS - 1) / EXT_THREADS, r0 = min(R, tid * per), r1 = min(R, r0 + per);
+    const int tid = threadIdx.x, R = (int)a.R, bs = (int)a.block_size, sh = 31 - __clz(bs);
+    const int nth = blockDim.x, per = (R + nth - 1) / nth, r0 = min(R, tid * per), r1 = min(R, r0 + per);
+    if (tid < 32) warp_tot[tid] = 0;
     pdl_trigger();
     pdl_wait();
     const int height = max(0, min(__ldg(a.n_free), (int)a.free_cap));
@@ -53,7 +54,7 @@ __global__ void __launch_bounds__(EXT_THREADS) kv_extend_kernel(rmoe_kv_extend_a
     auto need = [&](int r, int64_t first, int n) -> int64_t {  // blocks r asks for, -1: does not fit its row or T
         const int64_t len = max(0, __ldg(a.lens + r));
         if (len + n > (int64_t)a.max_blocks * bs || first + n > (int64_t)a.T) return -1;
-        return (len + n + bs - 1) / bs - (len + bs - 1) / bs;
+        return ((len + n + bs - 1) >> sh) - ((len + bs - 1) >> sh);
     };
     int64_t asked = 0, c = at;
     for (int r = r0; r < r1; r++) {
@@ -85,7 +86,7 @@ __global__ void __launch_bounds__(EXT_THREADS) kv_extend_kernel(rmoe_kv_extend_a
         a.cu[R] = s_cu[R];
         *a.n_free_out = __ldg(a.n_free) < 0 ? 0 : height - s_used;
     }
-    for (uint64_t t = blockIdx.x * (uint64_t)EXT_THREADS + tid; t < a.T; t += gridDim.x * (uint64_t)EXT_THREADS) {
+    for (uint64_t t = blockIdx.x * (uint64_t)nth + tid; t < a.T; t += gridDim.x * (uint64_t)nth) {
         int slot = -1, pos = 0;
         if ((int64_t)t < s_cu[R]) {
             int lo = 0, hi = R - 1;  // the last request whose first token is at or before t (and that has tokens)
@@ -96,16 +97,16 @@ __global__ void __launch_bounds__(EXT_THREADS) kv_extend_kernel(rmoe_kv_extend_a
             const int r = lo, len = max(0, __ldg(a.lens + r));
             pos = len + (int)((int64_t)t - s_cu[r]);
             if (s_first[r] >= 0) {
-                const int have = (len + bs - 1) / bs, page = pos / bs;
+                const int have = (len + bs - 1) >> sh, page = pos >> sh;
                 int32_t* entry = a.table + (size_t)r * a.max_blocks + page;
                 int block;
                 if (page < have) {
                     block = *entry;
                 } else {
                     block = __ldg(a.free_list + (height - 1 - s_first[r] - (page - have)));
-                    if (pos == max(page * bs, len)) *entry = block;  // the block's first new token
+                    if (pos == max(page << sh, len)) *entry = block;  // the block's first new token
                 }
-                slot = block < 0 ? -1 : block * bs + pos % bs;
+                slot = block < 0 ? -1 : (block << sh) + (pos & (bs - 1));
             }
         }
         a.positions[t] = pos;
@@ -116,7 +117,7 @@ __global__ void __launch_bounds__(EXT_THREADS) kv_extend_kernel(rmoe_kv_extend_a
 // One CTA: prefix sums of the blocks to give back, then a warp per request moves them.
 __global__ void __launch_bounds__(EXT_THREADS) kv_release_kernel(rmoe_kv_release_args a) {
     extern __shared__ int32_t s_at[];  // [R] stack position of the request's first block, -1: not done
-    __shared__ int64_t warp_tot[EXT_THREADS / 32];
+    __shared__ int64_t warp_tot[32];
     const int tid = threadIdx.x, R = (int)a.R, bs = (int)a.block_size;
     const int per = (R + EXT_THREADS - 1) / EXT_THREADS, r0 = min(R, tid * per), r1 = min(R, r0 + per);
     const int height = max(0, min(__ldg(a.n_free), (int)a.free_cap));
@@ -173,8 +174,9 @@ rmoe_status rmoe_kv_extend(const rmoe_kv_extend_args* a, void* stream) {
     static std::atomic<uint64_t> done{0};
     cudaError_t e = allow_smem(kv_extend_kernel, 132 << 10, done);
     if (e != cudaSuccess) return cuda_fail(e, "kv extend");
-    const unsigned grid = (unsigned)((a->T + EXT_THREADS - 1) / EXT_THREADS);
-    e = launch_pdl(kv_extend_kernel, dim3(grid < 1 ? 1 : grid < 148 ? grid : 148), dim3(EXT_THREADS), smem,
+    // small batches: fewer threads, whose barriers are shorter
+    const unsigned nth = a->R <= 256 && a->T <= 16384 ? 256 : EXT_THREADS, grid = (unsigned)((a->T + nth - 1) / nth);
+    e = launch_pdl(kv_extend_kernel, dim3(grid < 1 ? 1 : grid < 148 ? grid : 148), dim3(nth), smem,
                    static_cast<cudaStream_t>(stream), *a);
     return e == cudaSuccess ? RMOE_OK : cuda_fail(e, "kv extend launch");
 }
