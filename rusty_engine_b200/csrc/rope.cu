@@ -8,7 +8,10 @@
 
 #include <vector>
 
+#include <algorithm>
+
 #include "rope.cuh"
+#include "tc_ptx.cuh"
 
 namespace rmoe {
 
@@ -28,6 +31,104 @@ __global__ void __launch_bounds__(256, 3) rope_units_kernel(Rows q, Rows qo, Row
     pdl_trigger();
     pdl_wait();
     turn_items<T>(q, qo, k, ko, ra, T_, dim, blockIdx.x * 256ll + threadIdx.x, gridDim.x * 256ll, status);
+}
+
+// Long batches of heads that lie one after the other: a warp brings a token's q, k and angles into
+// its own part of shared memory as bulk copies, turns them there and sends them back as bulk
+// copies, three tokens deep.  The copies keep the memory busy with hardly any registers, where
+// per-thread loads reached 62-66% of the copy rate whatever their number; a ring shared by the
+// CTA's warps, in step from token to token, was no faster than those (8192 tokens of 32 + 4 heads of
+// 128 in bf16, B200).
+struct RopeStream {
+    uint32_t qb, kb, ab, stage;  // bytes of a token's q, k and angles, and of a stage
+    int warps;
+};
+static constexpr int RS_STAGES = 3, RS_MAX_WARPS = 8;
+
+template <typename T>
+__global__ void __launch_bounds__(RS_MAX_WARPS * 32)
+    rope_stream_kernel(Rows q, Rows qo, Rows k, Rows ko, RopeArg ra, int T_, int dim, RopeStream rs, unsigned* status) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t s_full[RS_MAX_WARPS][RS_STAGES];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const uint32_t skew = (128u - (smem_u32(smem_raw) & 127u)) & 127u;
+    uint8_t* ring = smem_raw + skew + w * RS_STAGES * rs.stage;
+    const uint32_t ring_s = smem_u32(ring);
+    if (lane == 0) {
+        for (int i = 0; i < RS_STAGES; i++) tc::mbar_init(smem_u32(&s_full[w][i]), 1);
+        tc::fence_mbar_init();
+    }
+    __syncwarp();
+    pdl_trigger();
+    pdl_wait();
+    const int step = gridDim.x * rs.warps, t0 = blockIdx.x + w * gridDim.x;  // tokens t0, t0 + step, ...
+    const int n = t0 < T_ ? (T_ - 1 - t0) / step + 1 : 0;
+    int pos = 0;         // lane l: of token 32 * (i / 32) + l
+    unsigned turned = 0; // bit s: the token in stage s is turned
+    auto load = [&](int i) {
+        const int64_t t = t0 + (int64_t)i * step;
+        if ((i & 31) == 0) {
+            const int64_t tl = t + (int64_t)lane * step;
+            pos = tl < T_ ? __ldg(ra.pos + tl) : 0;
+        }
+        const int p = __shfl_sync(0xffffffffu, pos, i & 31), s = i % RS_STAGES;
+        const bool in = (unsigned)p < (unsigned)ra.max_pos;
+        turned = in ? turned | 1u << s : turned & ~(1u << s);
+        if (lane == 0) {
+            const uint32_t bar = smem_u32(&s_full[w][s]), dst = ring_s + s * rs.stage;
+            if (!in) atomicOr(status, (unsigned)DERR_INDEX);
+            tc::mbar_arrive_expect_tx(bar, rs.qb + rs.kb + (in ? rs.ab : 0));
+            tc::bulk_g2s(dst, q.p + t * q.st * (int64_t)sizeof(T), rs.qb, bar);
+            if (rs.kb) tc::bulk_g2s(dst + rs.qb, k.p + t * k.st * (int64_t)sizeof(T), rs.kb, bar);
+            if (in) tc::bulk_g2s(dst + rs.qb + rs.kb, ra.table + (int64_t)p * (ra.rot / 2), rs.ab, bar);
+        }
+    };
+    int loaded = 0, i = 0;
+    bool dead = false;
+    for (; loaded < min(n, RS_STAGES); loaded++) load(loaded);
+    const int units = ra.rot >> 4, all = (q.heads + k.heads) * units;  // rotated units only
+    for (; i < n; i++) {
+        const int s = i % RS_STAGES;
+        dead = !__all_sync(0xffffffffu, tc::mbar_wait_tries(smem_u32(&s_full[w][s]), (i / RS_STAGES) & 1));
+        if (dead) break;
+        uint8_t* st = ring + s * rs.stage;
+        const float4* ang = reinterpret_cast<const float4*>(st + rs.qb + rs.kb);
+        if (turned >> s & 1) {
+#pragma unroll 2
+            for (int u = lane; u < all; u += 32) {
+                const int h = u / units, c = u - h * units;  // k's heads follow q's
+                int a, b;
+                unit_chunks(c, ra.rot, ra.half, a, b);
+                T* x = reinterpret_cast<T*>(st) + h * dim;
+                float v[16];
+                float4 cs[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) cs[j] = ang[c * 4 + j];
+                load8(x + a, true, v);
+                load8(x + b, true, v + 8);
+                turn_unit_by(v, cs, ra.half, ra.sign);
+                store8(x + a, true, v);
+                store8(x + b, true, v + 8);
+            }
+        }
+        tc::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            const int64_t t = t0 + (int64_t)i * step;
+            const uint32_t src = ring_s + s * rs.stage;
+            tc::bulk_s2g(qo.p + t * qo.st * (int64_t)sizeof(T), src, rs.qb);
+            if (rs.kb) tc::bulk_s2g(ko.p + t * ko.st * (int64_t)sizeof(T), src + rs.qb, rs.kb);
+            tc::bulk_commit();
+            tc::bulk_wait_read<1>();  // the token before has left its stage
+        }
+        __syncwarp();
+        if (i > 0 && loaded < n) load(loaded), loaded++;
+    }
+    if (dead) {
+        if (lane == 0) atomicOr(status, (unsigned)DERR_TIMEOUT);
+        for (; i < loaded; i++) tc::mbar_wait_tries(smem_u32(&s_full[w][i % RS_STAGES]), (i / RS_STAGES) & 1);
+    }
+    if (lane == 0) tc::bulk_wait<0>();
 }
 
 // Head and rotary sizes that are not multiples of 16: one thread per pair, then per copied element.
@@ -69,6 +170,24 @@ template <typename T>
 static cudaError_t rope_launch(const Rows& q, const Rows& qo, const Rows& k, const Rows& ko, const RopeArg& ra, int T_,
                                int dim, unsigned* status, cudaStream_t s) {
     const bool units = dim % 16 == 0 && ra.rot % 16 == 0;
+    const bool rows = q.vec && qo.vec && q.sh == dim && qo.sh == dim && (!k.heads || (k.vec && ko.vec && k.sh == dim && ko.sh == dim));
+    // the ring pays from a few tokens a warp on, and where the stages of three warps fit an SM
+    if (units && rows && q.heads && T_ >= 148 * 8) {
+        RopeStream rs;
+        rs.qb = (uint32_t)(q.heads * dim * sizeof(T));
+        rs.kb = (uint32_t)(k.heads * dim * sizeof(T));
+        rs.ab = (uint32_t)(ra.rot / 2 * sizeof(float2));
+        rs.stage = (rs.qb + rs.kb + rs.ab + 127) / 128 * 128;
+        constexpr uint32_t room = 220 << 10;
+        rs.warps = (int)std::min<uint32_t>(RS_MAX_WARPS, room / (RS_STAGES * rs.stage));
+        if (rs.warps >= 3) {
+            static std::atomic<uint64_t> done{0};
+            cudaError_t e = allow_smem(rope_stream_kernel<T>, room + 128, done);
+            if (e != cudaSuccess) return e;
+            return launch_pdl(rope_stream_kernel<T>, dim3(148), dim3(rs.warps * 32), rs.warps * RS_STAGES * rs.stage + 128, s, q, qo, k,
+                              ko, ra, T_, dim, rs, status);
+        }
+    }
     const uint64_t n = (uint64_t)T_ * (q.heads + k.heads) * (units ? dim / 16 : dim - ra.rot / 2), ctas = (n + 255) / 256;
     const unsigned most = units ? 148 * 3 : 148 * 64;  // units: the CTAs that are resident, each thread walks over many
     return launch_pdl(units ? rope_units_kernel<T> : rope_pairs_kernel<T>, dim3((unsigned)(ctas < most ? ctas : most)), dim3(256), 0,

@@ -87,7 +87,8 @@ def test_batch_extend_release_cycle(kv):
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("half", [True, False])
 @pytest.mark.parametrize("d,rot,nq,nk,T", [(128, 128, 32, 4, 7), (64, 32, 3, 1, 1), (256, 256, 2, 2, 130),
-                                           (80, 40, 5, 0, 9), (96, 24, 1, 1, 33), (128, 64, 8, 8, 1000)])
+                                           (80, 40, 5, 0, 9), (96, 24, 1, 1, 33), (128, 64, 8, 8, 1000), (128, 128, 6, 1, 1900),
+                                           (64, 32, 5, 0, 3001), (256, 256, 3, 2, 1184)])
 def test_rope_matches_float64(kv, dtype, half, d, rot, nq, nk, T):
     g = torch.Generator().manual_seed(T)
     cfg = kv.RopeConfig(rot, 1e6, kv.RopeLayout.Half if half else kv.RopeLayout.Interleaved)
@@ -121,6 +122,27 @@ def test_rope_odd_strides_in_place_and_back(kv):
         assert rope.apply(q, pos, out=q).data_ptr() == q.data_ptr() and torch.equal(q, want)
         back = rope.apply(want, pos, inverse=True)
         assert (back.float() - keep.float()).abs().max() < (1e-5 if dt == torch.float32 else 0.1)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rope_long_batches_in_place(kv, dtype):
+    """Long batches take another kernel: in place on views of a fused buffer, whose other heads stay,
+    against the same tokens in short batches bit for bit; a position outside leaves its token alone."""
+    from rusty_engine_b200._lib import RmoeError
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rope = kv.Rope(kv.RopeConfig(64, 1e4, kv.RopeLayout.Interleaved), 5000)
+    x = torch.randn((2500, 4 + 2 + 2, 128), generator=g, device="cuda").to(R.DT[dtype])
+    pos = torch.randint(0, 5000, (2500,), generator=g, device="cuda").to(torch.int32)
+    pos[7], pos[2400] = 5000, -3
+    keep = x.clone()
+    want = [rope.apply(x[i:i + 500, :4], pos[i:i + 500], x[i:i + 500, 4:6]) for i in range(0, 2500, 500)]
+    q, k = (torch.cat(w) for w in zip(*want))
+    rope.apply(x[:, :4], pos, x[:, 4:6], out=x[:, :4], k_out=x[:, 4:6])
+    assert torch.equal(x[:, :4], q) and torch.equal(x[:, 4:6], k) and torch.equal(x[:, 6:], keep[:, 6:])
+    assert torch.equal(x[7], keep[7]) and torch.equal(x[2400], keep[2400])
+    with pytest.raises(RmoeError, match="position"):
+        rope.check()
 
 
 @pytest.mark.parametrize("kw", [dict(scaling="linear", factor=8.0), dict(scaling="yarn", factor=4.0, orig=4096),
