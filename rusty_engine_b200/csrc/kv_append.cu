@@ -13,6 +13,7 @@ struct AppendArg {
     int T;
     int window;   // tokens of a CTA's window
     int kv_ctas;  // the CTAs from here on turn q
+    bool apart;   // q is turned by the kernel before this one, which had its inputs when it let this one start
 };
 
 // A run is the tokens of one call that go to consecutive slots of one block: they share a scale.
@@ -118,10 +119,11 @@ __device__ __forceinline__ void write_run(const KvArg& kv, const AppendArg& a, b
 template <typename T, int CODE>
 __global__ void __launch_bounds__(APT, 3) kv_append_kernel(KvArg kv, AppendArg a) {
     __shared__ float red[APT / 32];
-    __shared__ int s_run[128], s_n;  // first tokens of the runs that begin in the window
+    __shared__ int s_run[128], s_slot[128], s_n;  // the runs that begin in the window: first token and slot
+    __shared__ unsigned s_cont[APT / 32];
     const int tid = threadIdx.x;
     pdl_trigger();
-    pdl_wait();
+    if (!a.apart) pdl_wait();
     if ((int)blockIdx.x >= a.kv_ctas) {  // q, as the rope kernel turns it
         Rows none{};
         turn_items<T>(a.q, a.qo, none, none, a.rope, a.T, kv.dim, (int64_t)(blockIdx.x - a.kv_ctas) * APT + tid,
@@ -130,41 +132,47 @@ __global__ void __launch_bounds__(APT, 3) kv_append_kernel(KvArg kv, AppendArg a
     }
     const int per = 2 * kv.heads, win = blockIdx.x / per, hv = blockIdx.x - win * per, h = hv >> 1, bs = kv.bs;
     const bool isv = hv & 1;
+    // the window's slots and those that a run beginning in it can reach (window + bs <= 256): which
+    // of them continue their predecessor's run
+    const int t = win * a.window + tid;
+    const int slot = t < a.T ? __ldg(a.slots + t) : -1, prev = t > 0 && t < a.T ? __ldg(a.slots + t - 1) : -2;
+    const bool cont = slot >= 0 && (slot & (bs - 1)) != 0 && prev == slot - 1;
+    const unsigned cm = __ballot_sync(0xffffffffu, cont);
+    if ((tid & 31) == 0) s_cont[tid >> 5] = cm;
     if (tid == 0) s_n = 0;
     __syncthreads();
-    const int t = win * a.window + tid;
-    if (tid < a.window && t < a.T) {
-        const int slot = __ldg(a.slots + t), prev = t > 0 ? __ldg(a.slots + t - 1) : -2;
-        if (slot >= 0) {
-            if ((slot >> kv.shift) >= kv.n_blocks) {
-                if (hv == 0) atomicOr(kv.status, (unsigned)DERR_INDEX);
-            } else if ((slot & (bs - 1)) == 0 || prev != slot - 1) {
-                s_run[atomicAdd(&s_n, 1)] = t;
-            }
+    if (tid < a.window && slot >= 0 && !cont) {
+        if ((slot >> kv.shift) < kv.n_blocks) {
+            const int i = atomicAdd(&s_n, 1);
+            s_run[i] = tid;
+            s_slot[i] = slot;
+        } else if (hv == 0) {
+            atomicOr(kv.status, (unsigned)DERR_INDEX);
         }
     }
     __syncthreads();
     const int runs = s_n, lane = tid & 31, w = tid >> 5;
-    // the run's length: up to 32 slots at a time, by a warp
-    auto length = [&](int t0, int slot) {
-        const int room = min(bs - (slot & (bs - 1)), a.T - t0);
-        for (int n = 0;; n += 32) {
-            const bool same = n + lane < room && __ldg(a.slots + t0 + n + lane) == slot + n + lane;
-            const unsigned m = __ballot_sync(0xffffffffu, same);
-            if (m != 0xffffffffu) return n + __ffs(~m) - 1;
+    // the run that begins at token x of the window: 1 + the bits that are set from x + 1 on
+    auto length = [&](int x) {
+        int n = 1;
+        for (int b = x + 1;; b = (b | 31) + 1) {
+            if (b >= APT) return n;
+            const unsigned rest = ~(s_cont[b >> 5] >> (b & 31));  // first clear bit from b on
+            const int ones = rest ? __ffs(rest) - 1 : 32, room = 32 - (b & 31);
+            n += min(ones, room);
+            if (ones < room) return n;
         }
     };
     if (runs <= 2) {
         for (int i = 0; i < runs; i++) {
-            const int t0 = s_run[i], slot = __ldg(a.slots + t0);
-            write_run<T, CODE, APT>(kv, a, isv, h, t0, length(t0, slot), slot, tid, red);
+            write_run<T, CODE, APT>(kv, a, isv, h, win * a.window + s_run[i], length(s_run[i]), s_slot[i], tid, red);
         }
     } else {
         for (int i = w; i < runs; i += APT / 32) {
-            const int t0 = s_run[i], slot = __ldg(a.slots + t0);
-            write_run<T, CODE, 32>(kv, a, isv, h, t0, length(t0, slot), slot, lane, nullptr);
+            write_run<T, CODE, 32>(kv, a, isv, h, win * a.window + s_run[i], length(s_run[i]), s_slot[i], lane, nullptr);
         }
     }
+    if (a.apart) pdl_wait();  // the next kernel may take the end of this one for the end of both
 }
 
 // One thread per 16 elements of a slot and head, K then V.
@@ -207,16 +215,21 @@ static cudaError_t append_launch(const KvArg& kv, AppendArg a, cudaStream_t s) {
     const int64_t kvc = ((int64_t)a.T + a.window - 1) / a.window * kv.heads * 2;
     const int64_t qn = (int64_t)a.T * a.q.heads * (kv.dim / 16);
     // One launch for both where it is the launch that costs; for prompts q's stream goes through the
-    // rope kernel, whose threads need half the registers and keep more loads in flight.
-    const bool apart = qn > 148 * APT * 4;
-    if (apart) {
+    // rope kernel's bulk copies, and this kernel runs beside it: neither needs the other's results.
+    a.apart = qn > 148 * APT * 4;
+    if (a.apart) {
         const Rows none{};
         cudaError_t e = launch_rope_apply(a.q, a.qo, none, none, a.rope, a.T, kv.dim, Elt<T>::TYPE, kv.status, s);
         if (e != cudaSuccess) return e;
     }
-    const int64_t qc = apart ? 0 : (qn + APT - 1) / APT;
+    const int64_t qc = a.apart ? 0 : (qn + APT - 1) / APT;
     if (kvc + qc > 0x7fffffff) return cudaErrorInvalidConfiguration;
     a.kv_ctas = (int)kvc;
+    if (a.apart) {  // an SM runs both kernels at once only if they divide its memory alike
+        static std::atomic<uint64_t> done{0};
+        cudaError_t e = all_shared(kv_append_kernel<T, CODE>, done);
+        if (e != cudaSuccess) return e;
+    }
     return launch_pdl(kv_append_kernel<T, CODE>, dim3((unsigned)(kvc + qc)), dim3(APT), 0, s, kv, a);
 }
 

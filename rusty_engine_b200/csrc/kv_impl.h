@@ -68,6 +68,18 @@ inline cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) 
     return e;
 }
 
+// Has a kernel's launches ask for the largest shared memory of an SM, whatever they use of it.
+template <typename K>
+inline cudaError_t all_shared(K kernel, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_relaxed) & bit))) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
+
 inline uint32_t elt_size(uint32_t type) { return type == T_F32 ? 4 : 2; }
 inline bool elt_ok(uint32_t type) { return type == T_F32 || type == T_F16 || type == T_BF16; }
 
