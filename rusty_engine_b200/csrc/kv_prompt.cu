@@ -88,8 +88,8 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     const int heads = kv.heads, bs = kv.bs, group = a.group;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
 
-    pdl_trigger();
     pdl_wait();
+    pdl_trigger();  // the split kernel, which takes the other requests, fills the SMs that run out of work here
     // ---- which request, head and rows ----
     const int64_t max_rows = split_max_rows(a, heads, group, s_sum);
     if (max_rows == INT64_MAX) return;

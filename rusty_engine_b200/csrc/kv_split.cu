@@ -134,7 +134,9 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
 
     const int br = min(bs, TW), nb = TW / br;  // rows and number of a tile's boxes
     pdl_trigger();
-    pdl_wait();
+    // the prompt kernel before this one had its inputs when it let this one start, and its requests
+    // are not this one's: it is only waited for at the end
+    if (!a.prompts) pdl_wait();
 
     // ---- this CTA's share of the units ----
     const int per = (a.R + NT - 1) / NT;
@@ -763,6 +765,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         }
         __syncthreads();  // s_last is used again
     }
+    if (a.prompts) pdl_wait();
 }
 
 template <typename T, int CODE, int D, int NR>
