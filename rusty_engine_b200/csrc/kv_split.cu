@@ -100,6 +100,11 @@ __device__ __forceinline__ int64_t quot(int64_t a, int64_t b) {
     return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
+struct SplitSpan {    // an item that spans CTAs c0 .. c0 + n - 1
+    SplitPiece pc;
+    int c0, n;
+};
+
 struct SplitStart {   // where a warp's share begins
     SplitReq rq;
     int r;
@@ -125,7 +130,8 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     __shared__ int64_t s_first[NW];
     __shared__ int64_t s_tot[NW];
     __shared__ SplitPiece s_piece[2 * NW];
-    __shared__ int s_last;
+    __shared__ SplitSpan s_span[2];
+    __shared__ int s_last[2];
 
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, c = lane & 3;
     const uint32_t ring0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -688,6 +694,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         return x;
     };
     const unsigned valid = __ballot_sync(0xffffffffu, lane < 2 * NW && (s_piece[lane & (2 * NW - 1)].flags & 1));
+    int spans = 0;
     for (unsigned todo = valid; todo;) {
         const SplitPiece& pc = s_piece[__ffs(todo) - 1];
         // the slots that hold pieces of this item
@@ -721,19 +728,33 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 if (lane == 0) __stcg(slot + NR * M::ROW + row, mm), __stcg(slot + NR * (M::ROW + 1) + row, ll);
             }
         }
-        if (whole) continue;
-        // the CTAs that hold the item's first and last unit
-        auto cta_of = [&](int64_t u) {
-            const int64_t big = extra * (each + 1);
-            return (int)(u < big ? quot(u, each + 1) : extra + quot(u - big, each));
-        };
-        const int c0 = cta_of(pc.a), n = cta_of(pc.a + pc.tiles - 1) - c0 + 1;
+        if (!whole) {
+            // the CTAs that hold the item's first and last unit
+            auto cta_of = [&](int64_t u) {
+                const int64_t big = extra * (each + 1);
+                return (int)(u < big ? quot(u, each + 1) : extra + quot(u - big, each));
+            };
+            // at most two items of a CTA span others: the one it begins with and the one it ends with
+            const int k = (flags & 2) ? 1 : 0;
+            if (tid == 0) {
+                s_span[k].pc = pc;
+                s_span[k].c0 = cta_of(pc.a);
+                s_span[k].n = cta_of(pc.a + pc.tiles - 1) - s_span[k].c0 + 1;
+            }
+            spans |= 1 << k;
+        }
+    }
+    if (spans) {
         __threadfence();
         __syncthreads();
-        if (tid == 0) s_last = atomicAdd(ws.ticket + c0, 1u) == (unsigned)(n - 1);
+        if (tid < 2)
+            s_last[tid] = (spans >> tid & 1) && atomicAdd(ws.ticket + s_span[tid].c0, 1u) == (unsigned)(s_span[tid].n - 1);
         __syncthreads();
-        if (s_last) {
-            __threadfence();
+        if (s_last[0] || s_last[1]) __threadfence();
+#pragma unroll 1
+        for (int z = 0; z < 2; z++) {
+            if (!s_last[z]) continue;
+            const int c0 = s_span[z].c0, n = s_span[z].n;
             auto part = [&](int k) { return ws.part + (size_t)(2 * (c0 + k) + (k == 0 ? 1 : 0)) * M::PIECE; };
 #pragma unroll 1
             for (int row = w; row < NR; row += NW) {
@@ -759,11 +780,10 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     }
                 }
                 ll = wsum(ll);
-                emit(pc, row, mm, ll, o);
+                emit(s_span[z].pc, row, mm, ll, o);
             }
             if (tid == 0) ws.ticket[c0] = 0;
         }
-        __syncthreads();  // s_last is used again
     }
     if (a.prompts) pdl_wait();
 }
