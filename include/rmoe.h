@@ -372,7 +372,8 @@ typedef struct {
 RMOE_API rmoe_status rmoe_kv_release(const rmoe_kv_release_args* args, void* stream);
 
 /* The cache: codes [n_blocks][n_kv_heads][block_size][head_dim], 8 bits each, and one f32 scale
- * per block and head ([n_blocks][n_kv_heads]) for K and for V; a cached value is code * scale. */
+ * per block and head ([n_blocks][n_kv_heads], not negative) for K and for V; a cached value is
+ * code * scale. */
 enum { RMOE_KV_INT8 = 0, RMOE_KV_E4M3 = 1 };
 
 typedef struct {
@@ -397,8 +398,9 @@ RMOE_API rmoe_status rmoe_kv_status(rmoe_kv* kv);
  * tokens.  Per run and head: s = max(scale of the block if it holds earlier tokens, max|x| / 127
  * (448 for e4m3)), codes round(x / s) to nearest even; where s grew, the earlier codes are
  * rounded again to the new scale.  NaN is stored as 0 and infinities as the largest code, and
- * both set the status word.  With rope, k is turned by positions[t] first (in f32), and where
- * q.heads > 0 so is q into q_out. */
+ * both set the status word.  With rope (rot_dim a multiple of 16, at most head_dim), k is turned by
+ * positions[t] first (in f32), and where q.heads > 0 so is q into q_out (which may be q, but not
+ * overlap k or v). */
 typedef struct {
     rmoe_rows k, v, q, q_out;
     const int32_t *slots, *positions;

@@ -32,7 +32,9 @@ rmoe_status rmoe_kv_create(const rmoe_kv_desc* d, rmoe_kv** out) {
     rmoe_kv* kv = nullptr;
     try {
         kv = new rmoe_kv();
+        kv->own.ptrs.reserve(8);  // nothing below throws
     } catch (...) {
+        delete kv;
         return fail(RMOE_ERR_OOM, "cache handle");
     }
     kv->device = d->device;

@@ -1,5 +1,6 @@
 // kv_attend.cu -- attention over the 8-bit paged cache: checks, and the choice of kernel.
 #include <algorithm>
+#include <cmath>
 
 #include "kv_attend.h"
 
@@ -17,6 +18,9 @@ extern "C" rmoe_status rmoe_kv_attend(rmoe_kv* kv, const rmoe_kv_attend_args* a,
     if (a->q.heads == 0 || a->q.heads % kv->heads)
         return fail(RMOE_ERR_INVALID, "%u query heads over %u kv heads", a->q.heads, kv->heads);
     if (a->out.heads != a->q.heads) return fail(RMOE_ERR_INVALID, "out has %u heads, q %u", a->out.heads, a->q.heads);
+    if (!std::isfinite(a->scale)) return fail(RMOE_ERR_INVALID, "attention scale %g", a->scale);
+    if ((uint64_t)a->T * (a->q.heads / kv->heads) > 0x7fffffffull)  // rows are numbered in 32 bits
+        return fail(RMOE_ERR_UNSUPPORTED, "%u tokens x %u query heads per kv head", a->T, a->q.heads / kv->heads);
     if (a->T == 0) return RMOE_OK;
     if (a->R == 0) return fail(RMOE_ERR_INVALID, "tokens without requests");
     if (!a->lens || !a->cu || (a->max_blocks && !a->table)) return fail(RMOE_ERR_INVALID, "kv attend: null pointer");

@@ -273,7 +273,9 @@ rmoe_status rmoe_rope_create(const rmoe_rope_desc* d, rmoe_rope** out) {
     try {
         f.resize(pairs);
         r = new rmoe_rope();
+        r->own.ptrs.reserve(4);  // nothing below throws
     } catch (...) {
+        delete r;
         return fail(RMOE_ERR_OOM, "rope handle");
     }
     for (uint32_t i = 0; i < pairs; i++) {
