@@ -100,11 +100,6 @@ __device__ __forceinline__ int64_t quot(int64_t a, int64_t b) {
     return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
-struct SplitSpan {    // an item that spans CTAs c0 .. c0 + n - 1
-    SplitPiece pc;
-    int c0, n;
-};
-
 struct SplitStart {   // where a warp's share begins
     SplitReq rq;
     int r;
@@ -130,8 +125,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     __shared__ int64_t s_first[NW];
     __shared__ int64_t s_tot[NW];
     __shared__ SplitPiece s_piece[2 * NW];
-    __shared__ SplitSpan s_span[2];
-    __shared__ int s_last[2];
+    __shared__ int s_last;
 
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, c = lane & 3;
     const uint32_t ring0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -145,71 +139,95 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     if (!a.prompts) pdl_wait();
 
     // ---- this CTA's share of the units ----
-    const int per = (a.R + NT - 1) / NT;
-    const int64_t max_rows = a.prompts ? split_max_rows(a, heads, group, s_tot) : INT64_MAX;
-    int64_t mine = 0;
-    SplitReq rq{};
-    for (int r = tid * per; r < min(a.R, (tid + 1) * per); r++) {
-        rq = split_req(a, r, heads, group, bs, NR, TW, max_rows);
-        mine += (int64_t)rq.items * rq.tiles;
-    }
-    int64_t incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-    }
-    if (lane == 31) s_tot[w] = incl;
-    if (tid < 2 * NW) s_piece[tid].flags = 0;
+    if (lane < 2) s_piece[2 * w + lane].flags = 0;
     if (lane == 0) {
         for (int i = 0; i < DEPTH; i++) tc::mbar_init(smem_u32(&s_full[w][i]), 1 + nb);
         tc::fence_mbar_init();
     }
-    __syncthreads();
-    int64_t before = 0, W = 0;
-#pragma unroll
-    for (int i = 0; i < NW; i++) {
-        if (i < w) before += s_tot[i];
-        W += s_tot[i];
-    }
-    // a share of less than a tile per warp would only add joining
-    const int active = (int)min((int64_t)gridDim.x, (W + NW - 1) / NW);
-    const int64_t each = active ? quot(W, active) : 0;
-    const int extra = (int)(W - each * active);  // the first `extra` CTAs take one unit more
+    __syncwarp();
     const int bx = blockIdx.x;
-    const int64_t u0 = each * bx + min(bx, extra);
-    const int64_t cnt_u = bx < active ? each + (bx < extra) : 0;
-    const int64_t wbase = u0 + cnt_u / NW * w + min(w, (int)(cnt_u % NW)), wlen = cnt_u / NW + (w < cnt_u % NW);
-    // the thread that holds a warp's first unit tells it where that is
-    if (lane == 0) s_first[w] = wlen > 0 ? wbase : -1;
-    __syncthreads();
-    {
+    int64_t each = 0, wbase = 0, wlen = 0;  // units of a CTA; this warp's first unit and their number
+    int extra = 0;                           // the first `extra` CTAs take one unit more
+    auto shares = [&](int64_t W) {
+        // a share of less than a tile per warp would only add joining
+        const int active = (int)min((int64_t)gridDim.x, (W + NW - 1) / NW);
+        each = active ? quot(W, active) : 0;
+        extra = (int)(W - each * active);
+        const int64_t n = bx < active ? each + (bx < extra) : 0;
+        wbase = each * bx + min(bx, extra) + n / NW * w + min(w, (int)(n % NW));
+        wlen = n / NW + (w < n % NW);
+    };
+    auto scan = [&](int64_t x) {  // inclusive, over the warp
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        return x;
+    };
+    // the request of the warp's first unit, and how many of its units come before
+    SplitReq rq{};
+    int r = 0;
+    int64_t rem = 0, max_rows = INT64_MAX;
+    if (a.R <= 32 && !a.prompts) {  // every warp sums up by itself: two barriers less, 1.5 us
+        if (lane < a.R) rq = split_req(a, lane, heads, group, bs, NR, TW, max_rows);
+        const int64_t mine = (int64_t)rq.items * rq.tiles, incl = scan(mine), at = incl - mine;
+        shares(__shfl_sync(0xffffffffu, incl, 31));
+        const unsigned own = __ballot_sync(0xffffffffu, wbase >= at && wbase < at + mine);
+        r = own ? __ffs(own) - 1 : 0;
+        rem = wbase - __shfl_sync(0xffffffffu, at, r);
+        int* f = reinterpret_cast<int*>(&rq);
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(SplitReq) / 4); i++) f[i] = __shfl_sync(0xffffffffu, f[i], r);
+    } else {
+        const int per = (a.R + NT - 1) / NT;
+        if (a.prompts) max_rows = split_max_rows(a, heads, group, s_tot);
+        int64_t mine = 0;
+        for (int i = tid * per; i < min(a.R, (tid + 1) * per); i++) {
+            rq = split_req(a, i, heads, group, bs, NR, TW, max_rows);
+            mine += (int64_t)rq.items * rq.tiles;
+        }
+        const int64_t incl = scan(mine);
+        if (lane == 31) s_tot[w] = incl;
+        __syncthreads();
+        int64_t before = 0, W = 0;
+#pragma unroll
+        for (int i = 0; i < NW; i++) {
+            if (i < w) before += s_tot[i];
+            W += s_tot[i];
+        }
+        shares(W);
+        // the thread that holds a warp's first unit tells it where that is
+        if (lane == 0) s_first[w] = wlen > 0 ? wbase : -1;
+        __syncthreads();
         const int64_t at = before + incl - mine;
-        if (at + mine > u0 && at < u0 + cnt_u)
+        if (mine > 0)
 #pragma unroll 1
             for (int i = 0; i < NW; i++) {
                 const int64_t u = s_first[i];
                 if (u >= at && u < at + mine) {
-                    int64_t rem = u - at;
-                    int r = tid * per;
+                    int64_t left = u - at;
+                    int k = tid * per;
                     SplitReq q = rq;
                     if (per > 1) {
-                        q = split_req(a, r, heads, group, bs, NR, TW, max_rows);
-                        while (rem >= (int64_t)q.items * q.tiles) {
-                            rem -= (int64_t)q.items * q.tiles;
-                            q = split_req(a, ++r, heads, group, bs, NR, TW, max_rows);
+                        q = split_req(a, k, heads, group, bs, NR, TW, max_rows);
+                        while (left >= (int64_t)q.items * q.tiles) {
+                            left -= (int64_t)q.items * q.tiles;
+                            q = split_req(a, ++k, heads, group, bs, NR, TW, max_rows);
                         }
                     }
-                    s_start[i] = SplitStart{q, r, rem};
+                    s_start[i] = SplitStart{q, k, left};
                 }
             }
+        __syncthreads();
+        if (wlen > 0) {
+            rq = s_start[w].rq;
+            r = s_start[w].r;
+            rem = s_start[w].rem;
+        }
     }
-    __syncthreads();
 
     if (wlen > 0) {
-        rq = s_start[w].rq;
-        int r = s_start[w].r;
-        const int64_t rem = s_start[w].rem;
         int item = (int)quot(rem, rq.tiles), tile = (int)(rem - (int64_t)item * rq.tiles);
 
         // the rows of the current item, and its q
@@ -694,7 +712,6 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         return x;
     };
     const unsigned valid = __ballot_sync(0xffffffffu, lane < 2 * NW && (s_piece[lane & (2 * NW - 1)].flags & 1));
-    int spans = 0;
     for (unsigned todo = valid; todo;) {
         const SplitPiece& pc = s_piece[__ffs(todo) - 1];
         // the slots that hold pieces of this item
@@ -728,33 +745,19 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 if (lane == 0) __stcg(slot + NR * M::ROW + row, mm), __stcg(slot + NR * (M::ROW + 1) + row, ll);
             }
         }
-        if (!whole) {
-            // the CTAs that hold the item's first and last unit
-            auto cta_of = [&](int64_t u) {
-                const int64_t big = extra * (each + 1);
-                return (int)(u < big ? quot(u, each + 1) : extra + quot(u - big, each));
-            };
-            // at most two items of a CTA span others: the one it begins with and the one it ends with
-            const int k = (flags & 2) ? 1 : 0;
-            if (tid == 0) {
-                s_span[k].pc = pc;
-                s_span[k].c0 = cta_of(pc.a);
-                s_span[k].n = cta_of(pc.a + pc.tiles - 1) - s_span[k].c0 + 1;
-            }
-            spans |= 1 << k;
-        }
-    }
-    if (spans) {
+        if (whole) continue;
+        // the CTAs that hold the item's first and last unit
+        auto cta_of = [&](int64_t u) {
+            const int64_t big = extra * (each + 1);
+            return (int)(u < big ? quot(u, each + 1) : extra + quot(u - big, each));
+        };
+        const int c0 = cta_of(pc.a), n = cta_of(pc.a + pc.tiles - 1) - c0 + 1;
         __threadfence();
         __syncthreads();
-        if (tid < 2)
-            s_last[tid] = (spans >> tid & 1) && atomicAdd(ws.ticket + s_span[tid].c0, 1u) == (unsigned)(s_span[tid].n - 1);
+        if (tid == 0) s_last = atomicAdd(ws.ticket + c0, 1u) == (unsigned)(n - 1);
         __syncthreads();
-        if (s_last[0] || s_last[1]) __threadfence();
-#pragma unroll 1
-        for (int z = 0; z < 2; z++) {
-            if (!s_last[z]) continue;
-            const int c0 = s_span[z].c0, n = s_span[z].n;
+        if (s_last) {
+            __threadfence();
             auto part = [&](int k) { return ws.part + (size_t)(2 * (c0 + k) + (k == 0 ? 1 : 0)) * M::PIECE; };
 #pragma unroll 1
             for (int row = w; row < NR; row += NW) {
@@ -780,10 +783,11 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     }
                 }
                 ll = wsum(ll);
-                emit(s_span[z].pc, row, mm, ll, o);
+                emit(pc, row, mm, ll, o);
             }
             if (tid == 0) ws.ticket[c0] = 0;
         }
+        __syncthreads();  // s_last is used again
     }
     if (a.prompts) pdl_wait();
 }
