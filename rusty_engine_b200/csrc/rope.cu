@@ -24,7 +24,8 @@ __global__ void __launch_bounds__(256) rope_table_kernel(float2* table, const do
     }
 }
 
-// Units of 16 elements (rope.cuh), spread over all threads.
+// Units of 16 elements (rope.cuh), spread over all threads: short batches, and heads that do not lie
+// one after the other.  16 tokens of 32 + 4 heads of 128 in f32: 2.0 us (B200, calls in a graph), latency.
 template <typename T>
 __global__ void __launch_bounds__(256, 3) rope_units_kernel(Rows q, Rows qo, Rows k, Rows ko, RopeArg ra, int T_, int dim,
                                                             unsigned* status) {
@@ -38,7 +39,8 @@ __global__ void __launch_bounds__(256, 3) rope_units_kernel(Rows q, Rows qo, Row
 // copies, three tokens deep.  The copies keep the memory busy with hardly any registers, where
 // per-thread loads reached 62-66% of the copy rate whatever their number; a ring shared by the
 // CTA's warps, in step from token to token, was no faster than those (8192 tokens of 32 + 4 heads of
-// 128 in bf16, B200).
+// 128 in bf16, B200).  A ring per warp: 27.4 us, 153 MB, 5.6 TB/s = 85% of the copy rate;
+// 67 MB of q in and out: 25.6 us where a copy takes 24.7.
 struct RopeStream {
     uint32_t qb, kb, ab, stage;  // bytes of a token's q, k and angles, and of a stage
     int warps;
