@@ -18,6 +18,11 @@
 // fp16 in the operand registers; the order of d inside a contraction and of tokens inside a tile
 // are free, and are chosen so that each lane's operand is the 16 bytes that it reads.
 //
+// A tile of keys that none of an item's rows sees (after a causal prompt's early rows, before a
+// window) is neither fetched nor computed, and early and late row tiles take turns in the numbering, so
+// that the shares stay alike: a prompt of 2048 tokens, 16 heads over 4 of 256, 713 -> 477 us in bf16, 878
+// -> 588 in f32.
+//
 // Joining.  A share's incomplete first and last items leave (M, l, O) pieces; the CTA joins its
 // warps' pieces, and items that span CTAs go through a workspace slot per CTA, where the last
 // arriving CTA (an atomic count, nobody waits) joins them in CTA order: the result does not depend
@@ -92,6 +97,23 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
     uint2 v;
     asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(a));
     return v;
+}
+
+// Item -> kv head and tile of rows.  Early and late row tiles take turns: an early row of a causal
+// prompt sees few keys, and a warp's share of consecutive items then holds as many of either kind.
+struct SplitItem { int kh, rt; };
+__device__ __forceinline__ SplitItem split_item(int item, int items, int heads) {
+    if (items == heads) return {item, 0};
+    const int rts = items / heads, k = item / (2 * heads), j = item - k * 2 * heads;
+    if (2 * k + 1 == rts) return {j, k};  // the middle one has no partner
+    return {j >> 1, (j & 1) ? rts - 1 - k : k};
+}
+
+// Keys that some row of the row tile sees: lo .. hi - 1.
+struct SplitKeys { int lo, hi; };
+__device__ __forceinline__ SplitKeys split_keys(const AttendArg& a, const SplitReq& q, int rt, int nr, int group) {
+    const int first = rt * nr / group, last = min(q.n - 1, (rt * nr + nr - 1) / group);
+    return {a.window ? max(0, q.pos0 + first - a.window + 1) : 0, min(q.pos0 + last + 1, q.hi)};
 }
 
 struct SplitPiece {   // where a piece belongs
@@ -242,8 +264,9 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         // row row0 + i is token tok0 + (rem0 + i) / group, head (rem0 + i) % group of the group
         auto tok_of = [&](int i) { return tok0 + (group == 1 ? i : (int)__umulhi((uint32_t)(rem0 + i), a.group_inv)); };
         auto next_rows = [&]() {
-            kh = item % heads;
-            row0 = item / heads * NR;
+            const SplitItem it = split_item(item, rq.items, heads);
+            kh = it.kh;
+            row0 = it.rt * NR;
             tok0 = row0 / group;
             rem0 = row0 - tok0 * group;
 #pragma unroll
@@ -274,6 +297,8 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         int pr = r, pitem = item, ptile = tile;
         int64_t pleft = wlen;
         int pblk = -1;
+        SplitItem pit = split_item(pitem, pq.items, heads);
+        SplitKeys pkeys = split_keys(a, pq, pit.rt, NR, group);
         auto lookup = [&]() {  // lane b < nb: the block of box b of the tile to issue next
             const int j = (pq.t0 + ptile) * TW + lane * br;
             pblk = -1;
@@ -283,14 +308,15 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         auto issue = [&](int stage) {
             const uint32_t bar = smem_u32(&s_full[w][stage]);
             const int j = (pq.t0 + ptile) * TW + lane * br;
-            const bool want = lane < nb && j < pq.hi, ok = want && (unsigned)pblk < (unsigned)kv.n_blocks;
+            // a tile that no row sees is not fetched: its boxes count as missing
+            const int j0 = (pq.t0 + ptile) * TW;
+            const bool want = lane < nb && j < pq.hi && j0 < pkeys.hi && j0 + TW > pkeys.lo, ok = want && (unsigned)pblk < (unsigned)kv.n_blocks;
             if (want && !ok) atomicOr(kv.status, (unsigned)DERR_INDEX);
             const unsigned mask = __ballot_sync(0xffffffffu, ok);
             if (lane == 0) tc::mbar_arrive_expect_tx(bar, __popc(mask) * br * D * 2);
             __syncwarp();
             if (ok) {
-                const int kh = pitem % heads;
-                const int64_t bh = (int64_t)pblk * heads + kh;
+                const int64_t bh = (int64_t)pblk * heads + pit.kh;
                 const int row = (int)(bh * bs + (j & (bs - 1)));
                 const uint32_t dst = ring0 + (w * DEPTH + stage) * S::STAGE + lane * br * (D < 128 ? D : 128);
 #pragma unroll
@@ -313,6 +339,8 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     do pq = split_req(a, ++pr, heads, group, bs, NR, TW, max_rows);
                     while (pq.items == 0);
                 }
+                pit = split_item(pitem, pq.items, heads);
+                pkeys = split_keys(a, pq, pit.rt, NR, group);
             }
             lookup();
         };
@@ -382,6 +410,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const int all_hi = min(rq.pos0 + firstt + 1, rq.hi);
             const int all_lo = a.window ? max(0, rq.pos0 + last - a.window + 1) : 0;
             const int any_lo = a.window ? max(0, rq.pos0 + firstt - a.window + 1) : 0;
+            const int any_hi = min(rq.pos0 + last + 1, rq.hi);
 
             float o[QT][KS][4], m[QT][2], l[QT][2];
 #pragma unroll
@@ -399,186 +428,188 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 }
                 const uint32_t kb = ring0 + (w * DEPTH + stage) * S::STAGE, vb = kb + TW * D;
                 const int j0 = (rq.t0 + tile + s) * TW;
-                float kscale[MT], lv[MT], iv[MT];
-                bool gone = false;
-#pragma unroll
-                for (int i = 0; i < MT; i++) {
-                    const float2 sc = *reinterpret_cast<const float2*>(s_scale[w][stage][MT == 2 && br == 16 ? i : 0]);
-                    const float vs = v_scale_floor(sc.y);
-                    kscale[i] = sc.x;
-                    lv[i] = lg2(vs);
-                    iv[i] = rcp(vs);
-                    gone |= kscale[i] < 0.0f;
-                }
-                const bool masked = gone || j0 < all_lo || j0 + TW > all_hi;
-                if (CODE == RMOE_KV_E4M3 && masked) {
-                    // places that no row sees may hold the format's NaN, and 0 * NaN is NaN
-                    for (int i = lane; i < TW * (D / 16); i += 32) {
-                        const int t = i / (D / 16), ch = i % (D / 16), j = j0 + t;
-                        const bool no = j >= rq.hi || j < any_lo || (MT == 2 && t >= 16 ? kscale[MT - 1] : kscale[0]) < 0.0f;
-                        // whole rows are cleared, so the swizzle inside a row does not matter
-                        if (no)
-                            *reinterpret_cast<uint4*>(ring_ptr + (vb - ring0) + (D == 256 ? (ch / 8) * TW * 128 + t * 128 + (ch % 8) * 16 : t * D + ch * 16)) =
-                                make_uint4(0, 0, 0, 0);
-                    }
-                    tc::fence_proxy_async_smem();  // before the next copy into this stage
-                    __syncwarp();
-                }
-                // S^T = K q^T: rows tokens, columns query rows.  The tensor cores cut the sums of a
-                // chain of products short at each step, so a chain is 64 elements long and the
-                // chains are added by the f32 unit (256 elements in one chain cost 1e-5 of the
-                // score); the low halves have their own chain.
-                float st[QT][MT][4], su[PAIR ? QT : 1][PAIR ? MT : 1][4];
-#pragma unroll
-                for (int nt = 0; nt < QT; nt++)
+                if (j0 < any_hi && j0 + TW > any_lo) {  // some row sees it; otherwise it was not fetched
+                    float kscale[MT], lv[MT], iv[MT];
+                    bool gone = false;
 #pragma unroll
                     for (int i = 0; i < MT; i++) {
-                        st[nt][i][0] = st[nt][i][1] = st[nt][i][2] = st[nt][i][3] = 0.0f;
-                        if (PAIR) su[nt][i][0] = su[nt][i][1] = su[nt][i][2] = su[nt][i][3] = 0.0f;
+                        const float2 sc = *reinterpret_cast<const float2*>(s_scale[w][stage][MT == 2 && br == 16 ? i : 0]);
+                        const float vs = v_scale_floor(sc.y);
+                        kscale[i] = sc.x;
+                        lv[i] = lg2(vs);
+                        iv[i] = rcp(vs);
+                        gone |= kscale[i] < 0.0f;
                     }
-#pragma unroll
-                for (int hf = 0; hf < HF; hf++)
-#pragma unroll
-                    for (int i = 0; i < MT; i++) {
-                        uint4 x[2];
-#pragma unroll
-                        for (int z = 0; z < 2; z++) {
-                            const int row = 16 * i + 8 * z + tg;
-                            x[z] = D == 64 ? lds128(kb + row * 64 + ((c ^ ((row >> 1) & 3)) << 4))
-                                           : lds128(kb + (hf / 2) * TW * 128 + row * 128 + ((((hf & 1) * 4 + c) ^ (row & 7)) << 4));
+                    const bool masked = gone || j0 < all_lo || j0 + TW > all_hi;
+                    if (CODE == RMOE_KV_E4M3 && masked) {
+                        // places that no row sees may hold the format's NaN, and 0 * NaN is NaN
+                        for (int i = lane; i < TW * (D / 16); i += 32) {
+                            const int t = i / (D / 16), ch = i % (D / 16), j = j0 + t;
+                            const bool no = j >= rq.hi || j < any_lo || (MT == 2 && t >= 16 ? kscale[MT - 1] : kscale[0]) < 0.0f;
+                            // whole rows are cleared, so the swizzle inside a row does not matter
+                            if (no)
+                                *reinterpret_cast<uint4*>(ring_ptr + (vb - ring0) + (D == 256 ? (ch / 8) * TW * 128 + t * 128 + (ch % 8) * 16 : t * D + ch * 16)) =
+                                    make_uint4(0, 0, 0, 0);
                         }
-                        float ch[QT][4];
+                        tc::fence_proxy_async_smem();  // before the next copy into this stage
+                        __syncwarp();
+                    }
+                    // S^T = K q^T: rows tokens, columns query rows.  The tensor cores cut the sums of a
+                    // chain of products short at each step, so a chain is 64 elements long and the
+                    // chains are added by the f32 unit (256 elements in one chain cost 1e-5 of the
+                    // score); the low halves have their own chain.
+                    float st[QT][MT][4], su[PAIR ? QT : 1][PAIR ? MT : 1][4];
 #pragma unroll
-                        for (int nt = 0; nt < QT; nt++) ch[nt][0] = ch[nt][1] = ch[nt][2] = ch[nt][3] = 0.0f;
-                        const uint32_t x0[4] = {x[0].x, x[0].y, x[0].z, x[0].w}, x1[4] = {x[1].x, x[1].y, x[1].z, x[1].w};
+                    for (int nt = 0; nt < QT; nt++)
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            uint32_t f[4];
-                            widen4<CODE>(x0[k], f[0], f[2]);
-                            widen4<CODE>(x1[k], f[1], f[3]);
+                        for (int i = 0; i < MT; i++) {
+                            st[nt][i][0] = st[nt][i][1] = st[nt][i][2] = st[nt][i][3] = 0.0f;
+                            if (PAIR) su[nt][i][0] = su[nt][i][1] = su[nt][i][2] = su[nt][i][3] = 0.0f;
+                        }
 #pragma unroll
-                            for (int nt = 0; nt < QT; nt++) {
-                                mma_f16_16816(ch[nt], f, qh[nt][hf * 4 + k][0], qh[nt][hf * 4 + k][1]);
-                                if (PAIR) mma_f16_16816(su[nt][i], f, ql[nt][hf * 4 + k][0], ql[nt][hf * 4 + k][1]);
+                    for (int hf = 0; hf < HF; hf++)
+#pragma unroll
+                        for (int i = 0; i < MT; i++) {
+                            uint4 x[2];
+#pragma unroll
+                            for (int z = 0; z < 2; z++) {
+                                const int row = 16 * i + 8 * z + tg;
+                                x[z] = D == 64 ? lds128(kb + row * 64 + ((c ^ ((row >> 1) & 3)) << 4))
+                                               : lds128(kb + (hf / 2) * TW * 128 + row * 128 + ((((hf & 1) * 4 + c) ^ (row & 7)) << 4));
                             }
-                        }
+                            float ch[QT][4];
 #pragma unroll
-                        for (int nt = 0; nt < QT; nt++)
+                            for (int nt = 0; nt < QT; nt++) ch[nt][0] = ch[nt][1] = ch[nt][2] = ch[nt][3] = 0.0f;
+                            const uint32_t x0[4] = {x[0].x, x[0].y, x[0].z, x[0].w}, x1[4] = {x[1].x, x[1].y, x[1].z, x[1].w};
 #pragma unroll
-                            for (int e = 0; e < 4; e++) st[nt][i][e] += ch[nt][e];
-                    }
-                // weights
-                uint32_t ph[QT][MT][2], pl[PAIR ? QT : 1][MT][2];
+                            for (int k = 0; k < 4; k++) {
+                                uint32_t f[4];
+                                widen4<CODE>(x0[k], f[0], f[2]);
+                                widen4<CODE>(x1[k], f[1], f[3]);
 #pragma unroll
-                for (int nt = 0; nt < QT; nt++) {
-                    float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-                    for (int i = 0; i < MT; i++) {
-                        const float sc[2] = {qs[nt][0] * kscale[i], qs[nt][1] * kscale[i]};
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            st[nt][i][e] = fmaf(PAIR ? st[nt][i][e] + su[nt][i][e] : st[nt][i][e], sc[e & 1], lv[i]);
-                    }
-                    if (masked) {
-#pragma unroll
-                        for (int i = 0; i < MT; i++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const int q = e & 1, j = j0 + 16 * i + 8 * (e >> 1) + tg;
-                                if (j >= vhi[nt][q] || j < vlo[nt][q] || kscale[i] < 0.0f) st[nt][i][e] = -INFINITY;
+                                for (int nt = 0; nt < QT; nt++) {
+                                    mma_f16_16816(ch[nt], f, qh[nt][hf * 4 + k][0], qh[nt][hf * 4 + k][1]);
+                                    if (PAIR) mma_f16_16816(su[nt][i], f, ql[nt][hf * 4 + k][0], ql[nt][hf * 4 + k][1]);
+                                }
                             }
-                        asm volatile("" ::: "memory");  // a branch: few tiles are masked
-                    }
-#pragma unroll
-                    for (int i = 0; i < MT; i++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) mx[e & 1] = fmaxf(mx[e & 1], st[nt][i][e]);
-                    float al[2], mu[2];
-#pragma unroll
-                    for (int q = 0; q < 2; q++) {
-                        mx[q] = fmaxf(mx[q], __shfl_xor_sync(0xffffffffu, mx[q], 4));
-                        mx[q] = fmaxf(mx[q], __shfl_xor_sync(0xffffffffu, mx[q], 8));
-                        mx[q] = fmaxf(mx[q], __shfl_xor_sync(0xffffffffu, mx[q], 16));
-                        const float mn = fmaxf(m[nt][q], mx[q]);
-                        mu[q] = mn == -INFINITY ? 0.0f : mn;
-                        al[q] = ex2(m[nt][q] - mu[q]);
-                        m[nt][q] = mn;
-                    }
-                    if (__any_sync(0xffffffffu, al[0] != 1.0f || al[1] != 1.0f)) {
-                        l[nt][0] *= al[0];
-                        l[nt][1] *= al[1];
-#pragma unroll
-                        for (int i = 0; i < KS; i++) {
-                            o[nt][i][0] *= al[0];
-                            o[nt][i][1] *= al[1];
-                            o[nt][i][2] *= al[0];
-                            o[nt][i][3] *= al[1];
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < MT; i++) {
-                        float p[4];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            p[e] = ex2(st[nt][i][e] - mu[e & 1]);
-                            l[nt][e & 1] = fmaf(p[e], iv[i], l[nt][e & 1]);
-                        }
-#pragma unroll
-                        for (int z = 0; z < 2; z++) {
-                            const uint32_t hh = pack_f16x2(p[2 * z], p[2 * z + 1]);
-                            ph[nt][i][z] = movmatrix(hh);
-                            if (PAIR) {
-                                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hh));
-                                pl[nt][i][z] = movmatrix(pack_f16x2(p[2 * z] - f.x, p[2 * z + 1] - f.y));
-                            }
-                        }
-                    }
-                }
-                // O^T += V^T P^T: rows head elements, columns query rows
-#pragma unroll
-                for (int i = 0; i < MT; i++)
-#pragma unroll
-                    for (int x = 0; x < BX; x++) {
-                        uint32_t v[4][VB / 4];
-#pragma unroll
-                        for (int z = 0; z < 4; z++) {
-                            const int row = 16 * i + 8 * (z >> 1) + ((z & 1) ? t2c1 : t2c);
-                            if (D == 64) {
-                                const uint2 y = lds64(vb + row * 64 + (((vg >> 1) ^ ((row >> 1) & 3)) << 4) + (vg & 1) * 8);
-                                v[z][0] = y.x;
-                                v[z][1] = y.y;
-                            } else {
-                                const uint4 y = lds128(vb + x * TW * 128 + row * 128 + ((vg ^ (row & 7)) << 4));
-                                v[z][0] = y.x;
-                                v[z][1] = y.y;
-                                v[z][VB / 4 - 2] = y.z;
-                                v[z][VB / 4 - 1] = y.w;
-                            }
-                        }
-#pragma unroll
-                        for (int k = 0; k < VB / 4; k++) {
-                            uint32_t f[2][4];  // of the two O^T tiles of this word
-                            widen4<CODE>(__byte_perm(v[0][k], v[1][k], 0x5140), f[0][0], f[0][1]);
-                            widen4<CODE>(__byte_perm(v[2][k], v[3][k], 0x5140), f[0][2], f[0][3]);
-                            widen4<CODE>(__byte_perm(v[0][k], v[1][k], 0x7362), f[1][0], f[1][1]);
-                            widen4<CODE>(__byte_perm(v[2][k], v[3][k], 0x7362), f[1][2], f[1][3]);
 #pragma unroll
                             for (int nt = 0; nt < QT; nt++)
 #pragma unroll
-                                for (int y = 0; y < 2; y++) {
-                                    float* acc = o[nt][x * 8 + 2 * k + y];
-                                    if (PAIR) {  // a chain of two, as above
-                                        float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                                        mma_f16_16816(t, f[y], pl[nt][i][0], pl[nt][i][1]);
-                                        mma_f16_16816(t, f[y], ph[nt][i][0], ph[nt][i][1]);
+                                for (int e = 0; e < 4; e++) st[nt][i][e] += ch[nt][e];
+                        }
+                    // weights
+                    uint32_t ph[QT][MT][2], pl[PAIR ? QT : 1][MT][2];
 #pragma unroll
-                                        for (int e = 0; e < 4; e++) acc[e] += t[e];
-                                    } else {
-                                        mma_f16_16816(acc, f[y], ph[nt][i][0], ph[nt][i][1]);
-                                    }
+                    for (int nt = 0; nt < QT; nt++) {
+                        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                        for (int i = 0; i < MT; i++) {
+                            const float sc[2] = {qs[nt][0] * kscale[i], qs[nt][1] * kscale[i]};
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                st[nt][i][e] = fmaf(PAIR ? st[nt][i][e] + su[nt][i][e] : st[nt][i][e], sc[e & 1], lv[i]);
+                        }
+                        if (masked) {
+#pragma unroll
+                            for (int i = 0; i < MT; i++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    const int q = e & 1, j = j0 + 16 * i + 8 * (e >> 1) + tg;
+                                    if (j >= vhi[nt][q] || j < vlo[nt][q] || kscale[i] < 0.0f) st[nt][i][e] = -INFINITY;
                                 }
+                            asm volatile("" ::: "memory");  // a branch: few tiles are masked
+                        }
+#pragma unroll
+                        for (int i = 0; i < MT; i++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) mx[e & 1] = fmaxf(mx[e & 1], st[nt][i][e]);
+                        float al[2], mu[2];
+#pragma unroll
+                        for (int q = 0; q < 2; q++) {
+                            mx[q] = fmaxf(mx[q], __shfl_xor_sync(0xffffffffu, mx[q], 4));
+                            mx[q] = fmaxf(mx[q], __shfl_xor_sync(0xffffffffu, mx[q], 8));
+                            mx[q] = fmaxf(mx[q], __shfl_xor_sync(0xffffffffu, mx[q], 16));
+                            const float mn = fmaxf(m[nt][q], mx[q]);
+                            mu[q] = mn == -INFINITY ? 0.0f : mn;
+                            al[q] = ex2(m[nt][q] - mu[q]);
+                            m[nt][q] = mn;
+                        }
+                        if (__any_sync(0xffffffffu, al[0] != 1.0f || al[1] != 1.0f)) {
+                            l[nt][0] *= al[0];
+                            l[nt][1] *= al[1];
+#pragma unroll
+                            for (int i = 0; i < KS; i++) {
+                                o[nt][i][0] *= al[0];
+                                o[nt][i][1] *= al[1];
+                                o[nt][i][2] *= al[0];
+                                o[nt][i][3] *= al[1];
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < MT; i++) {
+                            float p[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                p[e] = ex2(st[nt][i][e] - mu[e & 1]);
+                                l[nt][e & 1] = fmaf(p[e], iv[i], l[nt][e & 1]);
+                            }
+#pragma unroll
+                            for (int z = 0; z < 2; z++) {
+                                const uint32_t hh = pack_f16x2(p[2 * z], p[2 * z + 1]);
+                                ph[nt][i][z] = movmatrix(hh);
+                                if (PAIR) {
+                                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hh));
+                                    pl[nt][i][z] = movmatrix(pack_f16x2(p[2 * z] - f.x, p[2 * z + 1] - f.y));
+                                }
+                            }
                         }
                     }
+                    // O^T += V^T P^T: rows head elements, columns query rows
+#pragma unroll
+                    for (int i = 0; i < MT; i++)
+#pragma unroll
+                        for (int x = 0; x < BX; x++) {
+                            uint32_t v[4][VB / 4];
+#pragma unroll
+                            for (int z = 0; z < 4; z++) {
+                                const int row = 16 * i + 8 * (z >> 1) + ((z & 1) ? t2c1 : t2c);
+                                if (D == 64) {
+                                    const uint2 y = lds64(vb + row * 64 + (((vg >> 1) ^ ((row >> 1) & 3)) << 4) + (vg & 1) * 8);
+                                    v[z][0] = y.x;
+                                    v[z][1] = y.y;
+                                } else {
+                                    const uint4 y = lds128(vb + x * TW * 128 + row * 128 + ((vg ^ (row & 7)) << 4));
+                                    v[z][0] = y.x;
+                                    v[z][1] = y.y;
+                                    v[z][VB / 4 - 2] = y.z;
+                                    v[z][VB / 4 - 1] = y.w;
+                                }
+                            }
+#pragma unroll
+                            for (int k = 0; k < VB / 4; k++) {
+                                uint32_t f[2][4];  // of the two O^T tiles of this word
+                                widen4<CODE>(__byte_perm(v[0][k], v[1][k], 0x5140), f[0][0], f[0][1]);
+                                widen4<CODE>(__byte_perm(v[2][k], v[3][k], 0x5140), f[0][2], f[0][3]);
+                                widen4<CODE>(__byte_perm(v[0][k], v[1][k], 0x7362), f[1][0], f[1][1]);
+                                widen4<CODE>(__byte_perm(v[2][k], v[3][k], 0x7362), f[1][2], f[1][3]);
+#pragma unroll
+                                for (int nt = 0; nt < QT; nt++)
+#pragma unroll
+                                    for (int y = 0; y < 2; y++) {
+                                        float* acc = o[nt][x * 8 + 2 * k + y];
+                                        if (PAIR) {  // a chain of two, as above
+                                            float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                            mma_f16_16816(t, f[y], pl[nt][i][0], pl[nt][i][1]);
+                                            mma_f16_16816(t, f[y], ph[nt][i][0], ph[nt][i][1]);
+#pragma unroll
+                                            for (int e = 0; e < 4; e++) acc[e] += t[e];
+                                        } else {
+                                            mma_f16_16816(acc, f[y], ph[nt][i][0], ph[nt][i][1]);
+                                        }
+                                    }
+                            }
+                        }
+                }
                 __syncwarp();  // every lane has read the stage
                 if (pleft > 0) issue(stage);
             }

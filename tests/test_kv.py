@@ -372,6 +372,17 @@ def test_attend_many_rows_edges(kv, code, dtype):
 
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("window", [0, 1, 33])
+@pytest.mark.parametrize("lens,new,bs,nq,nkv,d", [
+    ([200], [200], 16, 4, 2, 256), ([333, 40], [77, 40], 32, 3, 3, 256), ([150], [9], 64, 1, 1, 256),
+    ([90, 0, 61], [17, 3, 50], 16, 8, 4, 256), ([500], [24], 64, 5, 1, 64), ([260, 7], [12, 7], 16, 12, 4, 128)])
+def test_attend_prompts_on_split_keys(kv, code, dtype, window, lens, new, bs, nq, nkv, d):
+    """Even and odd numbers of row tiles, whose early rows see few of the keys."""
+    run_attend(kv, code, dtype, lens, new, bs, nq, nkv, d, window=window, seed=sum(new), poison=True)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_attend_scores_in_the_hundreds(kv, code, dtype):
     """Scores so far apart that the maximum grows from tile to tile.  A score of size s is a sum of
     128 products whose running sums the tensor cores cut to 24 bits at most 16 times, and is rounded
