@@ -28,9 +28,13 @@ static constexpr int PROMPT_MIN_ROWS = 64, PROMPT_PAIR_ROWS = 256, PROMPT_MIN_CT
 
 #ifdef __CUDACC__
 // The most rows of a request that the split kernel takes when the prompt kernel runs too.  The
-// prompt kernel works on 256 rows per CTA at ten times the split kernel's rate, but does not split
-// the keys: with fewer CTAs than a tenth of the chip the split kernel, which always fills it, is
-// the faster one.  Called by every thread of the CTA; s: a word per warp.
+// prompt kernel works on 256 rows per CTA at several times the split kernel's rate (2048 tokens: 4 to 5
+// times, 8192: 4 to 7), but does not split the keys: with few CTAs the split kernel, which always fills
+// the chip, is the faster one.  Prompt / split in us (B200, 32 heads over 4, 128 wide, bf16):
+//   16 CTAs: 128 tokens 19.8 / 10.9, 128 more on a cache of 8192 152.7 / 127.2
+//   24 CTAs: 192 tokens 21.1 / 20.4, 192 more on a cache of 8192 152.0 / 181.2
+// 64 wide and f32 cross between 12 and 24 too; f32, 128 wide, 16 CTAs on 8192 loses by the rule (138 / 178).
+// Called by every thread of the CTA; s: a word per warp.
 __device__ __forceinline__ int64_t split_max_rows(const AttendArg& a, int heads, int group, int64_t* s) {
     int64_t ctas = 0;
     for (int r = threadIdx.x; r < a.R; r += blockDim.x) {

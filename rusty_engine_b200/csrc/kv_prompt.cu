@@ -20,8 +20,8 @@
 //     tile has its own O in tensor memory, and the other four warps add the tiles up in registers.
 //
 // Measured (B200): 4096 new and 3 decoded tokens over up to 8192 keys, 32 heads over 4 kv heads of
-// 128, bf16, int8 cache: 484 us on changing inputs (465 when one input repeats), 412.6 GFLOP, 852
-// TFLOP/s = 52% of the cuBLAS rate; a 2048-token prompt in f32: 124 us (120), 34.4 GFLOP, 277 TFLOP/s (twice
+// 128, bf16, int8 cache: 482 to 493 us on changing inputs (465 when one input repeats), 412.6 GFLOP, 837 to 856
+// TFLOP/s = 51 to 52% of the cuBLAS rate; a 2048-token prompt in f32: 124 us (120), 34.4 GFLOP, 277 TFLOP/s (twice
 // that with the pairs' products).  No pipe is full (tensor
 // and special functions 47% each in bf16): softmax, P V and the next S of a row tile follow one another, and
 // only the other row tile's work hides them.  More row tiles do not fit: S and O of two fill tensor

@@ -21,16 +21,16 @@
 // A tile of keys that none of an item's rows sees (after a causal prompt's early rows, before a
 // window) is neither fetched nor computed, and early and late row tiles take turns in the numbering, so
 // that the shares stay alike: a prompt of 2048 tokens, 16 heads over 4 of 256, 713 -> 477 us in bf16, 878
-// -> 588 in f32.
+// -> 588 in f32.  The bookkeeping costs two requests of 131071 tokens 0.3 us.
 //
 // Joining.  A share's incomplete first and last items leave (M, l, O) pieces; the CTA joins its
 // warps' pieces, and items that span CTAs go through a workspace slot per CTA, where the last
 // arriving CTA (an atomic count, nobody waits) joins them in CTA order: the result does not depend
 // on timing.
 //
-// Measured (B200, int8 unless said): 32 requests of 2048 to 8192 tokens, bf16: 41.5 us, 171 MB, 4.1
-// TB/s = 63% of the copy rate; 2 requests of 131071 tokens, fp16, e4m3: 45.1 us, 206 MB, 4.6 TB/s; one of
-// 97 tokens, f32: 7.8 us.  DRAM traffic is the algorithmic bytes, the issue slots are 41% busy: what is
+// Measured (B200, int8 unless said): 32 requests of 2048 to 8192 tokens, bf16: 41.3 us, 171 MB, 4.1
+// TB/s = 63% of the copy rate; 2 requests of 131071 tokens, fp16, e4m3: 45.8 us, 206 MB, 4.5 TB/s; one of
+// 97 tokens, f32: 7.9 us.  DRAM traffic is the algorithmic bytes, the issue slots are 41% busy: what is
 // above the floor is latency, the steps before the first tile (lengths, block table and the first copy,
 // one after the other) and the joining at the end.
 #include <algorithm>
@@ -112,6 +112,7 @@ __device__ __forceinline__ SplitItem split_item(int item, int items, int heads) 
 // Keys that some row of the row tile sees: lo .. hi - 1.
 struct SplitKeys { int lo, hi; };
 __device__ __forceinline__ SplitKeys split_keys(const AttendArg& a, const SplitReq& q, int rt, int nr, int group) {
+    if (q.n == 1) return {0, q.hi};  // a decoded token: its tiles begin and end with its keys
     const int first = rt * nr / group, last = min(q.n - 1, (rt * nr + nr - 1) / group);
     return {a.window ? max(0, q.pos0 + first - a.window + 1) : 0, min(q.pos0 + last + 1, q.hi)};
 }
