@@ -12,9 +12,10 @@
 //   16-bit calls: two row tiles share every K / V tile (the widening is paid once for 256 rows);
 //     while one tile's softmax runs, the other's products do.  P goes back to tensor memory as
 //     fp16 over its own S and is the A operand from there.  O stays in tensor memory; it is only
-//     rescaled when a row's maximum grew by more than 2^8 (P then stays below 2^8, exact in
-//     range), by the softmax threads.
-//   f32 calls: q and P are fp16 pairs (hi + lo, twice the products), one row tile, S in two
+//     rescaled when a row's maximum grew by more than 2^LAG, by the softmax threads.
+//     P is carried as 2^UP times itself, so a weight has its 11 bits down to 2^-21 of the row's largest
+//     (2^-29 when M lags behind that).
+//   f32 calls: q and P (2^15 times itself) are fp16 pairs (hi + lo, twice the products), one row tile, S in two
 //     buffers.  The tensor cores cut every partial sum short, about 2^-24 per step and all one
 //     way, which over a long row is more than f32 attention may lose (up to 4.5e-6 measured); so each key
 //     tile has its own O in tensor memory, and the other four warps add the tiles up in registers.
@@ -39,6 +40,11 @@ static constexpr int PKV = 128;   // keys per tile
 template <int D, bool PAIR>
 struct PromptShape {
     static constexpr int NRT = PAIR ? 1 : 2;             // row tiles
+    // M may lag behind a row's maximum by LAG, and the weights are carried as 2^UP times themselves:
+    // together they reach 2^15 at most.  A shorter lag keeps more of small weights but rescales O more
+    // often (4096 new tokens in bf16: 8 466.6 us, 5 482.6, 3 493.7)
+    static constexpr int LAG = PAIR ? 0 : 8, UP = 15 - LAG;
+    static constexpr float DOWN = 1.0f / (1 << UP);
     static constexpr int QB = 128 * D * 2;               // fp16 bytes of a Q, K or V tile
     static constexpr int RAW = PKV * D;
     // operand buffers; f32 has room for three: K's is free again as soon as S is made, V's only after P V
@@ -351,7 +357,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
         const bool live = tok < n;
         T* op = reinterpret_cast<T*>(a.out.p) + (int64_t)(q0 + (live ? tok : 0)) * a.out.st + (int64_t)h * a.out.sh;
         auto finish = [&](int c, const float* v, float l) {  // 32 elements of the row
-            const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+            const float inv = l > 0.0f ? S::DOWN / l : (l == 0.0f ? 0.0f : l);
             float y[32];
 #pragma unroll
             for (int i = 0; i < 32; i++) y[i] = l == 0.0f ? 0.0f : v[i] * inv;
@@ -474,8 +480,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
                     for (int i = 2; i < 16; i++) x[i & 1] = fmaxf(x[i & 1], __uint_as_float(v[g * 16 + i]));
                     mx = fmaxf(mx, fmaf(fmaxf(x[0], x[1]), score_scale(qs, mt.x), mt.y));
                 }
-                // f32: M is the maximum; else it only moves when P could leave 2^8
-                const bool grow = PAIR ? mx > m : mx > m + 8.0f;
+                const bool grow = mx > m + (float)S::LAG;
                 const float mn = grow ? mx : m, mu = mn == -INFINITY ? 0.0f : mn;
                 const float al = grow ? ex2(m - mu) : 1.0f;
                 if (PAIR) {
@@ -501,7 +506,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
 #pragma unroll
                     for (int g = 0; g < 2; g++) {
                         const float4 mt = meta[2 * c + g];
-                        const float sc = score_scale(qs, mt.x), off = mt.y - mu;
+                        const float sc = score_scale(qs, mt.x), off = mt.y - mu + (float)S::UP;
                         const uint64_t sc2 = f2(sc, sc), off2 = f2(off, off);
                         uint64_t sum = 0;
 #pragma unroll
@@ -521,7 +526,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
                         }
                         float x, y;
                         un2(sum, x, y);
-                        l = fmaf(x + y, mt.z, l);
+                        l = fmaf((x + y) * S::DOWN, mt.z, l);
                     }
                     tc::tmem_st16(sp + c * 32, ph);
                     if (PAIR) tc::tmem_st16(sp + c * 32 + 16, pl);

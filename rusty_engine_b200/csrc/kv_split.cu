@@ -4,9 +4,10 @@
 // Mathematics.  With x_j = scale log2(e) ks_j q.kc_j + log2(vs_j) over the keys j that a row sees,
 //   out = sum_j 2^(x_j - M) vc_j / sum_j 2^(x_j - M) / vs_j ,   lse = (M + log2 of that sum) ln 2
 // for any M; M is the running maximum of x_j.  Folding the V scale into the exponent keeps the
-// weights of P V in (0, 1] whatever the scales are, so fp16 holds them; a scale below 2^-100 counts
-// as 2^-100.  Codes are exact in fp16; q is carried as fp16 times a power of two per row, f32
-// calls carry q and the weights as fp16 pairs (hi + lo), and all sums are f32.
+// weights of P V in (0, 1] whatever the scales are; a scale below 2^-100 counts as 2^-100.  Codes are
+// exact in fp16; q is carried as fp16 times a power of two per row and the weights as fp16 times
+// 2^15 (f32 calls: both as pairs, hi + lo), so that a weight has its 11 bits down to 2^-29 of the row's
+// largest (f32 calls: 22 bits down to 2^-18, one less for each factor 2 from there).  All sums are f32.
 //
 // Shape.  A unit of work is a tile of TW tokens of one item (request, kv head, tile of NR rows);
 // rows are a request's new tokens x the query heads that share the kv head.  All units of the call
@@ -556,11 +557,12 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                             }
 #pragma unroll
                             for (int z = 0; z < 2; z++) {
-                                const uint32_t hh = pack_f16x2(p[2 * z], p[2 * z + 1]);
+                                const float x = p[2 * z] * W_UP, y = p[2 * z + 1] * W_UP;
+                                const uint32_t hh = pack_f16x2(x, y);
                                 ph[nt][i][z] = movmatrix(hh);
                                 if (PAIR) {
                                     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hh));
-                                    pl[nt][i][z] = movmatrix(pack_f16x2(p[2 * z] - f.x, p[2 * z + 1] - f.y));
+                                    pl[nt][i][z] = movmatrix(pack_f16x2(x - f.x, y - f.y));
                                 }
                             }
                         }
@@ -633,7 +635,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         const int tok = tok_of(nt * 8 + 2 * c + q);
                         if (tok >= rq.n) continue;
                         const int h = kh * group + row0 + nt * 8 + 2 * c + q - tok * group;
-                        const float inv = l[nt][q] > 0.0f ? 1.0f / l[nt][q] : (l[nt][q] == 0.0f ? 0.0f : l[nt][q]);
+                        const float inv = l[nt][q] > 0.0f ? W_DOWN / l[nt][q] : (l[nt][q] == 0.0f ? 0.0f : l[nt][q]);
                         T* op = reinterpret_cast<T*>(a.out.p) + (int64_t)(rq.q0 + tok) * a.out.st + h * a.out.sh;
 #pragma unroll
                         for (int x = 0; x < BX; x++)
@@ -714,7 +716,7 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         const int rr = pc.row0 + row, tok = rr / group;
         if (tok >= pc.n) return;
         const int h = pc.head * group + rr - tok * group;
-        const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+        const float inv = l > 0.0f ? W_DOWN / l : (l == 0.0f ? 0.0f : l);
         T* op = reinterpret_cast<T*>(a.out.p) + (int64_t)(pc.q0 + tok) * a.out.st + (int64_t)h * a.out.sh + lane * VE;
         T y[VE];
 #pragma unroll

@@ -60,6 +60,12 @@ __device__ __forceinline__ int q_exponent(float mx) {
     return mx > 0.0f && mx <= 3.4e38f ? max(-126, min(113, ex)) : 0;
 }
 
+// The weights p = 2^(x - M) of a row go to the tensor cores as fp16, whose smallest step is 2^-24 and
+// whose largest value is 2^16: they are carried as p times a power of two, which the output is divided
+// by again.  Carried as p itself, the keys behind a dominant one were lost where its value is near 0 (4096
+// keys 14 nats below it: 2e-4 of an f32 output, all of it from 20 nats on; times 2^15: 1e-9 and 3e-7).
+static constexpr float W_UP = 32768.0f, W_DOWN = 1.0f / 32768.0f;
+
 static constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.69314718055994531f;
 
 }  // namespace rmoe

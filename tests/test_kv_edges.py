@@ -1,0 +1,49 @@
+"""Edges of the paged 8-bit KV cache operators (rusty_engine_b200.kv) on the GPU, against
+tests/kv_ref.py, with the tolerances of tests/test_kv.py unless a test derives its own."""
+import numpy as np
+import pytest
+import torch
+
+import kv_ref as R
+from test_kv import REL, ints, kv, rel, slots_of  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- a dominant key -----------------------------------------------------------------------------
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("at", [0, 700])
+@pytest.mark.parametrize("lens,new,nq,nkv,d", [
+    ([1500], [1], 8, 2, 128), ([1500, 1300], [1, 3], 16, 2, 64), ([1400], [2], 4, 1, 256),
+    ([1550], [200], 32, 8, 128), ([1550], [200], 32, 8, 64)])
+def test_attend_beside_a_dominant_key(kv, code, dtype, at, lens, new, nq, nkv, d):
+    """A key that takes nearly all of every row's weight while its value is 0: the output is what
+    the other keys, 14 (f32) or 17 nats below, add up to.  f32: the deepest weight is 2^-22 of the
+    row's largest; carried as 2^15 times itself in two fp16 it is off by at most 2^-25 / 2^-7, beside
+    the 20 * 2^-22 of the scores: 1e-5 holds.  16 bits: weights of 2^-24.5 of the largest, carried
+    as 2^7 times themselves, are rounded by at most 2^-25 each, the roundings of 1300 keys being
+    independent: 2^-7.5 / sqrt(3 * 1300) = 1e-4 of the sum; 2^-11 is five times that."""
+    depth, bs, g = (14.0 if dtype == "f32" else 17.0), 64, torch.Generator().manual_seed(d + at)
+    _, _, table = slots_of(lens, [0] * len(lens), bs, blocks := sum(-(-n // bs) for n in lens))
+    u = torch.randint(0, 2, (nkv, d), generator=g) * 2.0 - 1.0
+    k = torch.randint(-20, 21, (blocks, nkv, bs, d), generator=g).float()
+    v = (64 + 25 * torch.randn((blocks, nkv, bs, d), generator=g)).round().clamp(-127, 127)
+    for row in table:
+        k[row[at // bs], :, at % bs] = 60 * u
+        v[row[at // bs], :, at % bs] = 0
+    dt = torch.int8 if code == "int8" else torch.float8_e4m3fn
+    k, v = k.to(dt), v.to(dt)
+    ks, vs = torch.full((blocks, nkv), 1 / 60), torch.full((blocks, nkv), 1 / 64)
+    c = kv.KVCache.from_buffers(k.cuda(), v.cuda(), ks.cuda(), vs.cuda())
+    T = sum(new)
+    q = (u.repeat_interleave(nq // nkv, 0) + 0.1 * torch.randn((T, nq, d), generator=g)).to(R.DT[dtype])
+    cu, scale = np.concatenate(([0], np.cumsum(new))).tolist(), float(np.float32(depth / d))
+    mb = max(len(t) for t in table)
+    out, lse = c.attend(q.cuda(), ints([t + [-1] * (mb - len(t)) for t in table]), ints(lens), ints(cu), scale=scale,
+                        max_new=max(new), return_lse=True)
+    want, wl = R.attend(q, k.float(), v.float(), ks, vs, table, lens, cu, scale)
+    e = rel(out, want)
+    print(f"dominant key {code} {dtype} d {d} new {new}: rel-L2 {e:.2e}")
+    assert e <= REL[dtype] + (0.0 if dtype == "f32" else 2.0 ** -11), e
+    assert (lse.cpu().double() - wl).abs().max().item() <= 2e-5
