@@ -66,8 +66,10 @@ rmoe_status rmoe_kv_create(const rmoe_kv_desc* d, rmoe_kv** out) {
         if (ok && e == cudaSuccess) e = cudaMemset(kv->v, 0, bytes);
         if (ok && e == cudaSuccess) e = cudaMemset(kv->ks, 0, sb);
         if (ok && e == cudaSuccess) e = cudaMemset(kv->vs, 0, sb);
-        if (ok && e == cudaSuccess) e = cudaDeviceSynchronize();
     }
+    // a memset does not wait for the device, and non-blocking streams do not wait for its stream: the
+    // first call on one of those must not overtake it
+    if (ok && e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);
     if (!ok || e != cudaSuccess) {
         delete kv;
         cudaGetLastError();

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import kv_ref as R
-from test_kv import REL, ints, kv, rel, slots_of  # noqa: F401
+from test_kv import REL, cache_of, ints, kv, rel, slots_of  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +47,27 @@ def test_attend_beside_a_dominant_key(kv, code, dtype, at, lens, new, nq, nkv, d
     print(f"dominant key {code} {dtype} d {d} new {new}: rel-L2 {e:.2e}")
     assert e <= REL[dtype] + (0.0 if dtype == "f32" else 2.0 ** -11), e
     assert (lse.cpu().double() - wl).abs().max().item() <= 2e-5
+
+
+def test_a_new_cache_on_another_stream(kv):
+    """A cache made and used on a side stream while the default stream is busy, 20 times over memory
+    that the caches before it have used: its join counts are zeroed before its first call."""
+    c, *_ = cache_of(kv, "int8", 300, 2, 64, 128)
+    k, v, ks, vs = c.k, c.v, c.k_scale, c.v_scale
+    g = torch.Generator(device="cuda").manual_seed(4)
+    q = torch.randn((2, 16, 128), generator=g, device="cuda")
+    args = (q, ints([list(range(0, 150)), list(range(150, 300))]), ints([9500, 9000]), ints([0, 1, 2]))
+    want = c.attend(*args)
+    busy = torch.randn((4096, 4096), device="cuda")
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i in range(20):
+        for _ in range(5):
+            busy = (busy @ busy).clamp_(-1, 1)
+        with torch.cuda.stream(s):
+            other = kv.KVCache.from_buffers(k, v, ks, vs)
+            got = other.attend(*args)
+        s.synchronize()
+        assert torch.equal(got, want), i
+        other.check()
+        other.close()
