@@ -282,7 +282,12 @@ RMOE_API rmoe_status rmoe_gguf_moe_layer_desc(rmoe_gguf* g, uint32_t block, rmoe
  *
  * Element types of q / k / v / out are ggml codes: RMOE_GGML_F32, _F16 or _BF16.  All tensors
  * below are device memory of the handle's device; every call is stream-ordered and waits for
- * nothing.  rusty-engine's PagedKvCache (src/infer.rs:328) holds f32 rows and is not read by its
+ * nothing.  Calls on one cache may come on several streams: what they read and write of the cache's
+ * memory is then the caller's to order, as for any memory.  rmoe_kv_attend only reads it, and calls
+ * of it on different streams may overlap: each stream has a workspace of its own, allocated at
+ * its first call (2.5 MB with head_dim 128; from the 65th stream on a call may wait for the
+ * device).  Calls that a stream captures share another one: of graphs that were captured on the same
+ * stream and attend over the same cache, one may run at a time.  rusty-engine's PagedKvCache (src/infer.rs:328) holds f32 rows and is not read by its
  * forward; its attention (src/forward.rs:218-283) and RoPE (src/infer.rs:90-145) are the formulas
  * these calls compute, over a cache held in 8 bits. */
 

@@ -3,6 +3,32 @@
 
 #include "kv_attend.h"
 
+namespace rmoe {
+
+cudaError_t add_split_slot(rmoe_kv* kv) {
+    const size_t bytes = kv->sms * split_part_bytes((int)kv->dim);
+    // allowed while this or another thread captures a graph: nothing here belongs into one
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return e;
+    char* p = nullptr;
+    cudaStream_t s = nullptr;
+    e = cudaMalloc(&p, bytes + kv->sms * 4);
+    // on a stream of its own, so that nothing queued elsewhere is waited for
+    if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMemsetAsync(p + bytes, 0, kv->sms * 4, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    if (s) cudaStreamDestroy(s);
+    if (e == cudaSuccess)
+        kv->slots[kv->n_slots++] = SplitSlot{SplitSlot::FREE, 0, SplitWs{(float*)p, (unsigned*)(p + bytes)}};
+    else
+        cudaFree(p);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    return e;
+}
+
+}  // namespace rmoe
+
 using namespace rmoe;
 
 extern "C" {
@@ -46,11 +72,8 @@ rmoe_status rmoe_kv_create(const rmoe_kv_desc* d, rmoe_kv** out) {
     const uint64_t bytes = rows * d->head_dim, sb = (uint64_t)d->n_blocks * d->n_kv_heads * 4;
     cudaDeviceGetAttribute(&kv->sms, cudaDevAttrMultiProcessorCount, d->device);
     kv->status = (unsigned*)kv->own.alloc(16);
-    kv->split_part = (float*)kv->own.alloc(kv->sms * split_part_bytes((int)kv->dim));
-    kv->split_ticket = (unsigned*)kv->own.alloc(kv->sms * 4);
-    bool ok = kv->status && kv->split_part && kv->split_ticket;
+    bool ok = kv->status && add_split_slot(kv) == cudaSuccess;
     cudaError_t e = ok ? cudaMemset(kv->status, 0, 16) : cudaSuccess;
-    if (ok && e == cudaSuccess) e = cudaMemset(kv->split_ticket, 0, kv->sms * 4);
     if (given) {
         kv->k = (uint8_t*)d->k;
         kv->v = (uint8_t*)d->v;

@@ -6,6 +6,51 @@
 
 using namespace rmoe;
 
+// The workspace for a call on stream s.
+static rmoe_status split_ws(rmoe_kv* kv, cudaStream_t s, SplitWs& ws) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    cudaError_t e = cudaStreamIsCapturing(s, &cap);
+    const SplitSlot::Use use = cap == cudaStreamCaptureStatusNone ? SplitSlot::CALLS : SplitSlot::GRAPHS;
+    // while it captures, a stream may not be asked for its id
+    if (use == SplitSlot::GRAPHS) id = reinterpret_cast<uintptr_t>(s);
+    else if (e == cudaSuccess) e = cudaStreamGetId(s, &id);
+    if (e != cudaSuccess) return cuda_fail(e, "kv attend stream");
+    const std::lock_guard<std::mutex> lock(kv->slots_mu);
+    SplitSlot* free_slot = nullptr;
+    auto look = [&]() -> SplitSlot* {
+        for (int i = 0; i < kv->n_slots; i++) {
+            if (kv->slots[i].use == use && kv->slots[i].stream == id) return &kv->slots[i];
+            if (kv->slots[i].use == SplitSlot::FREE) free_slot = &kv->slots[i];
+        }
+        return nullptr;
+    };
+    SplitSlot* slot = look();
+    if (!slot && !free_slot && kv->n_slots < MAX_SPLIT_SLOTS) {
+        if ((e = add_split_slot(kv)) != cudaSuccess) {
+            cudaGetLastError();
+            return fail(RMOE_ERR_OOM, "kv attend: workspace for another stream: %s", cudaGetErrorString(e));
+        }
+        look();
+    }
+    if (!slot && !free_slot && use == SplitSlot::CALLS) {
+        // every slot is taken: once the device is done, those of plain calls are free again
+        if ((e = cudaDeviceSynchronize()) != cudaSuccess) return cuda_fail(e, "kv attend");
+        for (int i = 0; i < kv->n_slots; i++)
+            if (kv->slots[i].use == SplitSlot::CALLS) kv->slots[i].use = SplitSlot::FREE;
+        look();
+    }
+    if (!slot) {
+        if (!free_slot)
+            return fail(RMOE_ERR_UNSUPPORTED, "kv attend: calls on one cache from more than %d streams", MAX_SPLIT_SLOTS);
+        slot = free_slot;
+        slot->use = use;
+        slot->stream = id;
+    }
+    ws = slot->ws;
+    return RMOE_OK;
+}
+
 extern "C" rmoe_status rmoe_kv_attend(rmoe_kv* kv, const rmoe_kv_attend_args* a, void* stream) {
     if (!kv || !a) return fail(RMOE_ERR_INVALID, "null cache / arguments");
     if (!elt_ok(a->type)) return fail(RMOE_ERR_UNSUPPORTED, "kv attend: ggml type %u (F32, F16 or BF16)", a->type);
@@ -38,11 +83,13 @@ extern "C" rmoe_status rmoe_kv_attend(rmoe_kv* kv, const rmoe_kv_attend_args* a,
     const uint64_t longest = std::min<uint64_t>(a->max_new ? a->max_new : a->T > a->R ? a->T : 1, a->T);
     p.prompts = kv->dim <= 128 && longest * group >= PROMPT_MIN_ROWS &&
                 (a->T * group / PROMPT_PAIR_ROWS + std::min(a->R, a->T)) * kv->heads >= PROMPT_MIN_CTAS;
+    SplitWs ws{};
+    if ((st = split_ws(kv, s, ws))) return st;
     cudaError_t e = p.prompts ? launch_prompt(kv->prompt_maps, ka, p, a->type, (int)kv->code, s) : cudaSuccess;
     // 16 rows per item where a request has more than 8 on average: the cache is read once for them
     const uint64_t mean = group * (p.prompts ? 1 : (a->T + a->R - 1) / a->R);
     const int nr = mean > 8 && kv->dim <= 128 ? 16 : 8;
     if (e == cudaSuccess)
-        e = launch_split(kv->split_maps, ka, p, SplitWs{kv->split_part, kv->split_ticket}, kv->sms, nr, a->type, (int)kv->code, s);
+        e = launch_split(kv->split_maps, ka, p, ws, kv->sms, nr, a->type, (int)kv->code, s);
     return e == cudaSuccess ? RMOE_OK : cuda_fail(e, "kv attend launch");
 }

@@ -16,12 +16,8 @@ struct AttendArg {
     bool prompts;  // the prompt kernel runs too and takes the requests of more than split_max_rows rows
 };
 
-// Workspace of the split kernel: two (M, l, O) pieces per CTA, and a count per CTA that is 0
-// between calls.
-struct SplitWs {
-    float* part;
-    unsigned* ticket;
-};
+// Adds a workspace to the cache, its counts zeroed when this returns.
+cudaError_t add_split_slot(rmoe_kv* kv);
 
 // Rows of a request: its new tokens x the query heads that share a kv head.
 static constexpr int PROMPT_MIN_ROWS = 64, PROMPT_PAIR_ROWS = 256, PROMPT_MIN_CTAS = 24;

@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <mutex>
 
 #include "layer_impl.h"
 
@@ -19,6 +20,23 @@ namespace rmoe {
 struct KvMaps {
     CUtensorMap k, v;  // the codes as rows of head_dim bytes (make_code_map)
 };
+
+// Workspace of the split kernel: two (M, l, O) pieces per CTA, and a count per CTA that is 0
+// between calls.
+struct SplitWs {
+    float* part;
+    unsigned* ticket;
+};
+
+// The workspaces of a cache.  Calls on one stream follow one another and share one; calls on
+// different streams may run at the same time and have one each.  So have the calls that a stream
+// captures: their graph may run beside the stream's own later calls.
+struct SplitSlot {
+    enum Use { FREE, CALLS, GRAPHS } use;
+    unsigned long long stream;  // CALLS: its id, which no later stream of the process gets; GRAPHS: its handle
+    SplitWs ws;                 // one allocation, at part
+};
+static constexpr int MAX_SPLIT_SLOTS = 64;
 }  // namespace rmoe
 
 struct rmoe_kv {
@@ -30,9 +48,15 @@ struct rmoe_kv {
     rmoe::KvMaps split_maps{};     // boxes of a split-kernel tile
     rmoe::KvMaps prompt_maps{};    // boxes of a prompt-kernel tile: a block
     int sms = 0;
-    float* split_part = nullptr;   // split kernel: pieces of items that span CTAs
-    unsigned* split_ticket = nullptr;
+    std::mutex slots_mu;
+    rmoe::SplitSlot slots[rmoe::MAX_SPLIT_SLOTS]{};
+    int n_slots = 0;
     rmoe::Owned own;
+
+    rmoe_kv() = default;
+    ~rmoe_kv() {
+        for (int i = 0; i < n_slots; i++) cudaFree(slots[i].ws.part);
+    }
 };
 
 namespace rmoe {

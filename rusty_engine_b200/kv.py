@@ -277,6 +277,8 @@ class KVCache:
         blocks table[r], has the queries cu[r] .. cu[r + 1) at its last positions.  Causal; with a
         window, each query sees that many keys at most.  scale: 1 / sqrt(head_dim) by default.
         max_new: an upper bound of any request's new tokens, where known (chooses kernels only).
+        Only reads the cache: calls on different streams may overlap (each stream has a workspace of
+        its own; of graphs captured on the same stream one may run at a time).
         Returns out (as q), or (out, lse [tokens, q heads] f32)."""
         if stream is not None:
             with _on(stream, q, table, lens, cu, out):

@@ -71,3 +71,71 @@ def test_a_new_cache_on_another_stream(kv):
         assert torch.equal(got, want), i
         other.check()
         other.close()
+
+
+def test_attend_on_several_streams_at_once(kv):
+    """Long contexts (whose pieces are joined through a workspace) on several streams of one cache at
+    the same time, beside graphs that two streams captured: bit for bit what one call alone gives."""
+    c, *_ = cache_of(kv, "int8", 400, 2, 64, 128)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    cases = []
+    for i in range(4):
+        q = torch.randn((2 + 100 * (i == 3), 16, 128), generator=g, device="cuda")
+        tab = ints([list(range(i, 180 + i)), list(range(200 - i, 380 - i))])
+        lens, cu = ints([11500 - 700 * i, 9000]), ints([0, 1, q.shape[0]])
+        cases.append((q, tab, lens, cu))
+    want = [c.attend(*a) for a in cases]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    graphs, outs = [], []
+    for a, s in zip(cases[:2], streams):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            outs.append(c.attend(*a))
+        graphs.append(graph)
+    replayers = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for i in range(30):
+        got = [c.attend(*cases[(i + j) % 4], stream=s) for j, s in enumerate(streams)]
+        for graph, s in zip(graphs, replayers):
+            with torch.cuda.stream(s):
+                graph.replay()
+        here = c.attend(*cases[i % 4])
+        torch.cuda.synchronize()
+        for j, x in enumerate(got):
+            assert torch.equal(x, want[(i + j) % 4]), (i, j)
+        assert torch.equal(here, want[i % 4]) and all(torch.equal(x, w) for x, w in zip(outs, want))
+    c.check()
+
+
+def test_attend_on_more_streams_than_workspaces(kv):
+    """Streams that come and go, through the C entry: more than a cache keeps workspaces for, some
+    destroyed so that their handles are used again."""
+    import ctypes as C
+
+    from rusty_engine_b200 import _lib
+
+    c, *_ = cache_of(kv, "int8", 200, 2, 64, 128)
+    q, out = torch.randn((2, 16, 128), device="cuda"), torch.zeros((2, 16, 128), device="cuda")
+    tab, lens, cu = ints([list(range(0, 90)), list(range(100, 190))]), ints([5700, 5000]), ints([0, 1, 2])
+    want = c.attend(q, tab, lens, cu)
+    rows = lambda t: (t.data_ptr(), 16 * 128, 128, 16, 0)  # noqa: E731
+    args = _lib.KV_ATTEND_ARGS.pack(*rows(q), *rows(out), tab.data_ptr(), lens.data_ptr(), cu.data_ptr(), 0, 2, 90, 2,
+                                    0, float(np.float32(1 / np.sqrt(128))), 0, 1, 0)
+    rt = C.CDLL("libcudart.so.12")
+    torch.cuda.synchronize()
+    kept = []
+    for i in range(150):
+        h = C.c_void_p()
+        assert rt.cudaStreamCreateWithFlags(C.byref(h), 1) == 0
+        assert _lib.load().rmoe_kv_attend(c._h, args, h) == _lib.RMOE_OK, _lib.load().rmoe_last_error()
+        assert rt.cudaStreamSynchronize(h) == 0
+        assert torch.equal(out, want), i
+        out.zero_()
+        torch.cuda.synchronize()
+        if i % 3:
+            kept.append(h)
+        else:
+            assert rt.cudaStreamDestroy(h) == 0
+    for h in kept:
+        assert rt.cudaStreamDestroy(h) == 0
+    c.check()
