@@ -129,6 +129,7 @@ rmoe_status rmoe_kv_status(rmoe_kv* kv) {
     cudaError_t e = cudaDeviceSynchronize();
     if (e == cudaSuccess) e = cudaMemcpy(&hs, kv->status, 4, cudaMemcpyDeviceToHost);
     if (e == cudaSuccess && hs) e = cudaMemset(kv->status, 0, 4);
+    if (e == cudaSuccess && hs) e = cudaStreamSynchronize(cudaStreamLegacy);  // or it could clear a later call's error
     if (e != cudaSuccess) return cuda_fail(e, "cache status");
     if (hs)
         return fail(RMOE_ERR_DEVICE, "kv cache: device status 0x%x%s%s%s", hs,

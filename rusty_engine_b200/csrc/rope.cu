@@ -354,6 +354,7 @@ rmoe_status rmoe_rope_status(rmoe_rope* r) {
     cudaError_t e = cudaDeviceSynchronize();
     if (e == cudaSuccess) e = cudaMemcpy(&hs, r->status, 4, cudaMemcpyDeviceToHost);
     if (e == cudaSuccess && hs) e = cudaMemset(r->status, 0, 4);
+    if (e == cudaSuccess && hs) e = cudaStreamSynchronize(cudaStreamLegacy);  // or it could clear a later call's error
     if (e != cudaSuccess) return cuda_fail(e, "rope status");
     if (hs) return fail(RMOE_ERR_DEVICE, "rope: device status 0x%x (a position outside the table)", hs);
     return RMOE_OK;

@@ -139,3 +139,24 @@ def test_attend_on_more_streams_than_workspaces(kv):
     for h in kept:
         assert rt.cudaStreamDestroy(h) == 0
     c.check()
+
+
+def test_errors_right_after_a_check_are_kept(kv):
+    """Errors on a stream that does not wait for the default one, each met right after the check that
+    cleared the one before."""
+    from rusty_engine_b200._lib import RmoeError
+
+    c, rope = kv.KVCache(2, 16, 1, 64), kv.Rope(kv.RopeConfig(64), 10)
+    x, far = torch.randn((1, 1, 64), device="cuda"), ints([64])
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    for _ in range(50):
+        with torch.cuda.stream(s):
+            c.append(x, x, far)
+            rope.apply(x, far)
+        with pytest.raises(RmoeError, match="out of range"):
+            c.check()
+        with pytest.raises(RmoeError, match="position"):
+            rope.check()
+    c.check()
+    rope.check()
