@@ -395,7 +395,8 @@ RMOE_API void rmoe_kv_destroy(rmoe_kv* kv);
 /* The memory in use (desc->k, v, k_scale, v_scale are filled). */
 RMOE_API rmoe_status rmoe_kv_buffers(const rmoe_kv* kv, rmoe_kv_desc* desc);
 /* Device errors of the calls so far (a slot, block or position out of range, a K / V value that is
- * not finite, a timed-out wait); synchronises with the device and clears the word. */
+ * not finite, a timed-out wait); synchronises with the device and clears the word.  After a timed-out
+ * wait, attention results are wrong until this call has reported it. */
 RMOE_API rmoe_status rmoe_kv_status(rmoe_kv* kv);
 
 /* Writes T tokens' keys and values at slots[t] (-1: skipped).  Tokens of one block are given as
@@ -445,6 +446,10 @@ RMOE_API rmoe_status rmoe_kv_attend(rmoe_kv* kv, const rmoe_kv_attend_args* args
  * Returns RMOE_ERR_DEVICE with the timeout in the message (what a product call whose wait ran
  * out reports); the context stays usable.  RMOE_ERR_CUDA for any other outcome. */
 RMOE_API rmoe_status rmoe_selftest_bounded_wait(int32_t device, uint32_t limit_us);
+/* Self-test of the recovery after such a wait in rmoe_kv_attend (no counterpart in the reference):
+ * leaves the cache's workspaces and status word as a call does whose waits ran out.  The next
+ * rmoe_kv_status reports it, and calls after that are right again. */
+RMOE_API rmoe_status rmoe_selftest_kv_lost_wait(rmoe_kv* kv);
 
 /* Build info: "sm_100a <git-describe> <kernels...>". */
 RMOE_API const char* rmoe_build_info(void);

@@ -83,6 +83,7 @@ EXPORTS = [
     "rmoe_route_grouped", "rmoe_qmat_create", "rmoe_qmat_forward", "rmoe_qmat_status", "rmoe_qmat_destroy",
     "rmoe_gguf_open", "rmoe_gguf_close", "rmoe_gguf_tensor", "rmoe_gguf_meta_uint", "rmoe_gguf_moe_layer_desc",
     "rmoe_layer_router_refined", "rmoe_noalloc_status", "rmoe_selftest_bounded_wait",
+    "rmoe_selftest_kv_lost_wait",
     "rmoe_rope_create", "rmoe_rope_destroy", "rmoe_rope_apply", "rmoe_rope_status",
     "rmoe_kv_create", "rmoe_kv_destroy", "rmoe_kv_buffers", "rmoe_kv_status", "rmoe_kv_extend", "rmoe_kv_release",
     "rmoe_kv_append", "rmoe_kv_read", "rmoe_kv_attend",
@@ -113,6 +114,7 @@ def load():
         L.rmoe_layer_router_refined.argtypes = [vp, vp]
         L.rmoe_noalloc_status.argtypes = [i32]
         L.rmoe_selftest_bounded_wait.argtypes = [i32, u32]
+        L.rmoe_selftest_kv_lost_wait.argtypes = [vp]
         L.rmoe_layer_destroy.argtypes = [vp]
         L.rmoe_layer_destroy.restype = None
         L.rmoe_last_error.restype = C.c_char_p

@@ -129,6 +129,11 @@ rmoe_status rmoe_kv_status(rmoe_kv* kv) {
     cudaError_t e = cudaDeviceSynchronize();
     if (e == cudaSuccess) e = cudaMemcpy(&hs, kv->status, 4, cudaMemcpyDeviceToHost);
     if (e == cudaSuccess && hs) e = cudaMemset(kv->status, 0, 4);
+    if (hs & DERR_TIMEOUT) {
+        // CTAs of a call whose waits ran out may not have been counted: the next call starts from 0 again
+        const std::lock_guard<std::mutex> lock(kv->slots_mu);
+        for (int i = 0; i < kv->n_slots && e == cudaSuccess; i++) e = cudaMemset(kv->slots[i].ws.ticket, 0, kv->sms * 4);
+    }
     if (e == cudaSuccess && hs) e = cudaStreamSynchronize(cudaStreamLegacy);  // or it could clear a later call's error
     if (e != cudaSuccess) return cuda_fail(e, "cache status");
     if (hs)
@@ -137,6 +142,18 @@ rmoe_status rmoe_kv_status(rmoe_kv* kv) {
                     (hs & DERR_NONFINITE) ? " (a key or value that is not finite)" : "",
                     (hs & DERR_TIMEOUT) ? " (a bounded wait ran out)" : "");
     return RMOE_OK;
+}
+
+rmoe_status rmoe_selftest_kv_lost_wait(rmoe_kv* kv) {
+    if (!kv) return fail(RMOE_ERR_INVALID, "null cache");
+    DeviceGuard g(kv->device);
+    const std::lock_guard<std::mutex> lock(kv->slots_mu);
+    const unsigned hs = DERR_TIMEOUT;
+    cudaError_t e = cudaDeviceSynchronize();
+    for (int i = 0; i < kv->n_slots && e == cudaSuccess; i++) e = cudaMemset(kv->slots[i].ws.ticket, 1, kv->sms * 4);
+    if (e == cudaSuccess) e = cudaMemcpy(kv->status, &hs, 4, cudaMemcpyHostToDevice);
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    return e == cudaSuccess ? RMOE_OK : cuda_fail(e, "kv self-test");
 }
 
 }  // extern "C"

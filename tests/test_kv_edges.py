@@ -160,3 +160,24 @@ def test_errors_right_after_a_check_are_kept(kv):
             rope.check()
     c.check()
     rope.check()
+
+
+def test_attend_is_right_again_after_a_lost_wait(kv):
+    """Counts that a call left behind whose waits ran out: reported by check(), and gone after it."""
+    from rusty_engine_b200 import _lib
+
+    c, *_ = cache_of(kv, "int8", 400, 2, 64, 128)
+    q = torch.randn((2, 16, 128), device="cuda")
+    args = (q, ints([list(range(0, 180)), list(range(200, 380))]), ints([11500, 9000]), ints([0, 1, 2]))
+    s = torch.cuda.Stream()
+    want = c.attend(*args)
+    torch.cuda.synchronize()
+    assert torch.equal(c.attend(*args, stream=s), want)
+    for _ in range(2):
+        assert _lib.load().rmoe_selftest_kv_lost_wait(c._h) == _lib.RMOE_OK
+        with pytest.raises(_lib.RmoeError, match="bounded wait"):
+            c.check()
+        got = c.attend(*args), c.attend(*args, stream=s), c.attend(*args)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, want) for x in got)
+        c.check()
