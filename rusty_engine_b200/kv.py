@@ -129,7 +129,12 @@ class Rope:
         if stream is not None:
             with _on(stream, q, positions, k, out, k_out):
                 return self.apply(q, positions, k, out=out, k_out=k_out, inverse=inverse)
-        return self._apply(self._p, self.device, q, positions, k, out, k_out, inverse)
+        return self._apply(self._open(), self.device, q, positions, k, out, k_out, inverse)
+
+    def _open(self):
+        if not self._p:  # 0 would be taken for "no rope"
+            raise EngineError("the rope is closed")
+        return self._p
 
     def check(self):
         """Raises if a call so far met a position outside the table (synchronises)."""
@@ -258,8 +263,8 @@ class KVCache:
         if stream is not None:
             with _on(stream, k, v, slots, positions, q, q_out):
                 return self.append(k, v, slots, rope=rope, positions=positions, q=q, q_out=q_out)
-        return self._append(self._p, self.device, self.n_kv_heads, self.head_dim, k, v, slots, 0 if rope is None else rope._p,
-                            positions, q, q_out)
+        return self._append(self._open(), self.device, self.n_kv_heads, self.head_dim, k, v, slots,
+                            0 if rope is None else rope._open(), positions, q, q_out)
 
     def read(self, slots, dtype=None, *, stream=None):
         """(k, v) of cached tokens [slots, n_kv_heads, head_dim], code * scale, as `dtype` (float32)."""
@@ -269,7 +274,7 @@ class KVCache:
         if stream is not None:
             with _on(stream, slots):
                 return self.read(slots, dtype)
-        return self._read(self._p, self.k, slots, like)
+        return self._read(self._open(), self.k, slots, like)
 
     def attend(self, q, table, lens, cu, *, scale: Optional[float] = None, window: int = 0, max_new: Optional[int] = None,
                out=None, return_lse: bool = False, stream=None):
@@ -284,8 +289,13 @@ class KVCache:
             with _on(stream, q, table, lens, cu, out):
                 return self.attend(q, table, lens, cu, scale=scale, window=window, max_new=max_new, out=out,
                                    return_lse=return_lse)
-        return self._attend(self._p, self.device, self.head_dim, q, table, lens, cu, self._scale if scale is None else scale,
+        return self._attend(self._open(), self.device, self.head_dim, q, table, lens, cu, self._scale if scale is None else scale,
                             window, max_new or 0, out, return_lse)
+
+    def _open(self):
+        if not self._p:
+            raise EngineError("the cache is closed")
+        return self._p
 
     def check(self):
         """Raises if a call so far met a device error (synchronises and clears it)."""

@@ -181,3 +181,22 @@ def test_attend_is_right_again_after_a_lost_wait(kv):
         torch.cuda.synchronize()
         assert all(torch.equal(x, want) for x in got)
         c.check()
+
+
+# ---- handles ------------------------------------------------------------------------------------
+def test_a_closed_rope_is_refused(kv):
+    """Not taken for "no rope", which would write the keys unturned."""
+    c = kv.KVCache(2, 16, 1, 64)
+    rope = kv.Rope(kv.RopeConfig(64), 32)
+    x, slots = torch.randn((3, 1, 64), device="cuda"), ints([0, 1, 2])
+    rope.close()
+    before = c.k.clone()
+    for call in (lambda: c.append(x, x, slots, rope=rope, positions=slots), lambda: rope.apply(x, slots),
+                 lambda: c.append(x, x, slots, rope=rope, positions=slots, q=x)):
+        with pytest.raises(kv.EngineError, match="closed"):
+            call()
+    assert torch.equal(c.k, before)
+    c.close()
+    for call in (lambda: c.append(x, x, slots), lambda: c.read(slots), lambda: c.attend(x, ints([[0]]), ints([3]), ints([0, 3]))):
+        with pytest.raises(kv.EngineError, match="closed"):
+            call()
