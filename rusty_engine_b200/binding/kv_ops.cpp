@@ -101,6 +101,12 @@ double real(PyObject* o) {
     return v;
 }
 
+bool truth(PyObject* o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw Raised();
+    return v != 0;
+}
+
 // The calls run on the current stream, where their outputs are allocated too.
 void* stream_of(int64_t device) { return (void*)c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream(); }
 
@@ -158,7 +164,7 @@ PyObject* rope_apply(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         r.T = (uint32_t)q.size(0);
         r.head_dim = (uint32_t)q.size(2);
         r.positions = ints(pos, "positions", dev, q.size(0));
-        r.inverse = integer(a[7]) != 0;
+        r.inverse = truth(a[7]);
         check(rmoe_rope_apply((rmoe_rope*)integer(a[0]), &r, stream_of(dev)));
         return ko.defined() ? pair(out, ko) : THPVariable_Wrap(out);
     });
@@ -289,7 +295,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         r.table = ints(table, "table", dev);
         r.lens = ints(lens, "lens", dev, R);
         r.cu = ints(cu, "cu", dev, R + 1);
-        if (a[11] == Py_True) {
+        if (truth(a[11])) {
             lse = at::empty({T, q.size(1)}, q.options().dtype(at::kFloat));
             r.lse = lse.data_ptr<float>();
         }

@@ -200,3 +200,13 @@ def test_a_closed_rope_is_refused(kv):
     for call in (lambda: c.append(x, x, slots), lambda: c.read(slots), lambda: c.attend(x, ints([[0]]), ints([3]), ints([0, 3]))):
         with pytest.raises(kv.EngineError, match="closed"):
             call()
+
+
+def test_return_lse_takes_any_truth_value(kv):
+    c, *_ = cache_of(kv, "int8", 4, 2, 16, 64)
+    q = torch.randn((2, 4, 64), device="cuda")
+    for yes in (True, 1, np.True_):
+        out, lse = c.attend(q, ints([[0, 1]]), ints([20]), ints([0, 2]), return_lse=yes)
+        assert out.shape == q.shape and lse.shape == (2, 4)
+    for no in (False, 0, np.False_, None):
+        assert c.attend(q, ints([[0, 1]]), ints([20]), ints([0, 2]), return_lse=no).shape == q.shape
