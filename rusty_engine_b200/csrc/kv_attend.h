@@ -23,6 +23,9 @@ cudaError_t add_split_slot(rmoe_kv* kv);
 static constexpr int PROMPT_MIN_ROWS = 64, PROMPT_PAIR_ROWS = 256, PROMPT_MIN_CTAS = 24;
 
 #ifdef __CUDACC__
+// The first key that the query at position p sees (p may be negative, the window up to 2^31 - 1).
+__device__ __forceinline__ int first_seen(int window, int p) { return window && p >= window ? p - window + 1 : 0; }
+
 // The most rows of a request that the split kernel takes when the prompt kernel runs too.  The
 // prompt kernel works on 256 rows per CTA at several times the split kernel's rate (2048 tokens: 4 to 5
 // times, 8192: 4 to 7), but does not split the keys: with few CTAs the split kernel, which always fills

@@ -146,7 +146,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     const int len = __ldg(a.lens + r), pos0 = len - (__ldg(a.cu + r + 1) - __ldg(a.cu + r));
     const int hi = (int)min((int64_t)max(len, 0), (int64_t)a.max_blocks * bs);
     const int tok_last = min(n - 1, (row0 + NRT * 128 - 1) / group);
-    const int kmax = min(pos0 + tok_last + 1, hi), kmin = a.window ? max(0, pos0 + row0 / group - a.window + 1) : 0;
+    const int kmax = min(pos0 + tok_last + 1, hi), kmin = first_seen(a.window, pos0 + row0 / group);
     const int jt0 = kmin / PKV, nt = kmax > kmin ? (kmax + PKV - 1) / PKV - jt0 : 0;  // key tiles
 
     if (tid == 0) {
@@ -440,10 +440,10 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(smem_u32(&bars.q_full));
             // ---- softmax ----
-            const int vhi = live ? min(pos0 + tok + 1, hi) : 0, vlo = a.window ? max(0, pos0 + tok - a.window + 1) : 0;
+            const int vhi = live ? min(pos0 + tok + 1, hi) : 0, vlo = first_seen(a.window, pos0 + tok);
             // keys that every row of the tile sees
             const int first = (row0 + rt * 128) / group, last = min(n - 1, (row0 + rt * 128 + 127) / group);
-            const int all_hi = min(pos0 + first + 1, hi), all_lo = a.window ? max(0, pos0 + last - a.window + 1) : 0;
+            const int all_hi = min(pos0 + first + 1, hi), all_lo = first_seen(a.window, pos0 + last);
             float m = -INFINITY, l = 0.0f;
             for (int j = 0; j < nt; j++) {
                 const int sb = PAIR ? j & 1 : rt, key0 = (jt0 + j) * PKV;

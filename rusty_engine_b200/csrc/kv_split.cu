@@ -81,7 +81,7 @@ __device__ __forceinline__ SplitReq split_req(const AttendArg& a, int r, int hea
     q.pos0 = len - (c1 - c0);
     const int64_t rows = (int64_t)q.n * group;
     q.hi = (int)min((int64_t)max(len, 0), (int64_t)a.max_blocks * bs);
-    const int lo = a.window ? max(0, q.pos0 - a.window + 1) : 0;
+    const int lo = first_seen(a.window, q.pos0);
     q.t0 = min(lo, q.hi) / tw;
     q.tiles = max(1, (q.hi + tw - 1) / tw - q.t0);
     q.items = rows > max_rows ? 0 : (int)((rows + nr - 1) / nr) * heads;
@@ -115,7 +115,7 @@ struct SplitKeys { int lo, hi; };
 __device__ __forceinline__ SplitKeys split_keys(const AttendArg& a, const SplitReq& q, int rt, int nr, int group) {
     if (q.n == 1) return {0, q.hi};  // a decoded token: its tiles begin and end with its keys
     const int first = rt * nr / group, last = min(q.n - 1, (rt * nr + nr - 1) / group);
-    return {a.window ? max(0, q.pos0 + first - a.window + 1) : 0, min(q.pos0 + last + 1, q.hi)};
+    return {first_seen(a.window, q.pos0 + first), min(q.pos0 + last + 1, q.hi)};
 }
 
 struct SplitPiece {   // where a piece belongs
@@ -404,14 +404,14 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     qs[nt][i] = __shfl_sync(0xffffffffu, up, (2 * c + i) * 4);
                     const int t2 = tok_of(nt * 8 + 2 * c + i), p = rq.pos0 + t2;
                     vhi[nt][i] = t2 < rq.n ? min(p + 1, rq.hi) : 0;
-                    vlo[nt][i] = a.window ? max(0, p - a.window + 1) : 0;
+                    vlo[nt][i] = first_seen(a.window, p);
                 }
             }
             // keys that every row of the tile sees: no masks there
             const int last = min(rq.n - 1, tok_of(NR - 1)), firstt = tok0;
             const int all_hi = min(rq.pos0 + firstt + 1, rq.hi);
-            const int all_lo = a.window ? max(0, rq.pos0 + last - a.window + 1) : 0;
-            const int any_lo = a.window ? max(0, rq.pos0 + firstt - a.window + 1) : 0;
+            const int all_lo = first_seen(a.window, rq.pos0 + last);
+            const int any_lo = first_seen(a.window, rq.pos0 + firstt);
             const int any_hi = min(rq.pos0 + last + 1, rq.hi);
 
             float o[QT][KS][4], m[QT][2], l[QT][2];

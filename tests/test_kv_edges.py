@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import kv_ref as R
-from test_kv import REL, cache_of, ints, kv, rel, slots_of  # noqa: F401
+from test_kv import REL, cache_of, ints, kv, rel, run_attend, slots_of  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -210,3 +210,13 @@ def test_return_lse_takes_any_truth_value(kv):
         assert out.shape == q.shape and lse.shape == (2, 4)
     for no in (False, 0, np.False_, None):
         assert c.attend(q, ints([[0, 1]]), ints([20]), ints([0, 2]), return_lse=no).shape == q.shape
+
+
+# ---- windows ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 7])
+def test_attend_window_near_the_largest_integer(kv, dtype, window):
+    """More queries than cached tokens (positions below 0) under windows that mean "all keys"."""
+    run_attend(kv, "int8", dtype, [3, 40], [10, 5], 16, 8, 2, 64, window=window)
+    run_attend(kv, "int8", dtype, [3], [12], 16, 4, 2, 256, window=window)
+    run_attend(kv, "int8", dtype, [3, 200, 0], [300, 280, 90], 16, 16, 8, 64, window=window)
