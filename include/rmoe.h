@@ -423,7 +423,9 @@ RMOE_API rmoe_status rmoe_kv_read(rmoe_kv* kv, const int32_t* slots, uint32_t n,
 /* Attention of T query tokens over the cache (src/forward.rs:218-283, for R requests at once):
  * request r has lens[r] cached tokens, the queries of tokens cu[r] .. cu[r + 1) being those of its
  * last positions; query at position p sees keys max(0, p - window + 1) .. p (window 0: from 0),
- * query head h reads kv head h / (q heads / kv heads).
+ * query head h reads kv head h / (q heads / kv heads).  Table entries of blocks that no query sees are
+ * not used and may be anything; others outside the cache set the status word, and their keys count as
+ * unseen.
  *   out[t][h] = sum_j softmax_j(scale q.k_j) v_j ;  lse[t][h] = ln sum_j exp(scale q.k_j)
  * (lse, natural logarithm, optional: [T][q heads] f32).  A row that sees no key gives 0 and
  * -infinity, as do tokens past cu[R].  max_new: an upper bound of the new tokens of any request

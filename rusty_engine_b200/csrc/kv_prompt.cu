@@ -195,7 +195,8 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
             for (int j = 0; j < nt; j++) {
                 const int t = (jt0 + j) * PKV + 16 * lane;
                 const bool want = lane < 8 && t < kmax, ok = want && (unsigned)blk < (unsigned)kv.n_blocks;
-                if (want && !ok) atomicOr(kv.status, (unsigned)DERR_INDEX);
+                // (a block whose keys all lie before the window may have been given back)
+                if (want && !ok && t + 16 > kmin) atomicOr(kv.status, (unsigned)DERR_INDEX);
                 const int64_t bh = ok ? (int64_t)blk * heads + kh : 0;
                 const float ks = ok ? __ldg(kv.ks + bh) : 0.0f, vs = ok ? __ldg(kv.vs + bh) : 1.0f;
                 const int next = lookup(j + 1);

@@ -313,7 +313,8 @@ kv_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             // a tile that no row sees is not fetched: its boxes count as missing
             const int j0 = (pq.t0 + ptile) * TW;
             const bool want = lane < nb && j < pq.hi && j0 < pkeys.hi && j0 + TW > pkeys.lo, ok = want && (unsigned)pblk < (unsigned)kv.n_blocks;
-            if (want && !ok) atomicOr(kv.status, (unsigned)DERR_INDEX);
+            // (a block whose keys all lie before the window may have been given back)
+            if (want && !ok && j + br > first_seen(a.window, pq.pos0 + pit.rt * NR / group)) atomicOr(kv.status, (unsigned)DERR_INDEX);
             const unsigned mask = __ballot_sync(0xffffffffu, ok);
             if (lane == 0) tc::mbar_arrive_expect_tx(bar, __popc(mask) * br * D * 2);
             __syncwarp();

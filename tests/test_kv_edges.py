@@ -220,3 +220,38 @@ def test_attend_window_near_the_largest_integer(kv, dtype, window):
     run_attend(kv, "int8", dtype, [3, 40], [10, 5], 16, 8, 2, 64, window=window)
     run_attend(kv, "int8", dtype, [3], [12], 16, 4, 2, 256, window=window)
     run_attend(kv, "int8", dtype, [3, 200, 0], [300, 280, 90], 16, 16, 8, 64, window=window)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lens,new,bs,nq,nkv,d,window", [
+    ([700, 300], [1, 1], 16, 8, 2, 128, 100), ([700], [3], 16, 4, 1, 64, 55), ([700], [1], 16, 4, 1, 256, 55),
+    ([700], [40], 64, 4, 1, 256, 90), ([900], [300], 16, 32, 8, 128, 100), ([900], [300], 64, 32, 8, 64, 33)])
+def test_attend_blocks_before_the_window_may_be_gone(kv, dtype, lens, new, bs, nq, nkv, d, window):
+    """A server that gives blocks behind a sliding window back: entries of -1 (and beyond the cache)
+    that no query sees change nothing and are no error; one inside the window is."""
+    from rusty_engine_b200._lib import RmoeError
+
+    blocks = sum(-(-n // bs) for n in lens) + 1
+    c, *_ = cache_of(kv, "e4m3", blocks, nkv, bs, d)
+    _, _, table = slots_of(lens, [0] * len(lens), bs, blocks)
+    mb = max(len(t) for t in table)
+    full = ints([t + [-1] * (mb - len(t)) for t in table])
+    first = [max(0, n - m - window + 1) // bs for n, m in zip(lens, new)]
+    holes = full.clone()
+    for r, f in enumerate(first):
+        assert f > 0
+        holes[r, :f] = -1
+        holes[r, 0] = blocks + 5
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randn((sum(new), nq, d), generator=g, device="cuda").to(R.DT[dtype])
+    call = lambda t: c.attend(q, t, ints(lens), ints(np.concatenate(([0], np.cumsum(new))).tolist()), window=window,  # noqa: E731
+                              max_new=max(new), return_lse=True)
+    want, wl = call(full)
+    c.check()
+    got, gl = call(holes)
+    c.check()
+    assert torch.equal(got, want) and torch.equal(gl, wl)
+    holes[0, first[0]] = -1
+    call(holes)
+    with pytest.raises(RmoeError, match="out of range"):
+        c.check()
