@@ -430,7 +430,10 @@ RMOE_API rmoe_status rmoe_kv_read(rmoe_kv* kv, const int32_t* slots, uint32_t n,
  * (lse, natural logarithm, optional: [T][q heads] f32).  A row that sees no key gives 0 and
  * -infinity, as do tokens past cu[R].  max_new: an upper bound of the new tokens of any request
  * where the caller knows one (0: unknown); it only chooses kernels.  f32 calls carry q and the
- * probabilities as pairs of fp16; codes are exact in fp16. */
+ * probabilities as pairs of fp16, 16-bit calls the probabilities as one (times a power of two, in
+ * all); codes are exact in fp16, sums are f32.  A key whose weight times its block's V
+ * scale (0 counts as 2^-60, any other below 2^-100 as 2^-100) is below 2^-126 of another's in the
+ * row is left out of the sums. */
 typedef struct {
     rmoe_rows q, out;
     const int32_t *table, *lens, *cu;

@@ -4,8 +4,8 @@
 // Mathematics.  With x_j = scale log2(e) ks_j q.kc_j + log2(vs_j) over the keys j that a row sees,
 //   out = sum_j 2^(x_j - M) vc_j / sum_j 2^(x_j - M) / vs_j ,   lse = (M + log2 of that sum) ln 2
 // for any M; M is the running maximum of x_j.  Folding the V scale into the exponent keeps the
-// weights of P V in (0, 1] whatever the scales are; a scale below 2^-100 counts as 2^-100.  Codes are
-// exact in fp16; q is carried as fp16 times a power of two per row and the weights as fp16 times
+// weights of P V in (0, 1] whatever the scales are (v_scale_floor gives their limits).  Codes are exact in
+// fp16; q is carried as fp16 times a power of two per row and the weights as fp16 times
 // 2^15 (f32 calls: both as pairs, hi + lo), so that a weight has its 11 bits down to 2^-29 of the row's
 // largest (f32 calls: 22 bits down to 2^-18, one less for each factor 2 from there).  All sums are f32.
 //

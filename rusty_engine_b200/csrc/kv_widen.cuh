@@ -50,8 +50,14 @@ __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
 
 // The V scale enters the exponent: log2 of it is added to the score, and a row's sum takes its
 // reciprocal (to 2^-22: an error of the logarithm changes a block's weights alike in both sums and
-// is as small as the weights' own).  A scale below 2^-100 (zero included) counts as 2^-100.
-__device__ __forceinline__ float v_scale_floor(float vs) { return fmaxf(vs, 7.8886090522101181e-31f); }
+// is as small as the weights' own).  Exponentials below 2^-126 are 0, so a key whose weight times its
+// block's scale is 2^-126 of another's loses its share of the sum.  Values of 0 have no scale of their
+// own: their block counts as 2^-60, where it keeps its share beside scales of 2^46 (values of 9e15) from
+// 20 powers of two below them on (counted as 2^-100, zeros beside values of 1e10 lost it), and takes no
+// bits from the weights of blocks with scales above 2^-78.  Any other scale below 2^-100 counts as 2^-100.
+__device__ __forceinline__ float v_scale_floor(float vs) {
+    return vs == 0.0f ? 8.6736173798840355e-19f : fmaxf(vs, 7.8886090522101181e-31f);
+}
 
 // The exponent e that brings a row of q whose largest magnitude is mx to mx 2^-e in [2^13, 2^14);
 // 0 where there is nothing to scale (0, infinities, NaN).

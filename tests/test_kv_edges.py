@@ -255,3 +255,34 @@ def test_attend_blocks_before_the_window_may_be_gone(kv, dtype, lens, new, bs, n
     call(holes)
     with pytest.raises(RmoeError, match="out of range"):
         c.check()
+
+
+# ---- scales -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("big", [1.0, 1e10, 1e14])
+@pytest.mark.parametrize("lens,new,nq,nkv,d", [([200, 130], [1, 1], 8, 2, 128), ([180], [9], 4, 1, 256), ([700], [200], 32, 8, 64)])
+def test_attend_blocks_of_zeros_beside_large_values(kv, dtype, big, lens, new, nq, nkv, d):
+    """Blocks whose keys or values are all 0 (their scale is 0) keep their share of every row,
+    however large the other blocks' values are."""
+    bs = 16
+    blocks = sum(-(-n // bs) for n in lens)
+    c = kv.KVCache(blocks, bs, nkv, d)
+    slots, _, table = slots_of(lens, lens, bs, blocks)
+    g = torch.Generator().manual_seed(1)
+    T = len(slots)
+    k, v = torch.randn((T, nkv, d), generator=g), torch.randn((T, nkv, d), generator=g) * big
+    pos = torch.cat([torch.arange(n) for n in lens])
+    v[pos // bs % 3 == 0] = 0  # the first block too
+    k[pos // bs % 4 == 1] = 0
+    c.append(k.cuda(), v.cuda(), ints(slots))
+    assert (c.v_scale == 0).any() and (c.k_scale == 0).any()
+    q = torch.randn((sum(new), nq, d), generator=g).to(R.DT[dtype])
+    cu = np.concatenate(([0], np.cumsum(new))).tolist()
+    mb = max(len(t) for t in table)
+    out, lse = c.attend(q.cuda(), ints([t + [-1] * (mb - len(t)) for t in table]), ints(lens), ints(cu), max_new=max(new),
+                        return_lse=True)
+    want, wl = R.attend(q, c.k.cpu().float(), c.v.cpu().float(), c.k_scale.cpu(), c.v_scale.cpu(), table, lens, cu,
+                        float(np.float32(1 / np.sqrt(d))))
+    assert rel(out, want) <= REL[dtype]
+    assert (lse.cpu().double() - wl).abs().max().item() <= 2e-5
+    c.check()
