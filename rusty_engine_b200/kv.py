@@ -188,9 +188,13 @@ class KVBatch:
         self.n_free = torch.full((1,), n_blocks, dtype=torch.int32, device=dev)
 
     def extend(self, new_lens, total: int, *, stream=None) -> KVStep:
-        """extend_tables on this batch; lens and the stack move on."""
-        step = extend_tables(self.table, self.lens, new_lens, self.free, self.n_free, total, self.block_size, stream=stream)
-        self.lens, self.n_free = step.lens, step.n_free
+        """extend_tables on this batch; lens and the stack move on (in place, so that a step captured in
+        a CUDA graph is the next step at every replay)."""
+        if stream is not None:
+            with _on(stream, self.table, self.lens, new_lens, self.free, self.n_free):
+                return self.extend(new_lens, total)
+        step = extend_tables(self.table, self.lens, new_lens, self.free, self.n_free, total, self.block_size)
+        torch._foreach_copy_([self.lens, self.n_free], [step.lens, step.n_free])
         return step
 
     def release(self, done, *, stream=None):
@@ -205,7 +209,7 @@ class KVBatch:
                                              _int32(done, "done", self.table, R), self.n_free.data_ptr(), out.data_ptr(),
                                              R, mb, self.block_size, self.free.numel())
             _call(_lib.load().rmoe_kv_release(args, _stream()))
-        self.n_free = out
+        self.n_free.copy_(out)
 
 
 class KVCache:

@@ -286,3 +286,36 @@ def test_attend_blocks_of_zeros_beside_large_values(kv, dtype, big, lens, new, n
     assert rel(out, want) <= REL[dtype]
     assert (lse.cpu().double() - wl).abs().max().item() <= 2e-5
     c.check()
+
+
+def test_batch_step_in_a_cuda_graph_moves_on(kv):
+    """KVBatch.extend, append, attend and release captured once: every replay is the next step."""
+    b, e = kv.KVBatch(3, 8, 20, 16), kv.KVBatch(3, 8, 20, 16)
+    caches = [kv.KVCache(20, 16, 2, 64) for _ in (b, e)]
+    x = torch.randn((3, 8, 64), device="cuda")
+    done, new = ints([0, 0, 0]), ints([1, 1, 1])
+
+    def step(batch, c):
+        st = batch.extend(new, 3)
+        c.append(x[:, 4:6], x[:, 6:], st.slots)
+        out = c.attend(x[:, :4], batch.table, batch.lens, st.cu, max_new=1)
+        batch.release(done)
+        return out
+
+    first = ints([15, 0, 30])
+    for batch, c in zip((b, e), caches):
+        st = batch.extend(first, 45)
+        c.append(torch.ones((45, 2, 64), device="cuda"), torch.ones((45, 2, 64), device="cuda"), st.slots)
+        step(batch, c)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(b, caches[0])
+    for i in range(20):
+        x.copy_(torch.randn((3, 8, 64), device="cuda"))
+        done.copy_(ints([int(i == 7), 0, int(i == 11)]))
+        g.replay()
+        want = step(e, caches[1])
+        assert torch.equal(out, want), i
+        assert b.lens.tolist() == e.lens.tolist() and b.n_free.tolist() == e.n_free.tolist()
+        assert torch.equal(b.table, e.table)
+    assert b.lens.tolist() == [12, 21, 8]
