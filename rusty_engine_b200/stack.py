@@ -232,14 +232,15 @@ class MoEStack:
     def open_cache(self, max_requests: int, n_blocks: int, block_size: int = 64, max_pos: int = 4096, code=None,
                    rope_cfg=None):
         """A paged 8-bit KV cache of n_blocks blocks per layer for up to max_requests requests of up
-        to max_pos tokens, and the rotary plan (NeoX halves over the whole head by default)."""
+        to max_pos tokens (rounded up to whole blocks), and the rotary plan (NeoX halves over the whole head by default)."""
         from . import kv
 
         g = self.g
         cfg = rope_cfg or kv.RopeConfig(rot_dim=g.head_dim, base=g.rope_freq_base, layout=kv.RopeLayout.Half)
         code = kv.CacheCode.Int8 if code is None else code
-        self.rope = kv.Rope(cfg, max_pos, self.device)
-        self.batch = kv.KVBatch(max_requests, -(-max_pos // block_size), n_blocks, block_size, self.device)
+        per_request = -(-max_pos // block_size)
+        self.rope = kv.Rope(cfg, per_request * block_size, self.device)  # as far as a table row reaches
+        self.batch = kv.KVBatch(max_requests, per_request, n_blocks, block_size, self.device)
         self.caches = [kv.KVCache(n_blocks, block_size, g.n_kv_heads, g.head_dim, code, self.device) for _ in self.layers]
 
     def step(self, x, new_lens, max_new: Optional[int] = None, collect: bool = False):

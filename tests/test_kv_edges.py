@@ -319,3 +319,19 @@ def test_batch_step_in_a_cuda_graph_moves_on(kv):
         assert b.lens.tolist() == e.lens.tolist() and b.n_free.tolist() == e.n_free.tolist()
         assert torch.equal(b.table, e.table)
     assert b.lens.tolist() == [12, 21, 8]
+
+
+def test_open_cache_positions_reach_as_far_as_its_blocks(kv):
+    """max_pos inside a block: the table has room up to the block's end, and so has the rope."""
+    from rusty_engine_b200.stack import MoEStack, make_block
+    from test_stack import small_geometry
+
+    geo = small_geometry()
+    stack = MoEStack(geo, [make_block(geo, seed=3, dlo=0.001, dhi=0.004, attn_dlo=0.002, attn_dhi=0.01)], device=0)
+    stack.open_cache(max_requests=1, n_blocks=4, block_size=16, max_pos=20)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn((32, geo.d_model), generator=g, device="cuda")
+    stack.step(x, ints([32]), max_new=32)
+    assert stack.batch.lens.tolist() == [32]  # the table takes them
+    stack.caches[0].check()                   # and every position is turned
+    stack.close()
