@@ -48,15 +48,26 @@ BINDING_SRC = os.path.join(HERE, "binding", "kv_ops.cpp")
 BINDING = os.path.join(HERE, "_kv_ops.so")
 
 
-def build_binding() -> str:
-    """The torch-tensor entry of kv.py (binding/kv_ops.cpp), linked against librmoe.so and torch."""
+def build_binding():
+    """The torch-tensor entry of kv.py (binding/kv_ops.cpp), linked against librmoe.so and torch; its
+    path, or None where what it needs is missing (torch with CUDA, g++, Python's headers): librmoe.so
+    needs none of these, and kv.py says so when it is used."""
     deps = [BINDING_SRC, os.path.join(HERE, "..", "include", "rmoe.h")]
     if os.path.exists(BINDING) and os.path.getmtime(BINDING) >= max(os.path.getmtime(d) for d in deps):
         return BINDING
     import sysconfig
 
-    import torch
-    from torch.utils.cpp_extension import include_paths
+    try:
+        import torch
+        from torch.utils.cpp_extension import include_paths
+    except (ImportError, OSError) as e:
+        return _no_binding(str(e))
+    needs = [(os.path.join(os.path.dirname(torch.__file__), "lib", "libc10_cuda.so"), "torch without CUDA"),
+             (shutil.which("g++") or "", "no g++"),
+             (os.path.join(sysconfig.get_paths()["include"], "Python.h"), "no Python.h")]
+    for path, why in needs:
+        if not os.path.exists(path):
+            return _no_binding(why)
 
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cuda_inc = os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")
@@ -69,6 +80,11 @@ def build_binding() -> str:
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for {BINDING_SRC}:\n{r.stderr}")
     return BINDING
+
+
+def _no_binding(why: str):
+    print(f"{os.path.basename(BINDING)} not built ({why}): rusty_engine_b200.kv needs it, the C library does not", file=sys.stderr)
+    return None
 
 
 def build(verbose: bool = False, jobs: int = 8) -> str:
