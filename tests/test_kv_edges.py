@@ -335,3 +335,73 @@ def test_open_cache_positions_reach_as_far_as_its_blocks(kv):
     assert stack.batch.lens.tolist() == [32]  # the table takes them
     stack.caches[0].check()                   # and every position is turned
     stack.close()
+
+
+# ---- many requests, many runs -------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("reqs", [33, 40, 257, 300, 600])
+def test_attend_many_requests(kv, dtype, reqs):
+    """More requests than a warp's lanes, than the split kernel's threads and than the prompt
+    kernel's; empty ones among them; then the same beside prompts for the prompt kernel."""
+    rng = np.random.default_rng(reqs)
+    lens = rng.integers(0, 70, reqs).tolist()
+    new = [int(min(n, m)) for n, m in zip(rng.integers(0, 4, reqs), lens)]
+    run_attend(kv, "int8", dtype, lens, new, 16, 2, 1, 64)
+    run_attend(kv, "e4m3", dtype, lens, [min(n, 1) for n in lens], 32, 6, 2, 128, window=9)
+    for r, (n, m) in zip((reqs - 1, 0, reqs // 2), ((300, 260), (270, 270), (200, 130))):
+        lens[r], new[r] = n, m
+    run_attend(kv, "int8", dtype, lens, new, 16, 16, 8, 64)
+    run_attend(kv, "int8", dtype, lens, new, 64, 16, 8, 64, max_new=False, pad=7, window=50)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("bs", [16, 128])
+@pytest.mark.parametrize("reqs", [1025, 1500])
+def test_append_many_single_tokens(kv, code, bs, reqs):
+    """More than 1024 runs of one token each, some slots skipped."""
+    rng = np.random.default_rng(reqs + bs)
+    c, k, v, ks, vs = cache_of(kv, code, reqs, 2, bs, 64)
+    order = rng.permutation(reqs)
+    slots = [int(b) * bs + int(rng.integers(0, bs)) if rng.random() < 0.9 else -1 for b in order]
+    g = torch.Generator().manual_seed(7)
+    kn, vn = (torch.randn((reqs, 2, 64), generator=g) * torch.rand((reqs, 1, 1), generator=g) * 4 for _ in "kv")
+    c.append(kn.cuda(), vn.cuda(), ints(slots))
+    R.append(k, ks, kn.numpy(), slots, bs, code)
+    R.append(v, vs, vn.numpy(), slots, bs, code)
+    assert np.array_equal(c.k_scale.cpu().numpy(), ks) and np.array_equal(c.v_scale.cpu().numpy(), vs)
+    assert np.array_equal(c.k.float().cpu().numpy(), k) and np.array_equal(c.v.float().cpu().numpy(), v)
+    c.check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("T,nq,strided", [(640, 32, False), (1300, 16, False), (1300, 16, True)])
+def test_append_beside_the_rope_of_a_long_q(kv, dtype, T, nq, strided):
+    """A q long enough for its own kernel, beside which the cache is written: inputs that the stream
+    has just made, q in place, and attention right after, against the calls one by one, bit for bit."""
+    rope = kv.Rope(kv.RopeConfig(128, 1e6), 4096)
+    blocks = -(-T // 64)
+    a, b = (kv.KVCache(blocks, 64, 2, 128) for _ in "ab")
+    table, lens, cu = ints([list(range(blocks))]), ints([T]), ints([0, T])
+    g = torch.Generator(device="cuda").manual_seed(5)
+    for i in range(6):
+        base = torch.randn((T, nq + 4 + strided, 128), generator=g, device="cuda").to(R.DT[dtype])
+        pos = torch.arange(T, dtype=torch.int32, device="cuda")
+        x, slots = base * 2, pos + 0
+        q, k, v = x[:, :nq], x[:, nq:nq + 2], x[:, nq + 2:nq + 4]
+        if not strided:
+            q = q.contiguous()
+        got = a.append(k, v, slots, rope=rope, positions=pos, q=q, q_out=q)
+        out = a.attend(got, table, lens, cu, max_new=T)
+        torch.cuda.synchronize()
+        x = base * 2
+        qr, kr = rope.apply(x[:, :nq], pos, x[:, nq:nq + 2])
+        torch.cuda.synchronize()
+        b.append(kr.float(), x[:, nq + 2:nq + 4].float(), slots)
+        torch.cuda.synchronize()
+        assert torch.equal(got, qr), i
+        if dtype == "f32":  # (in 16 bits the keys would be rounded between rope and cache)
+            for m, n in ((a.k, b.k), (a.k_scale, b.k_scale)):
+                assert torch.equal(m, n), i
+        assert torch.equal(a.v, b.v) and torch.equal(a.v_scale, b.v_scale)
+        assert torch.equal(out, a.attend(qr, table, lens, cu, max_new=T))
+    a.check()
