@@ -405,3 +405,38 @@ def test_append_beside_the_rope_of_a_long_q(kv, dtype, T, nq, strided):
         assert torch.equal(a.v, b.v) and torch.equal(a.v_scale, b.v_scale)
         assert torch.equal(out, a.attend(qr, table, lens, cu, max_new=T))
     a.check()
+
+
+def test_attend_on_new_streams_while_another_captures(kv):
+    """A call that is captured and a plain one on another stream in the middle of the capture, each the
+    first of its stream: the workspaces they need are made without ending the capture."""
+    from rusty_engine_b200 import _lib
+
+    c, *_ = cache_of(kv, "int8", 200, 2, 64, 128)
+    q = torch.randn((2, 16, 128), device="cuda")
+    outs = [torch.zeros_like(q) for _ in range(3)]
+    tab, lens, cu = ints([list(range(0, 90)), list(range(100, 190))]), ints([5700, 5000]), ints([0, 1, 2])
+    want = c.attend(q, tab, lens, cu)
+    rows = lambda t: (t.data_ptr(), 16 * 128, 128, 16, 0)  # noqa: E731
+
+    def call(out, stream):
+        args = _lib.KV_ATTEND_ARGS.pack(*rows(q), *rows(out), tab.data_ptr(), lens.data_ptr(), cu.data_ptr(), 0, 2, 90, 2, 0,
+                                        float(np.float32(1 / np.sqrt(128))), 0, 1, 0)
+        assert _lib.load().rmoe_kv_attend(c._h, args, stream.cuda_stream) == _lib.RMOE_OK, _lib.load().rmoe_last_error()
+
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=streams[0]):
+        call(outs[0], streams[0])
+        call(outs[1], streams[1])
+        call(outs[2], streams[2])
+        call(outs[0], streams[0])
+    torch.cuda.synchronize()
+    assert torch.equal(outs[1], want) and torch.equal(outs[2], want) and not outs[0].any()
+    for _ in range(3):
+        outs[0].zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want)
+    c.check()
