@@ -19,8 +19,9 @@ struct AppendArg {
 // A run is the tokens of one call that go to consecutive slots of one block: they share a scale.
 // A CTA looks at `window` tokens for one head of K or V and writes the runs that begin there: all
 // threads together where few begin (prompts), a warp per run where many do (decoded tokens).
-// A run is bound by reading its elements once; up to HOLD units of 16 stay in registers between the
-// pass that finds the largest magnitude and the pass that rounds, the rest is read again (L2).
+// A run is bound by reading its elements once; up to HOLD units of 16 are held by a thread between the
+// pass that finds the largest magnitude and the pass that rounds, the rest is read again (L2).  Three CTAs an
+// SM leave a thread 80 registers, and 84 (f32) or 96 bytes of it spill.
 // Measured (B200): 8192 tokens of 4 + 4 heads of 128 in bf16 with rope, blocks of 64: 15.7 us, 25 MB, 1.6
 // TB/s (12.7 us without rope); it waits for its loads (slots, then elements and positions, then angles:
 // three trips, 21 warps an SM).  32 decoded tokens of f32 with the read of them: 5.8 us, latency.
@@ -178,8 +179,9 @@ __global__ void __launch_bounds__(APT, 3) kv_append_kernel(KvArg kv, AppendArg a
     if (a.apart) pdl_wait();  // the next kernel may take the end of this one for the end of both
 }
 
-// One thread per 16 elements of a slot and head, K then V.  8192 slots of 4 heads of 128 as bf16: 7.1
-// us, 25 MB, 3.5 TB/s (B200).
+// One thread per 16 elements of a slot and head, K then V.  8192 slots of 4 heads of 128 as bf16: 6.8
+// us, 25 MB, 3.7 TB/s; as f32 11.9 us, 42 MB (B200): a thread waits for its slot and then for its scale and
+// codes, with nothing else of it in flight.
 template <typename T, int CODE>
 __global__ void __launch_bounds__(256) kv_read_kernel(KvArg kv, const int32_t* slots, int n, T* ko, T* vo) {
     pdl_trigger();
@@ -214,7 +216,11 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvArg kv, const int32_t* s
 template <typename T, int CODE>
 static cudaError_t append_launch(const KvArg& kv, AppendArg a, cudaStream_t s) {
     // Decoded tokens are a run each: windows of 8 give every warp one, until such windows fill the
-    // chip; then a block's worth of tokens, in which a prompt begins one or two runs.
+    // chip; then a block's worth of tokens, in which a prompt begins one or two runs.  Windows of 8 / of a block
+    // in us (B200, bf16, 4 heads of 128): 256 decoded tokens in blocks of 64 4.0 / 12.7, 1024 8.9 / 18.5, 4096
+    // 28.9 / 28.5; in blocks of 16 1024 8.9 / 9.1, 4096 28.9 / 25.5.  Prompts in blocks of 64: 256 tokens 4.2 / 3.7,
+    // 1024 6.3 / 5.0, 4096 13.8 / 7.5.  The rule goes by tokens alone, which only the device could tell
+    // apart: from 1025 decoded tokens in blocks of 64 or 128 to some 4096 it loses up to 10 (128: 20) us.
     a.window = a.T <= 1024 ? 8 : kv.bs;
     const int64_t kvc = ((int64_t)a.T + a.window - 1) / a.window * kv.heads * 2;
     const int64_t qn = (int64_t)a.T * a.q.heads * (kv.dim / 16);

@@ -15,16 +15,16 @@
 //     rescaled when a row's maximum grew by more than 2^LAG, by the softmax threads.
 //     P is carried as 2^UP times itself, so a weight has its 11 bits down to 2^-21 of the row's largest
 //     (2^-29 when M lags behind that).
-//   f32 calls: q and P (2^15 times itself) are fp16 pairs (hi + lo, twice the products), one row tile, S in two
-//     buffers.  The tensor cores cut every partial sum short, about 2^-24 per step and all one
+//   f32 calls: q and P (2^15 times itself) are fp16 pairs (hi + lo, twice the products), one row tile, S in
+//     two buffers (head_dim 128: 92 bytes a thread spill).  The tensor cores cut every partial sum short, about 2^-24 per step and all one
 //     way, which over a long row is more than f32 attention may lose (up to 4.5e-6 measured); so each key
 //     tile has its own O in tensor memory, and the other four warps add the tiles up in registers.
 //
 // Measured (B200): 4096 new and 3 decoded tokens over up to 8192 keys, 32 heads over 4 kv heads of
-// 128, bf16, int8 cache: 482 to 493 us on changing inputs (465 when one input repeats), 412.6 GFLOP, 837 to 856
-// TFLOP/s = 51 to 52% of the cuBLAS rate; a 2048-token prompt in f32: 124 us (120), 34.4 GFLOP, 277 TFLOP/s (twice
-// that with the pairs' products).  No pipe is full (tensor
-// and special functions 47% each in bf16): softmax, P V and the next S of a row tile follow one another, and
+// 128, bf16, int8 cache: 480 to 493 us on changing inputs (462 when one input repeats), 412.6 GFLOP, 837 to 860
+// TFLOP/s = 51 to 52% of the cuBLAS rate; a 2048-token prompt in f32: 122 us (120), 34.4 GFLOP, 281 TFLOP/s (twice
+// that with the pairs' products), in bf16 63 us, 545 TFLOP/s; 64 wide 92 and 48 us.  No pipe is full (tensor
+// and special functions 47% each in the mixed batch in bf16): softmax, P V and the next S of a row tile follow one another, and
 // only the other row tile's work hides them.  More row tiles do not fit: S and O of two fill tensor
 // memory's 512 columns at head_dim 128.
 #include "kv_attend.h"

@@ -29,9 +29,9 @@
 // arriving CTA (an atomic count, nobody waits) joins them in CTA order: the result does not depend
 // on timing.
 //
-// Measured (B200, int8 unless said): 32 requests of 2048 to 8192 tokens, bf16: 41.3 us, 171 MB, 4.1
-// TB/s = 63% of the copy rate; 2 requests of 131071 tokens, fp16, e4m3: 45.8 us, 206 MB, 4.5 TB/s; one of
-// 97 tokens, f32: 7.9 us.  DRAM traffic is the algorithmic bytes, the issue slots are 41% busy: what is
+// Measured (B200, int8 unless said): 32 requests of 2048 to 8192 tokens, bf16: 41.5 us, 171 MB, 4.1
+// TB/s = 63% of the copy rate (f32 47.7); 2 requests of 131071 tokens, fp16, e4m3: 45.7 us, 206 MB, 4.5 TB/s;
+// one of 97 tokens, f32: 8.0 us; 512 requests of up to 512 tokens, bf16: 52.9 us, of up to 2048: 128.9.  DRAM traffic is the algorithmic bytes, the issue slots are 41% busy: what is
 // above the floor is latency, the steps before the first tile (lengths, block table and the first copy,
 // one after the other) and the joining at the end.
 #include <algorithm>
@@ -844,7 +844,8 @@ static cudaError_t split_launch(const KvMaps& maps, const KvArg& kv, const Atten
     return launch_pdl(k, dim3(std::min(sms, SPLIT_MAX_SMS)), dim3(SPLIT_NW * 32), smem, s, maps.k, maps.v, kv, a, ws);
 }
 
-// nr: 8 or 16 rows per item (16 only up to head_dim 128: the accumulators of 256 would spill)
+// nr: 8 or 16 rows per item (16 only up to head_dim 128: the accumulators of 256 alone would take 128
+// registers a thread; 8 rows of it spill 44 bytes in f32)
 template <typename T, int CODE>
 static cudaError_t split_dims(const KvMaps& maps, const KvArg& kv, const AttendArg& a, const SplitWs& ws, int sms, int nr,
                               cudaStream_t s) {

@@ -115,7 +115,8 @@ __global__ void __launch_bounds__(EXT_THREADS) kv_extend_kernel(rmoe_kv_extend_a
     }
 }
 
-// One CTA: prefix sums of the blocks to give back, then a warp per request moves them.
+// One CTA: prefix sums of the blocks to give back, then a warp per request moves them.  It runs once
+// when requests end: 8 requests of 500 tokens 4.6 us, 64 of 8192 8.4, 512 of 4096 23.5 (B200, in a graph).
 __global__ void __launch_bounds__(EXT_THREADS) kv_release_kernel(rmoe_kv_release_args a) {
     extern __shared__ int32_t s_at[];  // [R] stack position of the request's first block, -1: not done
     __shared__ int64_t warp_tot[32];

@@ -37,8 +37,8 @@ __global__ void __launch_bounds__(256, 3) rope_units_kernel(Rows q, Rows qo, Row
 // Long batches of heads that lie one after the other: a warp brings a token's q, k and angles into
 // its own part of shared memory as bulk copies, turns them there and sends them back as bulk
 // copies, three tokens deep.  The copies keep the memory busy with hardly any registers, where
-// per-thread loads reached 62-66% of the copy rate whatever their number; a ring shared by the
-// CTA's warps, in step from token to token, was no faster than those (8192 tokens of 32 + 4 heads of
+// per-thread loads of 16-bit heads reached 62-70% of the copy rate whatever their number; a ring shared by
+// the CTA's warps, in step from token to token, was no faster than those (8192 tokens of 32 + 4 heads of
 // 128 in bf16, B200).  A ring per warp: 27.4 us, 153 MB, 5.6 TB/s = 85% of the copy rate;
 // 67 MB of q in and out: 25.6 us where a copy takes 24.7.
 struct RopeStream {
@@ -185,7 +185,11 @@ static cudaError_t rope_launch(const Rows& q, const Rows& qo, const Rows& k, con
                                int dim, unsigned* status, cudaStream_t s) {
     const bool units = dim % 16 == 0 && ra.rot % 16 == 0;
     const bool rows = q.vec && qo.vec && q.sh == dim && qo.sh == dim && (!k.heads || (k.vec && ko.vec && k.sh == dim && ko.sh == dim));
-    // the ring pays from a few tokens a warp on, and where the stages of three warps fit an SM
+    // The ring pays for long batches of 16-bit heads, where the stages of three warps fit an SM.  Ring / units in
+    // us (B200, heads of 128): 8192 tokens in bf16, 32 + 4 heads 27.0 / 35.4, 64 + 4 53.9 / 63.9, 8 + 2
+    // 13.1 / 11.5; 2048 tokens of 32 + 4 9.0 / 10.7; 1184 8.0 / 6.6.  In f32, where a thread has twice the bytes
+    // in flight, the units reach 92 to 97% of the copy rate: 8192 tokens of 32 + 4 54.1 / 50.4, 44 + 2 71.9 /
+    // 64.7, 8 + 2 15.1 / 16.3; 2048 of 32 + 4 14.4 / 15.1.
     if (units && rows && q.heads && T_ >= 148 * 8) {
         RopeStream rs;
         rs.qb = (uint32_t)(q.heads * dim * sizeof(T));

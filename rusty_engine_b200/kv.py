@@ -262,8 +262,9 @@ class KVCache:
         self._like = {dt: torch.empty(0, dtype=dt, device=k.device) for dt in (torch.float32, torch.float16, torch.bfloat16)}
 
     def append(self, k, v, slots, *, rope: Optional[Rope] = None, positions=None, q=None, q_out=None, stream=None):
-        """Writes k and v [tokens, n_kv_heads, head_dim] at `slots` (int32, -1 skips).  With a
-        rope, k is turned by `positions` first, and so is q where given; returns the turned q."""
+        """Writes k and v [tokens, n_kv_heads, head_dim] at `slots` (int32, -1 skips); the tokens of one
+        block in one run of consecutive slots, as extend gives them.  With a rope, k is turned by
+        `positions` first, and so is q where given; returns the turned q."""
         if stream is not None:
             with _on(stream, k, v, slots, positions, q, q_out):
                 return self.append(k, v, slots, rope=rope, positions=positions, q=q, q_out=q_out)

@@ -232,7 +232,8 @@ class MoEStack:
     def open_cache(self, max_requests: int, n_blocks: int, block_size: int = 64, max_pos: int = 4096, code=None,
                    rope_cfg=None):
         """A paged 8-bit KV cache of n_blocks blocks per layer for up to max_requests requests of up
-        to max_pos tokens (rounded up to whole blocks), and the rotary plan (NeoX halves over the whole head by default)."""
+        to max_pos tokens (rounded up to whole blocks), and the rotary plan (NeoX halves over the
+        whole head by default)."""
         from . import kv
 
         g = self.g
